@@ -34,6 +34,8 @@ EXPORTS = (
     "dsb_backward_blend",
     "dsb_geometry_backward_views", "dsb_geometry_backward_views_stats",
     "dsb_forward_core", "dsb_image_loss_workspace_bytes", "dsb_image_loss_backward", "dsb_l1_loss_backward_u8", "dsb_adam_step",
+    "dsb_recurrence_workspace_bytes", "dsb_recurrence_checkpoint_bytes", "dsb_recurrence_forward", "dsb_recurrence_backward",
+    "dsb_recurrence_step", "dsb_dropout",
     "dsb_export_reference_lists",
     "dsb_stage_timing_enable", "dsb_stage_count", "dsb_stage_name", "dsb_stage_timing_read",
     "dsb_sort_pairs_static", "dsb_tile_marks_bytes", "dsb_forward", "dsb_take_device_status",
@@ -41,6 +43,8 @@ EXPORTS = (
     "dsb_debug_blend_forward_variant",
 )
 STATIC_SORT_MAX_ITEMS = 1 << 21
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # DSB_DTYPE_*
+GATE_FORMS = {"decay": 0, "logit": 1}                                # DSB_GATE_*
 
 
 class DsbCamera(C.Structure):
@@ -48,6 +52,13 @@ class DsbCamera(C.Structure):
                 ("scale_modifier", C.c_float), ("sh_degree", C.c_int32), ("max_sh_degree", C.c_int32),
                 ("matrices_transposed", C.c_int32), ("flags", C.c_int32), ("tile_row_band", C.c_int32),
                 ("viewmatrix", C.c_void_p), ("projmatrix", C.c_void_p), ("campos", C.c_void_p), ("bg", C.c_void_p)]
+
+
+class DsbRecurrence(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("sequences", C.c_int32), ("sequence_rows", C.c_int32), ("channels", C.c_int32),
+                ("gate_heads", C.c_int32), ("dtype", C.c_int32), ("gate_form", C.c_int32), ("coupled", C.c_int32),
+                ("reverse", C.c_int32), ("x_stride", C.c_int64), ("gate_stride", C.c_int64), ("offsets", C.c_void_p),
+                ("lengths", C.c_void_p)]
 
 
 class DsbError(RuntimeError):
@@ -89,7 +100,9 @@ def lib():
         l.dsb_stage_name.argtypes = [C.c_int32]
         l.dsb_stage_count.restype = C.c_int32
         l.dsb_stage_timing_enable.argtypes = [C.c_int32]
-        P, I32, I64, CAM = C.c_void_p, C.c_int32, C.c_int64, C.POINTER(DsbCamera)
+        P, I32, I64, CAM, REC = C.c_void_p, C.c_int32, C.c_int64, C.POINTER(DsbCamera), C.POINTER(DsbRecurrence)
+        for fn in (l.dsb_recurrence_workspace_bytes, l.dsb_recurrence_checkpoint_bytes):
+            fn.restype, fn.argtypes = C.c_int64, [REC]
         sig = {
             "dsb_preprocess": [CAM, I32] + [P] * 7 + [P] * 5 + [P],
             "dsb_plan_pairs": [CAM, I32, P, P, P, P, P, I64, C.POINTER(C.c_int64), P],
@@ -114,6 +127,10 @@ def lib():
             "dsb_image_loss_backward": [P, P, I32, I32, C.c_float, P, I64, P, P, P],
             "dsb_l1_loss_backward_u8": [P, P, I32, I32, P, P, P],
             "dsb_adam_step": [P, P, P, P, I64, C.c_double, C.c_double, C.c_double, C.c_double, I32, C.c_double, P],
+            "dsb_recurrence_forward": [REC, P, P, P, P, P, P, P, I64, P],
+            "dsb_recurrence_backward": [REC, P, P, P, P, P, I64, P, P, P, P, P, I64, P],
+            "dsb_recurrence_step": [REC, P, P, P, P, P],
+            "dsb_dropout": [P, P, P, I64, I64, I64, I64, I64, I32, C.c_double, C.c_uint64, C.c_uint64, P, P, P],
             "dsb_export_reference_lists": [P, I64, P, P, P, P],
             "dsb_forward": [CAM, I32] + [P] * 7 + [P] * 10 + [P, I64] + [P, I64] + [P, I64] + [P] * 4
                            + [C.POINTER(C.c_int64), C.POINTER(C.c_int64), C.POINTER(C.c_int32), P],

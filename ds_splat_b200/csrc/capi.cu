@@ -60,6 +60,11 @@ int finish_device_status_read(int value, cudaStream_t s) {
     const int rc = device_status_address(&word);
     if (rc != DSB_OK) return rc;
     DSB_CUDA_CHECK(cudaMemsetAsync(word, 0, sizeof(int), s));   // taken: the next report starts from a clean word
+    if (value == DSB_ERR_INVALID_ARGUMENT) {
+        set_error("an earlier call on this device was given sequence offsets or lengths out of order or range: its results "
+                  "are not valid");
+        return DSB_ERR_INVALID_ARGUMENT;
+    }
     set_error("a bounded device-side wait of an earlier call on this device expired (status %d): results of the calls "
               "enqueued since the last status check are not valid", value);
     return value == DSB_ERR_DEVICE_WAIT_EXPIRED ? DSB_ERR_DEVICE_WAIT_EXPIRED : DSB_ERR_CUDA;
@@ -725,6 +730,36 @@ int dsb_l1_loss_backward_u8(const float* image, const uint8_t* target, int32_t i
 int dsb_adam_step(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, int64_t count, double lr,
                   double beta1, double beta2, double eps, int32_t step, double grad_scale, void* stream) {
     return launch_adam(params, grads, exp_avg, exp_avg_sq, count, lr, beta1, beta2, eps, step, grad_scale, (cudaStream_t)stream);
+}
+
+int64_t dsb_recurrence_workspace_bytes(const DsbRecurrence* shape) { return shape ? recurrence_workspace_bytes(*shape) : 0; }
+int64_t dsb_recurrence_checkpoint_bytes(const DsbRecurrence* shape) { return shape ? recurrence_checkpoint_bytes(*shape) : 0; }
+
+int dsb_recurrence_forward(const DsbRecurrence* shape, const void* x, const void* gate, const float* state_in, void* h,
+                           float* state_out, float* checkpoints, void* workspace, int64_t workspace_bytes, void* stream) {
+    DSB_REQUIRE(shape, "recurrence: null shape");
+    return launch_recurrence_forward(*shape, x, gate, state_in, h, state_out, checkpoints, workspace, workspace_bytes,
+                                     (cudaStream_t)stream);
+}
+
+int dsb_recurrence_backward(const DsbRecurrence* shape, const void* x, const void* gate, const float* state_in,
+                            const float* checkpoints, const void* v_h, int64_t v_h_stride, const float* v_state_out, void* v_x,
+                            void* v_gate, float* v_state_in, void* workspace, int64_t workspace_bytes, void* stream) {
+    DSB_REQUIRE(shape, "recurrence: null shape");
+    return launch_recurrence_backward(*shape, x, gate, state_in, checkpoints, v_h, v_h_stride, v_state_out, v_x, v_gate,
+                                      v_state_in, workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
+int dsb_recurrence_step(const DsbRecurrence* shape, const void* x, const void* gate, float* state, void* h, void* stream) {
+    DSB_REQUIRE(shape, "recurrence: null shape");
+    return launch_recurrence_step(*shape, x, gate, state, h, (cudaStream_t)stream);
+}
+
+int dsb_dropout(const void* x, const void* residual, void* out, int64_t rows, int64_t cols, int64_t x_stride,
+                int64_t residual_stride, int64_t out_stride, int32_t dtype, double p, uint64_t seed, uint64_t step,
+                const int64_t* rng, int64_t* rng_used, void* stream) {
+    return launch_dropout(x, residual, out, rows, cols, x_stride, residual_stride, out_stride, dtype, p, seed, step, rng,
+                          rng_used, (cudaStream_t)stream);
 }
 
 int dsb_export_reference_lists(const uint64_t* sorted_pairs, int64_t k, const float* records, int64_t* keys, int32_t* ids,

@@ -248,4 +248,17 @@ int launch_image_loss(const float* image, const float* target, int H, int W, flo
 int launch_adam(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, int64_t count, double lr, double beta1,
                 double beta2, double eps, int step, double grad_scale, cudaStream_t s);
 
+int64_t recurrence_workspace_bytes(const DsbRecurrence& shape);
+int64_t recurrence_checkpoint_bytes(const DsbRecurrence& shape);
+int launch_recurrence_forward(const DsbRecurrence& shape, const void* x, const void* gate, const float* state_in, void* h,
+                              float* state_out, float* checkpoints, void* workspace, int64_t workspace_bytes, cudaStream_t s);
+int launch_recurrence_backward(const DsbRecurrence& shape, const void* x, const void* gate, const float* state_in,
+                               const float* checkpoints, const void* v_h, int64_t v_h_stride, const float* v_state_out,
+                               void* v_x, void* v_gate, float* v_state_in, void* workspace, int64_t workspace_bytes,
+                               cudaStream_t s);
+int launch_recurrence_step(const DsbRecurrence& shape, const void* x, const void* gate, float* state, void* h, cudaStream_t s);
+int launch_dropout(const void* x, const void* residual, void* out, int64_t rows, int64_t cols, int64_t x_stride,
+                   int64_t residual_stride, int64_t out_stride, int dtype, double p, uint64_t seed, uint64_t step,
+                   const int64_t* rng, int64_t* rng_used, cudaStream_t s);
+
 }  // namespace dsb

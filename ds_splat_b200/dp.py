@@ -186,6 +186,25 @@ class DensifyStats:
                            torch.zeros_like(self.grad_norm_sum))
 
 
+@dataclass(frozen=True)
+class SplatDropout:
+    """Dropout of whole splats in one training step: every opacity is zero with probability ``p`` and divided by 1 - p
+    otherwise, the same choice for all the views of the step (``sequence.dropout`` of the opacities with the generator's
+    pair (``seed``, ``step``); give every training step a ``step`` of its own).  A regulariser of training from few views.
+    Gradients are those with respect to the opacities before the dropout.  Divided opacities may exceed 1; the blend clamps
+    alpha as it always does.  Statistics kept by ``DensifyStats`` count a dropped splat's visibility and radius, with a
+    gradient of zero."""
+    p: float
+    seed: int
+    step: int = 0
+
+    def __post_init__(self):
+        if not 0.0 <= self.p <= 1.0:
+            raise ValueError(f"p must lie in [0, 1], got {self.p}")
+        if not (0 <= self.seed < 1 << 64 and 0 <= self.step < 1 << 64):
+            raise ValueError("seed and step must lie in [0, 2^64)")
+
+
 class _Lane:
     """Buffers of the per-view stages (pair list and its sort, image, transmittance, last contributor) and the stream
     they run on.  Lane 0 runs on the caller's stream; ``render_views`` adds lanes with streams of their own so that
@@ -234,6 +253,7 @@ class ViewRenderer:
         self.cov3d = torch.empty((n, 6), dtype=torch.float32, device=dev)
         self.plan_bytes = int(self.lib.dsb_plan_workspace_bytes_views(n, bv))
         self.plan_ws = torch.empty(self.plan_bytes, dtype=torch.uint8, device=dev)
+        self.dropped = None                  # opacities after dropout and their gradients: allocated when first needed
         self.view_streams = max(1, int(view_streams))   # lanes render_views spreads a batch's views over
         self.lanes = [_Lane()]
         self.last_k = 0
@@ -440,9 +460,15 @@ class ViewRenderer:
             g["opacities"].data_ptr(), g["scales"].data_ptr(), g["rotations"].data_ptr(), None, 1 if accumulate else 0,
             capi.stream_ptr()))
 
+    def _drop(self, x: torch.Tensor, out: torch.Tensor, dropout: SplatDropout, residual: Optional[torch.Tensor] = None):
+        capi = self._capi
+        capi.check(self.lib.dsb_dropout(
+            x.data_ptr(), capi.ptr(residual), out.data_ptr(), 1, self.n, self.n, self.n, self.n, capi.DTYPES[torch.float32],
+            float(dropout.p), int(dropout.seed), int(dropout.step), None, None, capi.stream_ptr()))
+
     @_on_own_device
     def render_views(self, cameras, image_grads, grads: GradientBuffer, accumulate: bool = False,
-                     stats: Optional[DensifyStats] = None):
+                     stats: Optional[DensifyStats] = None, dropout: Optional[SplatDropout] = None):
         """Forward + backward of ``cameras`` with the gradients of all of them summed into ``grads`` (added to its
         contents when ``accumulate``).  ``image_grads`` is a sequence of dL/dimage tensors or a callable
         ``(index, image) -> dL/dimage``; it is called under the stream its view runs on (``view_streams`` of them
@@ -450,9 +476,18 @@ class ViewRenderer:
         taken in batches of up to ``batch_views`` of one image size:
         one preprocess launch (with the tile layout of every view) and one plan (depth sorts, offset scans, a
         single read-back of the pair counts) for the batch, then per view the rest of the forward and the backward blend, then one per-splat backward for
-        the batch, which also updates ``stats`` (a ``DensifyStats``) when given."""
+        the batch, which also updates ``stats`` (a ``DensifyStats``) when given.  With ``dropout`` (a ``SplatDropout``)
+        the step renders what is left of the splats."""
         capi, lib, p = self._capi, self.lib, self.p
         g = grads.views
+        opacities, v_opacities = p["opacities"], g["opacities"]
+        if dropout is not None and len(cameras) > 0:
+            if self.dropped is None:
+                self.dropped = torch.empty((2, self.n), dtype=torch.float32, device=self.dev)
+            opacities, v_opacities = self.dropped
+            self._drop(p["opacities"], opacities, dropout)
+            if accumulate:
+                v_opacities.zero_()        # gathers this call's gradients alone; what `grads` holds is added at the end
         b0, first = 0, True
         self.last_ks = []          # pair count of every view of this call
         while b0 < len(cameras):
@@ -470,7 +505,7 @@ class ViewRenderer:
             nl = min(self.view_streams, nv)
             lanes = [self._lane(i) for i in range(nl)]
             capi.check(lib.dsb_preprocess_views(
-                cams, nv, self.n, p["means3d"].data_ptr(), p["shs"].data_ptr(), None, p["opacities"].data_ptr(),
+                cams, nv, self.n, p["means3d"].data_ptr(), p["shs"].data_ptr(), None, opacities.data_ptr(),
                 p["scales"].data_ptr(), p["rotations"].data_ptr(), None, ptrs([sl.records for sl in slots]),
                 ptrs([sl.radii for sl in slots]), ptrs([sl.tiles for sl in slots]), self.cov3d.data_ptr(),
                 ptrs([sl.depth_keys for sl in slots]), ptrs([self._marks(sl, *size) for sl in slots]),
@@ -509,7 +544,7 @@ class ViewRenderer:
                 cams, nv, self.n, p["means3d"].data_ptr(), p["scales"].data_ptr(), p["rotations"].data_ptr(),
                 self.cov3d.data_ptr(), ptrs([sl.records for sl in slots]), ptrs([sl.radii for sl in slots]),
                 ptrs([sl.grad_acc for sl in slots]), g["means3d"].data_ptr(), None, g["shs"].data_ptr(), None,
-                g["opacities"].data_ptr(), g["scales"].data_ptr(), g["rotations"].data_ptr(), None,
+                v_opacities.data_ptr(), g["scales"].data_ptr(), g["rotations"].data_ptr(), None,
                 1 if (accumulate or not first) else 0)
             if stats is None:
                 capi.check(lib.dsb_geometry_backward_views(*geo_args, capi.stream_ptr()))
@@ -520,6 +555,8 @@ class ViewRenderer:
                     stats.max_radius.data_ptr(), capi.stream_ptr()))
             first = False
             b0 = b1
+        if dropout is not None and len(cameras) > 0:
+            self._drop(v_opacities, g["opacities"], dropout, residual=g["opacities"] if accumulate else None)
 
 
 class ImageLoss:
@@ -766,25 +803,34 @@ def register_with_nccl(make_buffers, group=None, more_groups=()):
         return make_buffers(), None
 
 
+def _dropout_argument(dropout):
+    """Renderers of a caller's own need not know the argument to be used without dropout."""
+    return {} if dropout is None else {"dropout": dropout}
+
+
 def data_parallel_step(renderer: ViewRenderer, cameras: Sequence[CameraTensors], image_grads,
-                       grads: GradientBuffer, group=None, stats: Optional[DensifyStats] = None) -> None:
+                       grads: GradientBuffer, group=None, stats: Optional[DensifyStats] = None,
+                       dropout: Optional[SplatDropout] = None) -> None:
     """One step of the multi-view batch on this rank: forward + backward of each local camera (gradients
     summed into ``grads``), then the all-reduce.  ``cameras`` is this rank's shard; ``image_grads`` is the
-    matching sequence of dL/dimage tensors, or a callable ``(index, image) -> dL/dimage`` (the loss)."""
+    matching sequence of dL/dimage tensors, or a callable ``(index, image) -> dL/dimage`` (the loss).  ``dropout``: a
+    ``SplatDropout``, the same on every rank for a step that drops the same splats from all its cameras."""
     if len(cameras) == 0:
         grads.zero_()  # a rank without views still takes part in the collective
     else:
-        renderer.render_views(cameras, image_grads, grads, accumulate=False, stats=stats)
+        renderer.render_views(cameras, image_grads, grads, accumulate=False, stats=stats, **_dropout_argument(dropout))
     allreduce_gradients(grads, group)
 
 
 def training_step(renderer: ViewRenderer, cameras: Sequence[CameraTensors], image_grads, grads: GradientBuffer,
-                  optimizer: ShardedAdam, grad_scale: float = 1.0, stats: Optional[DensifyStats] = None) -> None:
+                  optimizer: ShardedAdam, grad_scale: float = 1.0, stats: Optional[DensifyStats] = None,
+                  dropout: Optional[SplatDropout] = None) -> None:
     """One whole training step on this rank: forward + backward of its cameras, then ``ShardedAdam.step`` (gradient
     reduce-scatter, Adam on the rank's slice, parameter all-gather).  The renderer must have been built on the views
-    of the optimizer's ``ParameterBuffer`` so that the next step renders the updated cloud."""
+    of the optimizer's ``ParameterBuffer`` so that the next step renders the updated cloud.  ``dropout``: as in
+    ``data_parallel_step``."""
     if len(cameras) == 0:
         grads.zero_()
     else:
-        renderer.render_views(cameras, image_grads, grads, accumulate=False, stats=stats)
+        renderer.render_views(cameras, image_grads, grads, accumulate=False, stats=stats, **_dropout_argument(dropout))
     optimizer.step(grads, grad_scale=grad_scale)

@@ -1,0 +1,293 @@
+"""Operators over sequences: the gated linear recurrence and counter-based dropout.
+
+``gated_recurrence`` runs, per channel,
+
+    f_t = gate_t (form="decay")  or  1 / (1 + exp(-gate_t)) (form="logit")
+    h_t = f_t h_{t-1} + x_t,     coupled:  h_t = f_t h_{t-1} + (1 - f_t) x_t
+
+over dense, padded or packed sequences, with gradients.  The rasterizer's blend is its coupled form, run from the back of a
+depth-ordered list to its front with the gate 1 - alpha shared by the colour channels; here the lists may hold any number
+of channels and come from anywhere:
+
+    # samples [N, C] of all rays, front to back, ray r in rows offsets[r] .. offsets[r + 1]
+    _, pixels = gated_recurrence(samples, 1 - alphas[:, None], offsets=offsets, form="decay", coupled=True, reverse=True,
+                                 final_only=True)
+
+``gated_recurrence_step`` takes one new row per sequence and updates the state in place.  ``dropout`` draws its mask from
+(seed, step, element index) and never stores it; ``dp.ViewRenderer.render_views`` drops splats with it.
+
+The reference has no counterpart of these.  Tensors are float32, float16 or bfloat16 on one CUDA device; states, sums and
+all arithmetic are float32, rounded once to the tensors' type.  Work is enqueued on the current stream of the inputs'
+device.  There is no fallback for other devices.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes as C
+from typing import Optional, Tuple, Union
+
+import torch
+
+from . import _capi
+
+
+def _on(device):
+    """Context with ``device`` current (the library launches on the current device)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _require(t, name, device=None, dtype=None):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if device is not None and t.device != device:
+        raise RuntimeError(f"{name} is on {t.device}, expected {device}")
+    if dtype is not None and t.dtype != dtype:
+        raise RuntimeError(f"{name} must be {dtype}, got {t.dtype}")
+
+
+def _rows(t: torch.Tensor, lanes: int):
+    """(tensor, elements between rows): ``t`` as rows of its last dimension, as it is where one stride leads from row to row
+    and, for loads of ``lanes`` elements, the rows start on such boundaries; a contiguous copy otherwise."""
+    width = t.shape[-1]
+    stride, rows = width, 1
+    plain = t.stride(-1) == 1 or width == 1
+    for size, step in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        if rows == 1:
+            stride = step
+        elif step != stride * rows:
+            plain = False
+        rows *= size
+    if plain and (lanes == 1 or (stride % lanes == 0 and t.data_ptr() % (lanes * t.element_size()) == 0)):
+        return t, stride
+    return t.clone(memory_format=torch.contiguous_format), width
+
+
+def _state(t: Optional[torch.Tensor], shape, device, name):
+    if t is None:
+        return None
+    _require(t, name, device, torch.float32)
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have the shape {list(shape)}, got {list(t.shape)}")
+    return _rows(t, 4 if shape[-1] % 4 == 0 else 1)[0].contiguous()
+
+
+def _describe(x, gate, sequences, sequence_rows, form, coupled, reverse, offsets, lengths):
+    """The call's DsbRecurrence and the tensors it points into."""
+    d, heads = x.shape[-1], gate.shape[-1]
+    lanes = 4 if (d // heads if heads != d else d) % 4 == 0 else 1
+    x, x_stride = _rows(x, lanes)
+    gate, gate_stride = _rows(gate, lanes if heads == d else 1)
+    shape = _capi.DsbRecurrence(x.numel() // d, sequences, sequence_rows, d, heads, _capi.DTYPES[x.dtype], _capi.GATE_FORMS[form],
+                                1 if coupled else 0, 1 if reverse else 0, x_stride, gate_stride, _capi.ptr(offsets),
+                                _capi.ptr(lengths))
+    return shape, x, gate, lanes
+
+
+def _check_gate(x, gate, form):
+    _require(x, "x")
+    if x.dtype not in _capi.DTYPES:
+        raise RuntimeError(f"x must be float32, float16 or bfloat16, got {x.dtype}")
+    _require(gate, "gate", x.device, x.dtype)
+    if form not in _capi.GATE_FORMS:
+        raise ValueError(f"form must be 'decay' or 'logit', got {form!r}")
+    if gate.dim() != x.dim() or gate.shape[:-1] != x.shape[:-1]:
+        raise ValueError(f"gate must have one row per row of x: {list(gate.shape)} against {list(x.shape)}")
+    d, heads = x.shape[-1], gate.shape[-1]
+    if d < 1 or heads < 1 or d % heads != 0:
+        raise ValueError(f"{d} channels do not split into {heads} gate heads")
+
+
+class _GatedRecurrence(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, state, offsets, lengths, form, coupled, reverse, final_only):
+        lib = _capi.lib()
+        dev, lead, d = x.device, x.shape[:-1], x.shape[-1]
+        sequences = offsets.numel() - 1 if offsets is not None else x.shape[0]
+        sequence_rows = 0 if offsets is not None else x.shape[1]
+        state = _state(state, (sequences, d), dev, "state")
+        with _on(dev):
+            shape, x, gate, _ = _describe(x, gate, sequences, sequence_rows, form, coupled, reverse, offsets, lengths)
+            keep = any(ctx.needs_input_grad[:3])
+            h = None if final_only else torch.empty((*lead, d), dtype=x.dtype, device=dev)
+            last = torch.empty((sequences, d), dtype=torch.float32, device=dev)
+            checkpoints = None
+            if keep:
+                checkpoints = torch.empty(int(lib.dsb_recurrence_checkpoint_bytes(C.byref(shape))), dtype=torch.uint8, device=dev)
+            nbytes = int(lib.dsb_recurrence_workspace_bytes(C.byref(shape)))
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+            _capi.check(lib.dsb_recurrence_forward(
+                C.byref(shape), x.data_ptr(), gate.data_ptr(), _capi.ptr(state), _capi.ptr(h), last.data_ptr(),
+                _capi.ptr(checkpoints), _capi.ptr(workspace), nbytes, _capi.stream_ptr()))
+        ctx.call = (sequences, sequence_rows, form, coupled, reverse)
+        if keep:
+            ctx.save_for_backward(x, gate, state, checkpoints, offsets, lengths)
+        ctx.set_materialize_grads(False)
+        return last if final_only else (h, last)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        lib = _capi.lib()
+        x, gate, state, checkpoints, offsets, lengths = ctx.saved_tensors
+        v_h, v_last = (None, grads[0]) if len(grads) == 1 else grads
+        if v_h is None and v_last is None:
+            return (None,) * 9
+        sequences, sequence_rows, form, coupled, reverse = ctx.call
+        dev, d = x.device, x.shape[-1]
+        need = ctx.needs_input_grad
+        with _on(dev):
+            shape, x, gate, lanes = _describe(x, gate, sequences, sequence_rows, form, coupled, reverse, offsets, lengths)
+            v_h, v_h_stride = _rows(v_h, lanes) if v_h is not None else (None, d)
+            v_last = _state(v_last, (sequences, d), dev, "the last state's gradient")
+            v_x = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
+            v_gate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if need[1] else None
+            v_state = torch.empty((sequences, d), dtype=torch.float32, device=dev) if need[2] else None
+            nbytes = int(lib.dsb_recurrence_workspace_bytes(C.byref(shape)))
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+            _capi.check(lib.dsb_recurrence_backward(
+                C.byref(shape), x.data_ptr(), gate.data_ptr(), _capi.ptr(state), _capi.ptr(checkpoints), _capi.ptr(v_h), v_h_stride,
+                _capi.ptr(v_last), _capi.ptr(v_x), _capi.ptr(v_gate), _capi.ptr(v_state), _capi.ptr(workspace), nbytes,
+                _capi.stream_ptr()))
+        return v_x, v_gate, v_state, None, None, None, None, None, None
+
+
+def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, state: Optional[torch.Tensor] = None, *,
+                     offsets: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None, form: str = "logit",
+                     coupled: bool = False, reverse: bool = False,
+                     final_only: bool = False) -> Tuple[Optional[torch.Tensor], torch.Tensor]:
+    """Runs the recurrence over every sequence and returns ``(h, last)``: all states, in the type of ``x``, and each
+    sequence's last state, float32.  Differentiable in ``x``, ``gate`` and ``state``.
+
+    x        [B, T, D]: B sequences of T rows; with ``lengths`` (int32 [B]) only the first ``lengths[b]`` of them belong to
+             sequence b.  [N, D] with ``offsets`` (int32 [S + 1], nondecreasing, within [0, N]): sequence s is rows
+             ``offsets[s] .. offsets[s + 1]`` (a tile's ``ranges`` of the rasterizer are such offsets).  At most 2^31 - 1 rows.
+    gate     x's shape with H for D: each of the H gates of a row is shared by D / H consecutive channels.  As logits
+             (``form="logit"``) decays near 1 keep their precision in 16-bit types; as ``"decay"`` they are taken as they
+             are and are meant to lie in [-1, 1].
+    state    float32 [S, D], each sequence's state before its first row; None = zeros.
+    reverse  run from each sequence's last row to its first (``last`` is then the state after the first row).
+    final_only  return ``(None, last)`` and do not write ``h``.
+
+    Rows that belong to no sequence come back as zeros, their gradients too; a sequence of no rows hands its state on.
+    Offsets and lengths live on the device and are not read back: values out of order or range make the results invalid and
+    are reported by ``dsb_take_device_status`` and by the rasterizer's calls that synchronise."""
+    _check_gate(x, gate, form)
+    if offsets is not None:
+        if lengths is not None:
+            raise ValueError("give offsets (packed rows) or lengths (padded rows), not both")
+        if x.dim() != 2:
+            raise ValueError(f"packed x must be [N, D], got {list(x.shape)}")
+        _require(offsets, "offsets", x.device, torch.int32)
+        if offsets.dim() != 1 or offsets.numel() < 1:
+            raise ValueError("offsets must be one-dimensional with one entry more than there are sequences")
+        offsets = offsets.contiguous()
+    else:
+        if x.dim() != 3:
+            raise ValueError(f"x must be [B, T, D] (or [N, D] with offsets), got {list(x.shape)}")
+        if lengths is not None:
+            _require(lengths, "lengths", x.device, torch.int32)
+            if tuple(lengths.shape) != (x.shape[0],):
+                raise ValueError(f"lengths must have one entry per sequence: {list(lengths.shape)} against {x.shape[0]}")
+            lengths = lengths.contiguous()
+    out = _GatedRecurrence.apply(x, gate, state, offsets, lengths, form, bool(coupled), bool(reverse), bool(final_only))
+    return (None, out) if final_only else out
+
+
+def gated_recurrence_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, *, form: str = "logit",
+                          coupled: bool = False) -> torch.Tensor:
+    """One row of every sequence: x [S, D], gate [S, H], ``state`` (float32 [S, D], contiguous) updated in place; returns
+    the new states in the type of ``x``.  For generating token by token; it keeps nothing for a backward pass."""
+    _check_gate(x, gate, form)
+    if x.dim() != 2:
+        raise ValueError(f"x must be [S, D], got {list(x.shape)}")
+    _require(state, "state", x.device, torch.float32)
+    if state.shape != x.shape:
+        raise ValueError(f"state must have the shape {list(x.shape)}, got {list(state.shape)}")
+    if not state.is_contiguous():
+        raise ValueError("state is updated in place and must be contiguous")
+    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or state.requires_grad):
+        raise RuntimeError("gated_recurrence_step has no backward pass: use gated_recurrence, or torch.no_grad()")
+    with _on(x.device):
+        shape, x, gate, _ = _describe(x, gate, x.shape[0], 0, form, coupled, False, None, None)
+        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        if h.numel():
+            _capi.check(_capi.lib().dsb_recurrence_step(C.byref(shape), x.data_ptr(), gate.data_ptr(), state.data_ptr(),
+                                                        h.data_ptr(), _capi.stream_ptr()))
+            torch.autograd.graph.increment_version(state)
+    return h
+
+
+def _launch_dropout(x, residual, p, seed, step, rng, rng_used):
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if out.numel() == 0:
+        return out
+    if x.is_contiguous() and (residual is None or residual.is_contiguous()):
+        cols = x_stride = residual_stride = x.numel()
+    else:
+        x, x_stride = _rows(x, 1)
+        cols = residual_stride = x.shape[-1]
+        if residual is not None:
+            residual, residual_stride = _rows(residual, 1)
+    _capi.check(_capi.lib().dsb_dropout(
+        x.data_ptr(), _capi.ptr(residual), out.data_ptr(), out.numel() // cols, cols, x_stride, residual_stride, cols,
+        _capi.DTYPES[x.dtype], p, seed, step, _capi.ptr(rng), _capi.ptr(rng_used), _capi.stream_ptr()))
+    return out
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, seed, step, rng):
+        with _on(x.device):
+            used = torch.empty(2, dtype=torch.int64, device=x.device) if rng is not None else None
+            out = _launch_dropout(x, residual, p, seed, step, rng, used)
+        ctx.call = (p, seed, step)
+        ctx.save_for_backward(used)     # the pair as it was: the caller may advance rng before the backward pass
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, v_out):
+        used, = ctx.saved_tensors
+        p, seed, step = ctx.call
+        v_x = None
+        if ctx.needs_input_grad[0]:
+            with _on(v_out.device):
+                v_x = _launch_dropout(v_out, None, p, seed, step, used, None)
+        return v_x, (v_out if ctx.needs_input_grad[1] else None), None, None, None, None
+
+
+def dropout(x: torch.Tensor, p: float, rng: Union[Tuple[int, int], torch.Tensor], *,
+            residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``[residual +] (keep ? x / (1 - p) : 0)`` with ``keep`` drawn per element with probability 1 - p from a counter-based
+    generator: word i mod 4 of Philox4x32-10 with the key ``seed`` and the counter (i div 4, ``step``), i the element's
+    row-major index, at least ``round(p 2^32)``.  The mask depends on nothing else and is drawn again in the backward pass.
+
+    rng  the pair (seed, step), each within [0, 2^64): one seed per place in a model, one step per training step.  Or an
+         int64 CUDA tensor of two elements holding them, read when the kernel runs: a captured graph draws a new mask at
+         every replay when the tensor is advanced between (or inside) the replays.
+    residual  a tensor of x's shape and type to add.
+
+    Dropped elements leave no trace of what they held; p = 1 drops everything."""
+    _require(x, "x")
+    if x.dtype not in _capi.DTYPES:
+        raise RuntimeError(f"x must be float32, float16 or bfloat16, got {x.dtype}")
+    if residual is not None:
+        _require(residual, "residual", x.device, x.dtype)
+        if residual.shape != x.shape:
+            raise ValueError(f"residual must have the shape of x: {list(residual.shape)} against {list(x.shape)}")
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"p must lie in [0, 1], got {p}")
+    if isinstance(rng, torch.Tensor):
+        _require(rng, "rng", x.device, torch.int64)
+        if rng.numel() != 2 or not rng.is_contiguous():
+            raise ValueError("rng must hold two elements, (seed, step)")
+        return _Dropout.apply(x, residual, p, 0, 0, rng)
+    seed, step = (int(v) for v in rng)
+    if not (0 <= seed < 1 << 64 and 0 <= step < 1 << 64):
+        raise ValueError("seed and step must lie in [0, 2^64)")
+    return _Dropout.apply(x, residual, p, seed, step, None)

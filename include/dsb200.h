@@ -462,6 +462,70 @@ int dsb_l1_loss_backward_u8(const float* image, const uint8_t* target, int32_t i
 int dsb_adam_step(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, int64_t count, double lr,
                   double beta1, double beta2, double eps, int32_t step, double grad_scale, void* stream);
 
+/* ---- sequence operators -----------------------------------------------------------------------------
+ * No reference counterparts.  Storage types of their tensors; all arithmetic, states and sums are in 32 bits. */
+#define DSB_DTYPE_F32 0
+#define DSB_DTYPE_F16 1
+#define DSB_DTYPE_BF16 2
+
+/* Gated linear recurrence over depth-ordered lists or any other sequences, per channel:
+ *     f_t = gate_t (DSB_GATE_DECAY) or 1 / (1 + exp(-gate_t)) (DSB_GATE_LOGIT)
+ *     h_t = f_t h_{t-1} + x_t,   or with `coupled`   h_t = f_t h_{t-1} + (1 - f_t) x_t
+ * from h_{-1} = state_in (zeros when NULL) to state_out = the last h, over each of `sequences` sequences.  The blend of
+ * dsb_blend_forward is the coupled form run back to front (`reverse`) with gate 1 - alpha shared by the colour
+ * channels; this entry takes any number of channels and any lists, a tile's `ranges` among them.
+ *
+ * Rows: x and h are [rows][channels], gate is [rows][gate_heads]; each head's gate is shared by channels / gate_heads
+ * consecutive channels.  Rows are x_stride / gate_stride elements apart; h and the gradients are contiguous.
+ *   sequence_rows > 0: sequence s is rows s * sequence_rows ..., rows == sequences * sequence_rows; with `lengths`
+ *                      (int32 per sequence on the device) only its first lengths[s] rows belong to it.
+ *   sequence_rows == 0: packed; sequence s is rows [offsets[s], offsets[s+1]) (int32 on the device, nondecreasing,
+ *                      within [0, rows]).
+ * Rows that belong to no sequence are written as zeros, in h and in the gradients, and nothing in them reaches a result.
+ * A sequence of no rows hands its state on.  Offsets or lengths out of order or range keep every access in bounds and
+ * are reported through the device status word (DSB_ERR_INVALID_ARGUMENT); the results are then not valid.
+ * States and their gradients are float [sequences][channels].  Decays are meant to lie in [-1, 1]: the scan forms
+ * products of a sequence's decays, which overflow where the sequence itself would not if many of them are larger.
+ *
+ * checkpoints (dsb_recurrence_checkpoint_bytes; NULL when no backward follows) receives the states between the pieces
+ * a sequence is cut into, which the backward starts from; nothing else is kept.  workspace:
+ * dsb_recurrence_workspace_bytes, for either direction, free again when the call's work is done.
+ * Results do not depend on timing: the same call gives the same bits. */
+#define DSB_GATE_DECAY 0
+#define DSB_GATE_LOGIT 1
+typedef struct DsbRecurrence {
+    int64_t rows;
+    int32_t sequences, sequence_rows;
+    int32_t channels, gate_heads;
+    int32_t dtype, gate_form, coupled, reverse;
+    int64_t x_stride, gate_stride;
+    const int32_t* offsets; /* device, [sequences + 1]; packed only */
+    const int32_t* lengths; /* device, [sequences]; NULL = all sequence_rows */
+} DsbRecurrence;
+int64_t dsb_recurrence_workspace_bytes(const DsbRecurrence* shape);
+int64_t dsb_recurrence_checkpoint_bytes(const DsbRecurrence* shape);
+int dsb_recurrence_forward(const DsbRecurrence* shape, const void* x, const void* gate, const float* state_in /* may be NULL */,
+                           void* h /* NULL: only the state is wanted */, float* state_out,
+                           float* checkpoints /* may be NULL */, void* workspace, int64_t workspace_bytes, void* stream);
+/* v_h (rows v_h_stride elements apart) or v_state_out may be NULL (zero); of the results v_x, v_gate and v_state_in
+ * those that are NULL are not wanted.  v_gate sums over the channels that share a gate, in a fixed order. */
+int dsb_recurrence_backward(const DsbRecurrence* shape, const void* x, const void* gate, const float* state_in /* as forward */,
+                            const float* checkpoints, const void* v_h, int64_t v_h_stride, const float* v_state_out,
+                            void* v_x, void* v_gate, float* v_state_in, void* workspace, int64_t workspace_bytes, void* stream);
+/* The same for one new row of every sequence: x [sequences][channels], gate [sequences][gate_heads], state updated in
+ * place, h contiguous.  Of `shape`, rows == sequences; offsets, lengths, sequence_rows and reverse are not looked at. */
+int dsb_recurrence_step(const DsbRecurrence* shape, const void* x, const void* gate, float* state, void* h, void* stream);
+
+/* Dropout from a counter-based generator; the mask is not stored, the backward is the same call on the gradient:
+ *     out_i = [residual_i +] (word_i >= round(p * 2^32) ? x_i / (1 - p) : 0)
+ * with word_i = word (i mod 4) of Philox4x32-10 under the key `seed` and the counter (i div 4, step), i = row * cols +
+ * col.  residual may be NULL; out may be x or residual.  rng: NULL, or two int64 on the device (seed, step) that
+ * replace the arguments, so that a captured graph draws a new mask when they change; rng_used (may be NULL) then
+ * receives the pair that was used. */
+int dsb_dropout(const void* x, const void* residual, void* out, int64_t rows, int64_t cols, int64_t x_stride,
+                int64_t residual_stride, int64_t out_stride, int32_t dtype, double p, uint64_t seed, uint64_t step,
+                const int64_t* rng, int64_t* rng_used, void* stream);
+
 /* Test/export helper: rebuild the reference-format sorted lists from this library's packed pairs:
  * keys[i] = (tile << 32) | sign-extended depth bits of the splat, ids[i] = splat id
  * (the layout cpp/rasterizer_kernels.cu:283,299-301 produces and thrust sorts). */
