@@ -7,14 +7,20 @@
 //
 // A stretch of rows maps the state before it to the state after it as h -> a h + b, and two stretches compose as
 // (a2 a1, a2 b1 + b2); a stretch in which a sequence begins maps every h to b ("closed": its a is never looked at, so
-// that an infinity of the sequence before cannot meet a zero).  Rows are cut into chunks of a tile's rows, channels into
-// blocks; a tile's thread runs L consecutive rows of V channels, the warp composes its threads' maps, the block its warps'.
-//   1. aggregate: every tile's map
-//   2. carry:     one thread per sequence chain and channel walks the chunks' maps and leaves the state before each chunk
-//   3. apply:     every tile again, now with the state it starts from
-// The backward runs the same three steps from the last row to the first on q, and recomputes h inside a tile from the
-// state its chunk starts with (a checkpoint of the forward), in 32 bits: the h that was written out is rounded to the
-// storage type and need not be kept.
+// that an infinity of the sequence before cannot meet a zero).
+//
+// A block walks along one stretch of rows and a block of channels, tile by tile, and carries the state in registers: it
+// reads everything once and writes everything once.  Inside a tile a thread runs L consecutive rows of V channels, a warp
+// composes its threads' maps with shuffles, the block its warps' through shared memory (one barrier a tile); the next
+// tile's rows are on their way into shared memory meanwhile (each thread copies what it will read itself, so their arrival
+// needs no barrier).  Where sequences and channels alone make too few blocks for the GPU, a sequence is cut into segments:
+// a first launch leaves every segment's map, and each block of the second starts from the composition of those before it.
+// That reads the inputs twice, the second time mostly from L2 where the call is small enough to need it.
+//
+// The backward walks from the last row to the first on q, and recomputes h inside a tile from the state the tile starts
+// with (a checkpoint of the forward), in 32 bits: the h that was written out is rounded to the storage type and need not
+// be kept.  Every order of composition is fixed by the shape alone, so results do not depend on timing; no block waits for
+// another.
 #include <type_traits>
 
 #include "vector_io.cuh"
@@ -23,9 +29,11 @@ namespace dsb {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr long long kMaxRows = (1ll << 31) - 1;
+constexpr int kStages = 2;
+constexpr int kTables = 3;      // one is read, one was read by the slowest warp, one is written
 
 struct Layout {            // how a call is cut; the same for the forward and the backward of one shape
     int vec;               // channels per thread: 4 or 1
@@ -33,8 +41,10 @@ struct Layout {            // how a call is cut; the same for the forward and th
     int per_head;          // channels that share a gate; all of them when every channel has its own
     int heads;             // 1 when every channel has its own gate
     int parts;             // channel blocks per head
-    bool table;            // chunks may hold sequence borders: one chain over all rows; else one chain per sequence
-    long long chains, chain_rows;
+    bool table;            // tiles may hold sequence borders: one chain over all rows; else one chain per sequence
+    int tile_rows;
+    long long chains, chain_rows, tiles;   // tiles of a chain
+    long long segments, segment_tiles;     // of a chain
 };
 
 struct Args {
@@ -42,17 +52,16 @@ struct Args {
     void *h, *v_x, *v_gate;
     const float *state_in, *v_state_out;
     float *state_out, *v_state_in;
-    float* checkpoints;
-    float *map_a, *map_b;  // [chains][chunks][channels]; map_a becomes the state before each chunk
-    int* map_closed;       // [chains][chunks]
+    float* checkpoints;    // [chains][tiles][channels]: the state before each tile
+    float *map_a, *map_b;  // [chains][segments][channels]
+    int* map_closed;       // [chains][segments]
     float* gate_parts;     // [parts][rows][heads], when a head spans several channel blocks
     const int *offsets, *lengths;
     int* device_status;
     long long rows, chain_rows, chains;
     long long x_stride, gate_stride, v_h_stride;   // negative when the scan runs from the last row to the first
     long long h_stride, gate_out_stride;           // channels / heads of contiguous results, with the same sign
-    long long chunks, checkpoint_chunks;
-    int checkpoint_rows;
+    long long tiles, segments, segment_tiles;
     int sequences, sequence_rows, channels, gate_heads, heads, per_head, parts, lg_tx;
     int logit, coupled, reverse, shared;
 };
@@ -62,34 +71,42 @@ struct Args {
 // m = exp(-|g|) / (1 + exp(-|g|)) <= 1/2, with the sign saying which one it is.
 __device__ __forceinline__ float encode_gate(float g, int logit) {
     if (!logit) return g;
-    const float y = -fabsf(g);
-    // exp(y) = 2^(y log2 e): the product's rounding error and the constant's own are added back to first order
+    float y, r;
+    asm("max.NaN.f32 %0, %1, 0fC2B40000;" : "=f"(y) : "f"(-fabsf(g)));   // -90: exp is 0 beside 1 long before; NaN stays NaN
+    // exp(y) = 2^(y log2 e), the product's rounding error added back to first order
     const float hi = y * 1.44269502f;
-    const float lo = fmaf(y, 1.92596303e-8f, fmaf(y, 1.44269502f, -hi));
+    const float lo = fmaf(y, 1.44269502f, -hi);
     float t = exp2f(hi);
-    t = y < -80.f ? t : fmaf(t, lo * 0.693147181f, t);   // beyond, t is 0 beside 1 (and lo is NaN at infinity)
-    const float d = 1.f + t;
-    float r = __fdividef(1.f, d);
-    r = fmaf(r, fmaf(-d, r, 1.f), r);                     // one Newton step: 1 / d to rounding
+    t = fmaf(t, lo * 0.693147181f, t);
+    t = y <= -90.f ? 0.f : t;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + t));
     return copysignf(t * r, g);
 }
-__device__ __forceinline__ float gate_f(float m, int logit) {
-    return logit ? (signbit(m) ? -m : 1.f - m) : m;
-}
-__device__ __forceinline__ float gate_k(float m, int logit) {   // 1 - f
-    return logit ? (signbit(m) ? 1.f + m : m) : 1.f - m;
+__device__ __forceinline__ void decode_gate(float m, int logit, float& f, float& k) {
+    const float rest = 1.f - (logit ? fabsf(m) : m);
+    const bool small_f = logit ? __float_as_int(m) < 0 : true;   // a decay is f itself
+    const float own = logit ? fabsf(m) : m;
+    f = small_f ? own : rest;
+    k = small_f ? rest : own;
 }
 
-// ---- which rows begin and end sequences ------------------------------------------------------------------------------
+// ---- rows that begin and end sequences ------------------------------------------------------------------------------
+// In the order of the scan: position p is row p, or rows - 1 - p when the scan runs backwards; sequence k of the scan is
+// the tensor's sequence k, or sequences - 1 - k.
 constexpr int kNone = -1, kOutside = -2;
 
-struct ChainRows {         // without a table: the chain is one sequence
+__device__ __forceinline__ int sequence_id(const Args& a, int k) { return a.reverse ? a.sequences - 1 - k : k; }
+// Where the scan's packed sequence k begins (k = sequences: where the last one ends).
+__device__ __forceinline__ long long packed_start(const Args& a, long long k) {
+    return a.reverse ? a.rows - a.offsets[a.sequences - k] : a.offsets[k];
+}
+struct ChainRows {         // without a table: the chain is one sequence, and holds positions [lo, hi)
     int sequence;
-    long long lo, hi;      // the positions that belong to it
+    long long lo, hi;
 };
 __device__ __forceinline__ ChainRows chain_rows_of(const Args& a, int chain) {
     ChainRows c;
-    c.sequence = a.reverse ? a.sequences - 1 - chain : chain;
+    c.sequence = sequence_id(a, chain);
     long long len = a.sequence_rows;
     if (a.lengths) len = min(max(a.lengths[c.sequence], 0), a.sequence_rows);
     c.lo = a.reverse ? a.sequence_rows - len : 0;
@@ -97,14 +114,14 @@ __device__ __forceinline__ ChainRows chain_rows_of(const Args& a, int chain) {
     return c;
 }
 
-// How many of offsets[0 .. n) are <= row; called by one whole warp.
-__device__ __forceinline__ int count_not_above(const int* offsets, int n, long long row) {
+// How many of the scan's packed sequences k begin at or before p; called by one whole warp.
+__device__ __forceinline__ int begun_by(const Args& a, long long p) {
     const int lane = threadIdx.x & 31;
-    int lo = 0, len = n;
+    int lo = 0, len = a.sequences;
     while (len > 0) {
         const int step = (len + 31) / 32;
         const long long at = (long long)lane * step;
-        const bool below = at < len && offsets[lo + at] <= row;
+        const bool below = at < len && packed_start(a, lo + at) <= p;
         const int below_count = __popc(__ballot_sync(0xffffffffu, below));
         if (below_count == 0) break;
         const int skip = (below_count - 1) * step + 1;
@@ -114,56 +131,55 @@ __device__ __forceinline__ int count_not_above(const int* offsets, int n, long l
     return lo;
 }
 
-// first[r] / end[r]: the sequence that begins / ends at position p0 + r, kNone, or (first only) kOutside.
-__device__ void fill_row_table(const Args& a, long long p0, int tile_rows, int* first, int* end, int* s_seq) {
+// first[r] / end[r]: the sequence that begins / ends at position p0 + r, kNone, or (first only) kOutside.  A tile is plain
+// when all its rows belong to a sequence that neither begins nor ends there.  Tables are made for one tile while the one
+// before it is worked on; the block's next barrier publishes them.  `cursor` is the scan's sequence to begin looking at (the
+// last to begin at or before p0); in shared memory, kept by this function from tile to tile.
+struct RowTable {
+    int* first;
+    int* end;
+};
+__device__ void fill_row_table(const Args& a, long long p0, int tile_rows, RowTable t) {
     const int tid = threadIdx.x;
     if (a.sequence_rows > 0) {
         for (int r = tid; r < tile_rows; r += kThreads) {
             const long long p = p0 + r;
             int f = kOutside, e = kNone;
             if (p < a.rows) {
-                const int turn = (int)(p / a.sequence_rows), t = (int)(p - (long long)turn * a.sequence_rows);
-                const int seq = a.reverse ? a.sequences - 1 - turn : turn;
+                const int turn = (int)(p / a.sequence_rows), pos = (int)(p - (long long)turn * a.sequence_rows);
+                const int seq = sequence_id(a, turn);
                 const int len = a.lengths ? min(max(a.lengths[seq], 0), a.sequence_rows) : a.sequence_rows;
                 const int lo = a.reverse ? a.sequence_rows - len : 0;
-                if (t >= lo && t < lo + len) {
-                    f = t == lo ? seq : kNone;
-                    e = t == lo + len - 1 ? seq : kNone;
+                if (pos >= lo && pos < lo + len) {
+                    f = pos == lo ? seq : kNone;
+                    e = pos == lo + len - 1 ? seq : kNone;
                 }
             }
-            first[r] = f;
-            end[r] = e;
+            t.first[r] = f;
+            t.end[r] = e;
         }
-    } else {
-        const long long p1 = min(p0 + tile_rows, a.rows);
-        const long long row0 = a.reverse ? a.rows - p1 : p0, row1 = a.reverse ? a.rows - p0 : p1;
-        const long long all0 = a.offsets[0], all1 = a.offsets[a.sequences];
-        for (int r = tid; r < tile_rows; r += kThreads) {
-            const long long p = p0 + r, row = a.reverse ? a.rows - 1 - p : p;
-            first[r] = p < p1 && row >= all0 && row < all1 ? kNone : kOutside;
-            end[r] = kNone;
-        }
-        if (tid < 32) {
-            const int n = count_not_above(a.offsets, a.sequences, row0);
-            if (tid == 0) *s_seq = max(n - 1, 0);
-        }
-        __syncthreads();
-        for (int s = *s_seq + tid; s < a.sequences; s += kThreads) {
-            const long long o0 = a.offsets[s], o1 = a.offsets[s + 1];
-            if (o0 >= row1) break;
-            if (o0 >= o1) continue;
-            const long long front = a.reverse ? o1 - 1 : o0, back = a.reverse ? o0 : o1 - 1;
-            if (front >= row0 && front < row1) {
-                const int r = (int)(a.reverse ? row1 - 1 - front : front - row0);
-                first[r] = s;
-            }
-            if (back >= row0 && back < row1) {
-                const int r = (int)(a.reverse ? row1 - 1 - back : back - row0);
-                end[r] = s;
-            }
-        }
+        return;
     }
+    const long long p1 = min(p0 + tile_rows, a.rows);
+    const long long all0 = packed_start(a, 0), all1 = packed_start(a, a.sequences);
+    for (int r = tid; r < tile_rows; r += kThreads) {
+        const long long p = p0 + r;
+        t.first[r] = p < p1 && p >= all0 && p < all1 ? kNone : kOutside;
+        t.end[r] = kNone;
+    }
+    int k0 = 0;
+    if (tid < 32) k0 = max(begun_by(a, p0) - 1, 0);
+    __shared__ int s_k0;
+    if (tid == 0) s_k0 = k0;
     __syncthreads();
+    for (long long k = s_k0 + tid; k < a.sequences; k += kThreads) {
+        const long long o0 = packed_start(a, k), o1 = packed_start(a, k + 1);
+        if (o0 >= p1) break;
+        if (o0 >= o1) continue;
+        const int id = sequence_id(a, (int)k);
+        if (o0 >= p0) t.first[o0 - p0] = id;
+        if (o1 > p0 && o1 <= p1) t.end[o1 - 1 - p0] = id;
+    }
 }
 
 // Sequences without rows hand their state on; offsets and lengths out of order or range are reported.
@@ -202,10 +218,13 @@ __device__ __forceinline__ void identity(Map<V>& m) {
 // m <- m after e (e comes first along the scan)
 template <int V>
 __device__ __forceinline__ void compose_after(Map<V>& m, const Map<V>& e) {
-    if (m.closed) return;
+    const bool open = !m.closed;
 #pragma unroll
-    for (int v = 0; v < V; ++v) { m.b[v] = fmaf(m.a[v], e.b[v], m.b[v]); m.a[v] *= e.a[v]; }
-    m.closed = e.closed;
+    for (int v = 0; v < V; ++v) {
+        m.b[v] = open ? fmaf(m.a[v], e.b[v], m.b[v]) : m.b[v];
+        m.a[v] *= e.a[v];
+    }
+    m.closed |= e.closed;
 }
 template <int V>
 __device__ __forceinline__ void apply_map(float (&h)[V], const Map<V>& m) {
@@ -213,18 +232,18 @@ __device__ __forceinline__ void apply_map(float (&h)[V], const Map<V>& m) {
     for (int v = 0; v < V; ++v) h[v] = m.closed ? m.b[v] : fmaf(m.a[v], h[v], m.b[v]);
 }
 
+// The warps' maps of one tile, for one direction.
 template <int V>
-struct Shared {
+struct alignas(16) WarpMaps {     // read and written V floats at a time
     float a[kWarps][32 * V], b[kWarps][32 * V];
     int closed[kWarps];
-    int seq;
 };
 
-// Lanes that hold the same channels on consecutive row groups are tx apart.  From every thread's own map `m`:
-// the warp's running composition, its total in shared memory, and the map of the warp's rows before this thread's.
-// FORWARD: rows run with the lane; else against it.
+// Lanes that hold the same channels on consecutive row groups are tx apart.  From every thread's own map: the warp's
+// total in shared memory, and the map of the warp's rows before this thread's.  FORWARD: rows run with the lane; else
+// against it.
 template <int V, bool FORWARD>
-__device__ __forceinline__ Map<V> compose_warp(const Map<V>& own, int lg_tx, Shared<V>& sh) {
+__device__ __forceinline__ Map<V> compose_warp(const Map<V>& own, int lg_tx, WarpMaps<V>& sh) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tx = 1 << lg_tx;
     Map<V> run = own;
     for (int off = tx; off < 32; off <<= 1) {
@@ -239,46 +258,63 @@ __device__ __forceinline__ Map<V> compose_warp(const Map<V>& own, int lg_tx, Sha
     }
     if (FORWARD ? lane >= 32 - tx : lane < tx) {
         const int at = (lane & (tx - 1)) * V;
-#pragma unroll
-        for (int v = 0; v < V; ++v) { sh.a[warp][at + v] = run.a[v]; sh.b[warp][at + v] = run.b[v]; }
+        store_floats<float, V>(&sh.a[warp][at], run.a);
+        store_floats<float, V>(&sh.b[warp][at], run.b);
         if ((lane & (tx - 1)) == 0) sh.closed[warp] = run.closed;
     }
     Map<V> before;
+    identity(before);
+    if (tx < 32) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        before.a[v] = FORWARD ? __shfl_up_sync(0xffffffffu, run.a[v], tx) : __shfl_down_sync(0xffffffffu, run.a[v], tx);
-        before.b[v] = FORWARD ? __shfl_up_sync(0xffffffffu, run.b[v], tx) : __shfl_down_sync(0xffffffffu, run.b[v], tx);
+        for (int v = 0; v < V; ++v) {
+            before.a[v] = FORWARD ? __shfl_up_sync(0xffffffffu, run.a[v], tx) : __shfl_down_sync(0xffffffffu, run.a[v], tx);
+            before.b[v] = FORWARD ? __shfl_up_sync(0xffffffffu, run.b[v], tx) : __shfl_down_sync(0xffffffffu, run.b[v], tx);
+        }
+        before.closed = FORWARD ? __shfl_up_sync(0xffffffffu, run.closed, tx) : __shfl_down_sync(0xffffffffu, run.closed, tx);
+        if (FORWARD ? lane < tx : lane >= 32 - tx) identity(before);
     }
-    before.closed = FORWARD ? __shfl_up_sync(0xffffffffu, run.closed, tx) : __shfl_down_sync(0xffffffffu, run.closed, tx);
-    if (FORWARD ? lane < tx : lane >= 32 - tx) identity(before);
     return before;
 }
 template <int V>
-__device__ __forceinline__ Map<V> warp_total(const Shared<V>& sh, int warp, int tx) {
+__device__ __forceinline__ Map<V> warp_map(const WarpMaps<V>& sh, int warp, int tx) {
     Map<V> m;
+    const Pack<float, V> pa = load_pack<float, V>(&sh.a[warp][tx * V]), pb = load_pack<float, V>(&sh.b[warp][tx * V]);
 #pragma unroll
-    for (int v = 0; v < V; ++v) { m.a[v] = sh.a[warp][tx * V + v]; m.b[v] = sh.b[warp][tx * V + v]; }
+    for (int v = 0; v < V; ++v) { m.a[v] = pa.e[v]; m.b[v] = pb.e[v]; }
     m.closed = sh.closed[warp];
     return m;
 }
+// carry: the state before the tile -> the state after it.  Returns the state before this thread's warp.
+template <int V, bool FORWARD>
+__device__ __forceinline__ void pass_warps(const WarpMaps<V>& sh, int tx, float (&carry)[V], float (&mine)[V]) {
+    const int warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+        const int w = FORWARD ? i : kWarps - 1 - i;
+        if (w == warp) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) mine[v] = carry[v];
+        }
+        apply_map(carry, warp_map<V>(sh, w, tx));
+    }
+}
 
-// ---- a tile's place ------------------------------------------------------------------------------------------------
+// ---- a block's place -----------------------------------------------------------------------------------------------------
 struct Place {
     int chain, head, part, channel, tx;
-    long long chunk, p0;
-    int row0;              // this thread's first row inside the tile
+    long long segment;
+    int row0;              // this thread's first row inside a tile
     bool active;
     ChainRows rows;
 };
-template <int V, int L>
-__device__ __forceinline__ Place place_of(const Args& a, long long tile, int tile_rows, bool table) {
+template <int V, int L, bool TABLE>
+__device__ __forceinline__ Place place_of(const Args& a) {
     Place p;
     const int blocks = a.heads * a.parts;
-    const int block = (int)(tile % blocks);
-    const long long rest = tile / blocks;
+    const long long rest = blockIdx.x / blocks;
+    const int block = (int)(blockIdx.x - rest * blocks);
     p.chain = (int)(rest % a.chains);
-    p.chunk = rest / a.chains;
-    p.p0 = p.chunk * tile_rows;
+    p.segment = rest / a.chains;
     p.head = block / a.parts;
     p.part = block - p.head * a.parts;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -287,21 +323,30 @@ __device__ __forceinline__ Place place_of(const Args& a, long long tile, int til
     const int c = (p.part << a.lg_tx) * V + p.tx * V;
     p.active = c < a.per_head;
     p.channel = p.head * a.per_head + c;
-    if (!table) p.rows = chain_rows_of(a, p.chain);
+    if (!TABLE) p.rows = chain_rows_of(a, p.chain);
     return p;
 }
-// The sequence that begins at the thread's row l (kNone, kOutside), and the one that ends there.
-template <bool TABLE>
-__device__ __forceinline__ int first_at(const Place& p, const int* table, int l) {
-    if (TABLE) return table[p.row0 + l];
-    const long long t = p.p0 + p.row0 + l;
-    return t < p.rows.lo || t >= p.rows.hi ? kOutside : t == p.rows.lo ? p.rows.sequence : kNone;
-}
-template <bool TABLE>
-__device__ __forceinline__ int end_at(const Place& p, const int* table, int l) {
-    if (TABLE) return table[p.row0 + l];
-    return p.p0 + p.row0 + l == p.rows.hi - 1 ? p.rows.sequence : kNone;
-}
+
+// What a thread knows of its L rows of one tile.  first(l) / end(l): the sequence that begins / ends there, or negative.
+template <int L, bool TABLE>
+struct Rows {
+    const int *t_first, *t_end;
+    int lo, hi, sequence;      // without a table: rows l in [lo, hi) belong to `sequence`, which begins at lo and ends at hi - 1
+    __device__ __forceinline__ Rows(const Place& p, long long p0, RowTable t) {
+        if (TABLE) {
+            t_first = t.first + p.row0;
+            t_end = t.end + p.row0;
+        } else {
+            const long long at = p0 + p.row0;
+            lo = (int)min(max(p.rows.lo - at, -1ll), (long long)L);       // -1: began before
+            hi = (int)min(max(p.rows.hi - at, -1ll), (long long)L + 1);   // L + 1: goes on
+            sequence = p.rows.sequence;
+        }
+    }
+    __device__ __forceinline__ bool outside(int l) const { return TABLE ? t_first[l] == kOutside : l < lo || l >= hi; }
+    __device__ __forceinline__ int first(int l) const { return TABLE ? t_first[l] : l == lo && l < hi ? sequence : kNone; }
+    __device__ __forceinline__ int end(int l) const { return TABLE ? t_end[l] : l == hi - 1 && l >= lo ? sequence : kNone; }
+};
 
 template <int V>
 __device__ __forceinline__ void load_state(const float* states, long long index, int channels, int channel, float (&o)[V]) {
@@ -315,254 +360,391 @@ __device__ __forceinline__ void load_state(const float* states, long long index,
     for (int v = 0; v < V; ++v) o[v] = q.e[v];
 }
 
-// The thread's rows of x and the gate, all loads in flight together: x as floats, the gate encoded.  Rows that belong to no
-// sequence: x = 0 and, whatever the form, a map that leaves the state as it is is the caller's business.
-template <typename T, int V, int L, bool TABLE>
-__device__ __forceinline__ void load_rows(const Args& a, const Place& p, const int* first, float (&x)[L][V], float (&m)[L][V]) {
-    const T* px = static_cast<const T*>(a.x) + (p.chain * a.chain_rows + p.p0 + p.row0) * a.x_stride + p.channel;
-    const T* pg = static_cast<const T*>(a.gate) + (p.chain * a.chain_rows + p.p0 + p.row0) * a.gate_stride +
-                  (a.shared ? p.head : p.channel);
-    Pack<T, V> rx[L], rg[L];
+// ---- rows on their way through shared memory ---------------------------------------------------------------------------
+// A thread's V elements of row l, tensor k: slot (k L + l) of the stage, lanes side by side.
+template <typename T, int V>
+__device__ __forceinline__ void copy_async(T* to, const T* from, bool there) {
+    constexpr int kBytes = V * sizeof(T);
+    if (kBytes == 2) {
+        memset(to, 0, kBytes);
+        if (there) *to = *from;
+    } else {
+        const unsigned at = (unsigned)__cvta_generic_to_shared(to);
+        const int bytes = there ? kBytes : 0;    // what is not copied is filled with zeros
+        if (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(bytes) : "memory");
+        else if (kBytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(at), "l"(from), "r"(bytes) : "memory");
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(at), "l"(from), "r"(bytes) : "memory");
+    }
+}
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_landed() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+template <typename T, int V, int L, int TENSORS>
+struct alignas(16) Stage {
+    T v[TENSORS][L][kThreads][V];
+};
+
+// Rows p0 + row0 .. of one tensor; rows past the chain's end become zeros.  Rows that belong to no sequence but lie within
+// the tensor are copied like the others and masked where they are used.
+template <typename T, int V, int L>
+__device__ __forceinline__ void fetch_rows(T (*to)[kThreads][V], const T* base, long long stride, const Args& a, const Place& p,
+                                           long long p0) {
+    const long long at = p0 + p.row0;
+    const T* from = base + (p.chain * a.chain_rows + at) * stride;
+    const int left = p.active ? (int)min(a.chain_rows - at, (long long)L) : 0;
+#pragma unroll
+    for (int l = 0; l < L; ++l) copy_async<T, V>(to[l][threadIdx.x], l < left ? from + l * stride : base, l < left);
+}
+// The gates of the rows, encoded.  Shared ones are read directly: every thread of a row wants the same value.
+template <typename T, int V, int L>
+__device__ __forceinline__ void fetch_gates(T (*to)[kThreads][V], T (&own)[L], const Args& a, const Place& p, long long p0) {
+    const T* base = static_cast<const T*>(a.gate) + (a.shared ? p.head : p.channel);
+    if (!a.shared) {
+        fetch_rows<T, V, L>(to, base, a.gate_stride, a, p, p0);
+        return;
+    }
+    const long long at = p0 + p.row0;
+    const T* from = base + (p.chain * a.chain_rows + at) * a.gate_stride;
+    const int left = p.active ? (int)min(a.chain_rows - at, (long long)L) : 0;
 #pragma unroll
     for (int l = 0; l < L; ++l) {
-        const bool there = p.active && first_at<TABLE>(p, first, l) != kOutside;
-        if (there) {
-            rx[l] = load_pack<T, V>(px + l * a.x_stride);
-            if (a.shared) rg[l].e[0] = pg[l * a.gate_stride];
-            else rg[l] = load_pack<T, V>(pg + l * a.gate_stride);
+        if (l < left) own[l] = from[l * a.gate_stride];
+        else memset(&own[l], 0, sizeof(T));
+    }
+}
+template <typename T, int V, int L>
+__device__ __forceinline__ void read_gates(const T (*from)[kThreads][V], const T (&own)[L], const Args& a, float (&m)[L][V]) {
+#pragma unroll
+    for (int l = 0; l < L; ++l) {
+        if (a.shared) {
+            const float one = encode_gate(to_float(own[l]), a.logit);
+#pragma unroll
+            for (int v = 0; v < V; ++v) m[l][v] = one;
         } else {
-            memset(&rx[l], 0, sizeof(rx[l]));
-            memset(&rg[l], 0, sizeof(rg[l]));
+            const Pack<T, V> g = load_pack<T, V>(from[l][threadIdx.x]);
+#pragma unroll
+            for (int v = 0; v < V; ++v) m[l][v] = encode_gate(to_float(g.e[v]), a.logit);
         }
     }
+}
+
+// The state (or q) at the segment's beginning: the maps of the segments before it, each warp a share of them, in order.
+template <int V, bool FORWARD>
+__device__ void carry_of_segment(const Args& a, const Place& p, WarpMaps<V>& sh, float (&carry)[V]) {
+    const long long before = FORWARD ? p.segment : a.segments - 1 - p.segment;
 #pragma unroll
-    for (int l = 0; l < L; ++l) {
+    for (int v = 0; v < V; ++v) carry[v] = 0.f;
+    if (before == 0) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long share = (before + kWarps - 1) / kWarps;
+    const long long i0 = min(share * warp, before), i1 = min(i0 + share, before);
+    Map<V> all;
+    identity(all);
+    if (lane < (1 << a.lg_tx)) {
+#pragma unroll 4
+        for (long long i = i0; i < i1; ++i) {
+            const long long at = p.chain * a.segments + (FORWARD ? i : a.segments - 1 - i);
+            Map<V> m;
+            identity(m);
+            m.closed = a.map_closed[at];
+            if (p.active) {
+                const Pack<float, V> pa = load_pack<float, V>(a.map_a + at * a.channels + p.channel);
+                const Pack<float, V> pb = load_pack<float, V>(a.map_b + at * a.channels + p.channel);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            x[l][v] = to_float(rx[l].e[v]);
-            if (a.shared) m[l][v] = v == 0 ? encode_gate(to_float(rg[l].e[0]), a.logit) : m[l][0];
-            else m[l][v] = encode_gate(to_float(rg[l].e[v]), a.logit);
+                for (int v = 0; v < V; ++v) { m.a[v] = pa.e[v]; m.b[v] = pb.e[v]; }
+            }
+            compose_after(m, all);
+            all = m;
         }
+        store_floats<float, V>(&sh.a[warp][p.tx * V], all.a);
+        store_floats<float, V>(&sh.b[warp][p.tx * V], all.b);
+        if (p.tx == 0) sh.closed[warp] = all.closed;
     }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) apply_map(carry, warp_map<V>(sh, w, p.tx));
+    __syncthreads();
+}
+
+// Leaves the composition of a whole segment's tiles (APPLY = false).
+template <int V>
+__device__ __forceinline__ void store_segment_map(const Args& a, const Place& p, const Map<V>& all) {
+    if (threadIdx.x >= (1 << a.lg_tx) || !p.active) return;
+    const long long at = p.chain * a.segments + p.segment;
+    store_floats<float, V>(a.map_a + at * a.channels + p.channel, all.a);
+    store_floats<float, V>(a.map_b + at * a.channels + p.channel, all.b);
+    if (p.tx == 0) a.map_closed[at] = all.closed;
 }
 
 template <typename T, int V, int L, bool TABLE, bool APPLY>
 __global__ void __launch_bounds__(kThreads)
 recurrence_forward_kernel(const Args a) {
-    __shared__ Shared<V> sh;
-    extern __shared__ int s_table[];
+    typedef Stage<T, V, L, 2> Ring;
+    extern __shared__ __align__(16) unsigned char s_raw[];
+    Ring* ring = reinterpret_cast<Ring*>(s_raw);
+    int* tables = reinterpret_cast<int*>(s_raw + kStages * sizeof(Ring));
+    __shared__ WarpMaps<V> sh[2];
     const int tile_rows = kWarps * (32 >> a.lg_tx) * L;
-    int* first = s_table;
-    int* end = s_table + tile_rows;
-    const Place p = place_of<V, L>(a, blockIdx.x, tile_rows, TABLE);
-    if (TABLE) fill_row_table(a, p.p0, tile_rows, first, end, &sh.seq);
-    float f[L][V], b[L][V];
-    load_rows<T, V, L, TABLE>(a, p, first, b, f);
+    const Place p = place_of<V, L, TABLE>(a);
+    const long long t0 = p.segment * a.segment_tiles, t1 = min(t0 + a.segment_tiles, a.tiles);
+    const T* x = static_cast<const T*>(a.x) + p.channel;
+    auto table = [&](long long t) { int* at = tables + (int)(t % kTables) * 2 * tile_rows; return RowTable{at, at + tile_rows}; };
 
-    Map<V> own;
-    identity(own);
+    float carry[V];
+    Map<V> all;
+    identity(all);
+    if (APPLY) carry_of_segment<V, true>(a, p, sh[0], carry);
+    T gate_now[L], gate_next[L];
+    fetch_rows<T, V, L>(ring[0].v[0], x, a.x_stride, a, p, t0 * tile_rows);
+    fetch_gates<T, V, L>(ring[0].v[1], gate_next, a, p, t0 * tile_rows);
+    copies_issued();
+    if (TABLE) {
+        fill_row_table(a, t0 * tile_rows, tile_rows, table(t0));
+        __syncthreads();
+    }
+    for (long long t = t0; t < t1; ++t) {
+        const int stage = (int)(t - t0) & 1;
+        const long long p0 = t * tile_rows;
 #pragma unroll
-    for (int l = 0; l < L; ++l) {
-        const int s = first_at<TABLE>(p, first, l);
-        float st[V];
-        if (s >= 0 && p.active) load_state<V>(a.state_in, s, a.channels, p.channel, st);
-        if (s >= 0) own.closed = 1;
+        for (int l = 0; l < L; ++l) gate_now[l] = gate_next[l];
+        if (t + 1 < t1) {
+            fetch_rows<T, V, L>(ring[stage ^ 1].v[0], x, a.x_stride, a, p, p0 + tile_rows);
+            fetch_gates<T, V, L>(ring[stage ^ 1].v[1], gate_next, a, p, p0 + tile_rows);
+        }
+        copies_issued();
+        copies_landed<1>();
+        const Rows<L, TABLE> rows(p, p0, table(t));
+        float f[L][V], b[L][V];
+        read_gates<T, V, L>(ring[stage].v[1], gate_now, a, f);
+        Map<V> own;
+        identity(own);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const float m = f[l][v];
-            f[l][v] = s == kOutside ? 1.f : gate_f(m, a.logit);
-            if (a.coupled) b[l][v] *= gate_k(m, a.logit);
-            own.b[v] = fmaf(f[l][v], s >= 0 && p.active ? st[v] : own.b[v], b[l][v]);
-            own.a[v] *= f[l][v];
+        for (int l = 0; l < L; ++l) {
+            const int s = rows.first(l);
+            const bool outside = rows.outside(l);
+            const Pack<T, V> px = load_pack<T, V>(ring[stage].v[0][l][threadIdx.x]);
+            float st[V];
+            if (s >= 0) {
+                own.closed = 1;
+                if (p.active) load_state<V>(a.state_in, s, a.channels, p.channel, st);
+            }
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float k;
+                decode_gate(f[l][v], a.logit, f[l][v], k);
+                const float xv = to_float(px.e[v]);
+                b[l][v] = outside ? 0.f : a.coupled ? xv * k : xv;
+                f[l][v] = outside ? 1.f : f[l][v];
+                own.b[v] = fmaf(f[l][v], s >= 0 && p.active ? st[v] : own.b[v], b[l][v]);
+                own.a[v] *= f[l][v];
+            }
+        }
+        const Map<V> before = compose_warp<V, true>(own, a.lg_tx, sh[stage]);
+        if (TABLE && t + 1 < t1) fill_row_table(a, p0 + tile_rows, tile_rows, table(t + 1));
+        __syncthreads();
+        if (!APPLY) {
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                Map<V> m = warp_map<V>(sh[stage], w, p.tx);
+                compose_after(m, all);
+                all = m;
+            }
+            continue;
+        }
+        if (a.checkpoints && threadIdx.x < (1 << a.lg_tx) && p.active)
+            store_floats<float, V>(a.checkpoints + (p.chain * a.tiles + t) * a.channels + p.channel, carry);
+        float h[V];
+        pass_warps<V, true>(sh[stage], p.tx, carry, h);
+        apply_map(h, before);
+        T* ph = a.h ? static_cast<T*>(a.h) + (p.chain * a.chain_rows + p0 + p.row0) * a.h_stride + p.channel : nullptr;
+        const int left = p.active ? (int)min(a.chain_rows - p0 - p.row0, (long long)L) : 0;
+#pragma unroll
+        for (int l = 0; l < L; ++l) {
+            const int s = rows.first(l), e = rows.end(l);
+            if (s >= 0 && p.active) load_state<V>(a.state_in, s, a.channels, p.channel, h);
+            const bool outside = rows.outside(l);
+            float o[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                h[v] = fmaf(f[l][v], h[v], b[l][v]);
+                o[v] = outside ? 0.f : h[v];
+            }
+            if (ph && l < left) store_floats<T, V>(ph + l * a.h_stride, o);
+            if (e >= 0 && p.active) store_floats<float, V>(a.state_out + (long long)e * a.channels + p.channel, h);
         }
     }
-    const Map<V> before = compose_warp<V, true>(own, a.lg_tx, sh);
-    __syncthreads();
-    const int warp = threadIdx.x >> 5;
-    const long long at = (p.chain * a.chunks + p.chunk) * a.channels + p.channel;
-    if (!APPLY) {
-        if (warp == 0 && (threadIdx.x & 31) < (1 << a.lg_tx) && p.active) {
-            Map<V> all = warp_total<V>(sh, kWarps - 1, p.tx);
-            for (int w = kWarps - 2; w >= 0; --w) compose_after(all, warp_total<V>(sh, w, p.tx));
-            store_floats<float, V>(a.map_a + at, all.a);
-            store_floats<float, V>(a.map_b + at, all.b);
-            if (p.tx == 0) a.map_closed[p.chain * a.chunks + p.chunk] = all.closed;
-        }
-        return;
-    }
-    float h[V];
-    load_state<V>(p.active && a.chunks > 1 ? a.map_a : nullptr, p.chain * a.chunks + p.chunk, a.channels, p.channel, h);
-    for (int w = 0; w < warp; ++w) apply_map(h, warp_total<V>(sh, w, p.tx));
-    apply_map(h, before);
-    const long long p_first = p.p0 + p.row0;
-    if (a.checkpoints && p.active && p_first < a.chain_rows && p_first % a.checkpoint_rows == 0)
-        store_floats<float, V>(a.checkpoints + (p.chain * a.checkpoint_chunks + p_first / a.checkpoint_rows) * a.channels + p.channel, h);
-    T* ph = a.h ? static_cast<T*>(a.h) + (p.chain * a.chain_rows + p_first) * a.h_stride + p.channel : nullptr;
-#pragma unroll
-    for (int l = 0; l < L; ++l) {
-        const int s = first_at<TABLE>(p, first, l), e = end_at<TABLE>(p, end, l);
-        if (s >= 0 && p.active) load_state<V>(a.state_in, s, a.channels, p.channel, h);
-        float o[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            h[v] = fmaf(f[l][v], h[v], b[l][v]);
-            o[v] = s == kOutside ? 0.f : h[v];
-        }
-        if (ph && p.active && p_first + l < a.chain_rows) store_floats<T, V>(ph + l * a.h_stride, o);
-        if (e >= 0 && p.active) store_floats<float, V>(a.state_out + (long long)e * a.channels + p.channel, h);
-    }
-    pass_empty_sequences(a, a.state_in, a.state_out);
-}
-
-// From the chunks' maps to the state before each chunk (after it, when the scan runs against the chunks).
-template <bool FORWARD>
-__global__ void __launch_bounds__(kThreads) recurrence_carry_kernel(const Args a) {
-    const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= a.chains * a.channels) return;
-    const long long chain = i / a.channels;
-    const int c = (int)(i - chain * a.channels);
-    float s = 0.f;
-    for (long long j = 0; j < a.chunks; ++j) {
-        const long long chunk = chain * a.chunks + (FORWARD ? j : a.chunks - 1 - j);
-        const float ma = a.map_a[chunk * a.channels + c], mb = a.map_b[chunk * a.channels + c];
-        a.map_a[chunk * a.channels + c] = s;
-        s = a.map_closed[chunk] ? mb : fmaf(ma, s, mb);
-    }
+    if (APPLY) pass_empty_sequences(a, a.state_in, a.state_out);
+    else store_segment_map<V>(a, p, all);
 }
 
 template <typename T, int V, int L, bool TABLE, bool APPLY>
 __global__ void __launch_bounds__(kThreads)
 recurrence_backward_kernel(const Args a) {
-    __shared__ Shared<V> sh;
-    extern __shared__ int s_table[];
+    typedef Stage<T, V, L, 3> Ring;
+    extern __shared__ __align__(16) unsigned char s_raw[];
+    Ring* ring = reinterpret_cast<Ring*>(s_raw);
+    int* tables = reinterpret_cast<int*>(s_raw + kStages * sizeof(Ring));
+    __shared__ WarpMaps<V> sh[2], sh_forward[2];
     const int tile_rows = kWarps * (32 >> a.lg_tx) * L;
-    int* first = s_table;
-    int* end = s_table + tile_rows;
-    const Place p = place_of<V, L>(a, blockIdx.x, tile_rows, TABLE);
-    if (TABLE) fill_row_table(a, p.p0, tile_rows, first, end, &sh.seq);
-    const int warp = threadIdx.x >> 5;
-    const long long p_first = p.p0 + p.row0;
-    float u[L][V], m[L][V], d[L][V];
-    {
-        const T* pd = static_cast<const T*>(a.v_h) + (p.chain * a.chain_rows + p_first) * a.v_h_stride + p.channel;
-        Pack<T, V> rd[L];
-#pragma unroll
-        for (int l = 0; l < L; ++l) {
-            const bool there = a.v_h && p.active && first_at<TABLE>(p, first, l) != kOutside;
-            if (there) rd[l] = load_pack<T, V>(pd + l * a.v_h_stride);
-            else memset(&rd[l], 0, sizeof(rd[l]));
+    const Place p = place_of<V, L, TABLE>(a);
+    const long long t0 = p.segment * a.segment_tiles, t1 = min(t0 + a.segment_tiles, a.tiles);
+    const T* x = static_cast<const T*>(a.x) + p.channel;
+    const T* vh = static_cast<const T*>(a.v_h) + p.channel;
+    auto table = [&](long long t) { int* at = tables + (int)(t % kTables) * 2 * tile_rows; return RowTable{at, at + tile_rows}; };
+
+    float q_carry[V], start[V], start_next[V];
+    Map<V> all;
+    identity(all);
+    if (APPLY) carry_of_segment<V, false>(a, p, sh[0], q_carry);
+    T gate_now[L], gate_next[L];
+    auto fetch = [&](int stage, long long t) {
+        if (a.v_h) fetch_rows<T, V, L>(ring[stage].v[0], vh, a.v_h_stride, a, p, t * tile_rows);
+        fetch_gates<T, V, L>(ring[stage].v[1], gate_next, a, p, t * tile_rows);
+        if (APPLY) {
+            fetch_rows<T, V, L>(ring[stage].v[2], x, a.x_stride, a, p, t * tile_rows);
+            load_state<V>(p.active ? a.checkpoints : nullptr, p.chain * a.tiles + t, a.channels, p.channel, start_next);
         }
-        load_rows<T, V, L, TABLE>(a, p, first, u, m);
-#pragma unroll
-        for (int l = 0; l < L; ++l)
-#pragma unroll
-            for (int v = 0; v < V; ++v) d[l][v] = to_float(rd[l].e[v]);
+    };
+    fetch((int)(t1 - 1 - t0) & 1, t1 - 1);
+    copies_issued();
+    if (TABLE) {
+        fill_row_table(a, (t1 - 1) * tile_rows, tile_rows, table(t1 - 1));
+        __syncthreads();
     }
-    if (APPLY) {   // u_t <- h_{t-1}, coupled: h_{t-1} - x_t
-        Map<V> own;
+    for (long long t = t1 - 1; t >= t0; --t) {
+        const int stage = (int)(t - t0) & 1;
+        const long long p0 = t * tile_rows;
+#pragma unroll
+        for (int l = 0; l < L; ++l) gate_now[l] = gate_next[l];
+#pragma unroll
+        for (int v = 0; v < V; ++v) start[v] = start_next[v];
+        if (t > t0) fetch(stage ^ 1, t - 1);
+        copies_issued();
+        copies_landed<1>();
+        const Rows<L, TABLE> rows(p, p0, table(t));
+        float m[L][V], u[L][V];
+        read_gates<T, V, L>(ring[stage].v[1], gate_now, a, m);
+        Map<V> own, before;
+        if (APPLY) {
+            identity(own);
+#pragma unroll
+            for (int l = 0; l < L; ++l) {
+                const int s = rows.first(l);
+                const bool outside = rows.outside(l);
+                const Pack<T, V> px = load_pack<T, V>(ring[stage].v[2][l][threadIdx.x]);
+                float st[V];
+                if (s >= 0) {
+                    own.closed = 1;
+                    if (p.active) load_state<V>(a.state_in, s, a.channels, p.channel, st);
+                }
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    float f, k;
+                    decode_gate(m[l][v], a.logit, f, k);
+                    const float xv = to_float(px.e[v]);
+                    const float b = outside ? 0.f : a.coupled ? xv * k : xv;
+                    f = outside ? 1.f : f;
+                    own.b[v] = fmaf(f, s >= 0 && p.active ? st[v] : own.b[v], b);
+                    own.a[v] *= f;
+                }
+            }
+            before = compose_warp<V, true>(own, a.lg_tx, sh_forward[stage]);
+        }
         identity(own);
 #pragma unroll
-        for (int l = 0; l < L; ++l) {
-            const int s = first_at<TABLE>(p, first, l);
-            float st[V];
-            if (s >= 0 && p.active) load_state<V>(a.state_in, s, a.channels, p.channel, st);
-            if (s >= 0) own.closed = 1;
+        for (int l = L - 1; l >= 0; --l) {
+            const int e = rows.end(l);
+            const bool outside = rows.outside(l);
+            Pack<T, V> pd;
+            if (a.v_h) pd = load_pack<T, V>(ring[stage].v[0][l][threadIdx.x]);
+            float q[V];
+            if (e >= 0) {
+                own.closed = 1;
+                if (p.active) load_state<V>(a.v_state_out, e, a.channels, p.channel, q);
+            }
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const float f = s == kOutside ? 1.f : gate_f(m[l][v], a.logit);
-                const float b = a.coupled ? u[l][v] * gate_k(m[l][v], a.logit) : u[l][v];
-                own.b[v] = fmaf(f, s >= 0 && p.active ? st[v] : own.b[v], b);
+                float f, k;
+                decode_gate(m[l][v], a.logit, f, k);
+                f = outside ? 1.f : f;
+                const float d = outside || !a.v_h ? 0.f : to_float(pd.e[v]);
+                own.b[v] = f * (d + (e >= 0 && p.active ? q[v] : own.b[v]));
                 own.a[v] *= f;
             }
         }
-        const Map<V> before = compose_warp<V, true>(own, a.lg_tx, sh);
+        const Map<V> after = compose_warp<V, false>(own, a.lg_tx, sh[stage]);
+        if (TABLE && t > t0) fill_row_table(a, p0 - tile_rows, tile_rows, table(t - 1));
         __syncthreads();
-        float h[V];
-        load_state<V>(p.active && p.chunk > 0 ? a.checkpoints : nullptr, p.chain * a.checkpoint_chunks + p.chunk, a.channels,
-                      p.channel, h);
-        for (int w = 0; w < warp; ++w) apply_map(h, warp_total<V>(sh, w, p.tx));
-        apply_map(h, before);
+        if (!APPLY) {
 #pragma unroll
-        for (int l = 0; l < L; ++l) {
-            const int s = first_at<TABLE>(p, first, l);
+            for (int w = kWarps - 1; w >= 0; --w) {
+                Map<V> n = warp_map<V>(sh[stage], w, p.tx);
+                compose_after(n, all);
+                all = n;
+            }
+            continue;
+        }
+        float h[V], q[V];
+        pass_warps<V, true>(sh_forward[stage], p.tx, start, h);
+        apply_map(h, before);
+        pass_warps<V, false>(sh[stage], p.tx, q_carry, q);
+        apply_map(q, after);
+#pragma unroll
+        for (int l = 0; l < L; ++l) {          // u_t: h_{t-1}, coupled: h_{t-1} - x_t
+            const int s = rows.first(l);
             if (s >= 0 && p.active) load_state<V>(a.state_in, s, a.channels, p.channel, h);
+            const bool outside = rows.outside(l);
+            const Pack<T, V> px = load_pack<T, V>(ring[stage].v[2][l][threadIdx.x]);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const float f = s == kOutside ? 1.f : gate_f(m[l][v], a.logit);
-                const float x = u[l][v];
-                const float b = a.coupled ? x * gate_k(m[l][v], a.logit) : x;
-                u[l][v] = a.coupled ? h[v] - x : h[v];
-                h[v] = fmaf(f, h[v], b);
+                float f, k;
+                decode_gate(m[l][v], a.logit, f, k);
+                const float xv = to_float(px.e[v]);
+                const float b = outside ? 0.f : a.coupled ? xv * k : xv;
+                u[l][v] = a.coupled ? h[v] - xv : h[v];
+                h[v] = fmaf(outside ? 1.f : f, h[v], b);
             }
         }
-        __syncthreads();   // the warps' totals are about to be overwritten
-    }
-    Map<V> own;
-    identity(own);
+        const long long row = p.chain * a.chain_rows + p0 + p.row0;
+        const int left = (int)min(a.chain_rows - p0 - p.row0, (long long)L);
+        T* px = a.v_x ? static_cast<T*>(a.v_x) + row * a.h_stride + p.channel : nullptr;
 #pragma unroll
-    for (int l = L - 1; l >= 0; --l) {
-        const int s = first_at<TABLE>(p, first, l), e = end_at<TABLE>(p, end, l);
-        float q[V];
-        if (e >= 0 && p.active) load_state<V>(a.v_state_out, e, a.channels, p.channel, q);
-        if (e >= 0) own.closed = 1;
+        for (int l = L - 1; l >= 0; --l) {
+            const int s = rows.first(l), e = rows.end(l);
+            if (e >= 0 && p.active) load_state<V>(a.v_state_out, e, a.channels, p.channel, q);
+            const bool outside = rows.outside(l) || !p.active;
+            Pack<T, V> pd;
+            if (a.v_h) pd = load_pack<T, V>(ring[stage].v[0][l][threadIdx.x]);
+            float dx[V], dg[V], sum = 0.f;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const float f = s == kOutside ? 1.f : gate_f(m[l][v], a.logit);
-            own.b[v] = f * (d[l][v] + (e >= 0 && p.active ? q[v] : own.b[v]));
-            own.a[v] *= f;
-        }
-    }
-    const Map<V> after = compose_warp<V, false>(own, a.lg_tx, sh);
-    __syncthreads();
-    const long long at = (p.chain * a.chunks + p.chunk) * a.channels + p.channel;
-    if (!APPLY) {
-        if (warp == 0 && (threadIdx.x & 31) < (1 << a.lg_tx) && p.active) {
-            Map<V> all = warp_total<V>(sh, 0, p.tx);
-            for (int w = 1; w < kWarps; ++w) compose_after(all, warp_total<V>(sh, w, p.tx));
-            store_floats<float, V>(a.map_a + at, all.a);
-            store_floats<float, V>(a.map_b + at, all.b);
-            if (p.tx == 0) a.map_closed[p.chain * a.chunks + p.chunk] = all.closed;
-        }
-        return;
-    }
-    float q[V];
-    load_state<V>(p.active && a.chunks > 1 ? a.map_a : nullptr, p.chain * a.chunks + p.chunk, a.channels, p.channel, q);
-    for (int w = kWarps - 1; w > warp; --w) apply_map(q, warp_total<V>(sh, w, p.tx));
-    apply_map(q, after);
-    T* px = a.v_x ? static_cast<T*>(a.v_x) + (p.chain * a.chain_rows + p_first) * a.h_stride + p.channel : nullptr;
-    const long long gate_row = (p.chain * a.chain_rows + p_first);
-#pragma unroll
-    for (int l = L - 1; l >= 0; --l) {
-        const int s = first_at<TABLE>(p, first, l), e = end_at<TABLE>(p, end, l);
-        if (e >= 0 && p.active) load_state<V>(a.v_state_out, e, a.channels, p.channel, q);
-        const bool row_there = p_first + l < a.chain_rows;
-        float dx[V], dg[V], sum = 0.f;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const bool outside = s == kOutside || !p.active;
-            const float f = s == kOutside ? 1.f : gate_f(m[l][v], a.logit), k = gate_k(m[l][v], a.logit);
-            const float g = d[l][v] + q[v];
-            dx[v] = outside ? 0.f : a.coupled ? k * g : g;
-            dg[v] = outside ? 0.f : a.logit ? g * u[l][v] * (f * k) : g * u[l][v];
-            sum += dg[v];
-            q[v] = f * g;
-        }
-        if (px && p.active && row_there) store_floats<T, V>(px + l * a.h_stride, dx);
-        if (s >= 0 && p.active && a.v_state_in) store_floats<float, V>(a.v_state_in + (long long)s * a.channels + p.channel, q);
-        if (a.v_gate) {
-            if (!a.shared) {
-                if (p.active && row_there) store_floats<T, V>(static_cast<T*>(a.v_gate) + (gate_row + l) * a.gate_out_stride + p.channel, dg);
-            } else {
-                for (int off = (1 << a.lg_tx) >> 1; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-                if (p.tx == 0 && row_there) {
-                    const long long o = (gate_row + l) * a.gate_out_stride + p.head;
-                    if (a.parts == 1) from_float(sum, static_cast<T*>(a.v_gate)[o]);
-                    else a.gate_parts[(a.reverse ? (a.rows - 1) * a.gate_heads + o : o) + (long long)p.part * a.rows * a.gate_heads] = sum;
+            for (int v = 0; v < V; ++v) {
+                float f, k;
+                decode_gate(m[l][v], a.logit, f, k);
+                const float g = (outside || !a.v_h ? 0.f : to_float(pd.e[v])) + q[v];
+                dx[v] = outside ? 0.f : a.coupled ? k * g : g;
+                dg[v] = outside ? 0.f : a.logit ? g * u[l][v] * (f * k) : g * u[l][v];
+                sum += dg[v];
+                q[v] = outside ? q[v] : f * g;
+            }
+            if (px && p.active && l < left) store_floats<T, V>(px + l * a.h_stride, dx);
+            if (s >= 0 && p.active && a.v_state_in) store_floats<float, V>(a.v_state_in + (long long)s * a.channels + p.channel, q);
+            if (a.v_gate) {
+                if (!a.shared) {
+                    if (p.active && l < left) store_floats<T, V>(static_cast<T*>(a.v_gate) + (row + l) * a.gate_out_stride + p.channel, dg);
+                } else {
+                    for (int off = (1 << a.lg_tx) >> 1; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                    if (p.tx == 0 && l < left) {
+                        const long long o = (row + l) * a.gate_out_stride + p.head;
+                        if (a.parts == 1) from_float(sum, static_cast<T*>(a.v_gate)[o]);
+                        else a.gate_parts[(a.reverse ? (a.rows - 1) * a.gate_heads + o : o) + (long long)p.part * a.rows * a.gate_heads] = sum;
+                    }
                 }
             }
         }
     }
-    pass_empty_sequences(a, a.v_state_out, a.v_state_in);
+    if (APPLY) pass_empty_sequences(a, a.v_state_out, a.v_state_in);
+    else store_segment_map<V>(a, p, all);
 }
 
 // v_gate = sum of the channel blocks' shares of it, in their order
@@ -594,7 +776,9 @@ recurrence_step_kernel(const T* x, const T* gate, float* state, T* h, const long
         const float m = shared && v > 0 ? m0 : encode_gate(to_float(pg.e[v]), logit);
         m0 = m;
         const float xv = to_float(px.e[v]);
-        o[v] = fmaf(gate_f(m, logit), ps.e[v], coupled ? gate_k(m, logit) * xv : xv);
+        float f, k;
+        decode_gate(m, logit, f, k);
+        o[v] = fmaf(f, ps.e[v], coupled ? k * xv : xv);
     }
     store_floats<float, V>(state + i, o);
     store_floats<T, V>(h + i, o);
@@ -602,8 +786,10 @@ recurrence_step_kernel(const T* x, const T* gate, float* state, T* h, const long
 
 // ---- host ----------------------------------------------------------------------------------------------------------------
 
-constexpr int rows_per_thread(int vec, bool forward) { return vec == 4 ? (forward ? 8 : 4) : (forward ? 16 : 8); }
-int tile_rows_of(const Layout& l, bool forward) { return kWarps * (32 >> l.lg_tx) * rows_per_thread(l.vec, forward); }
+// Consecutive rows of a thread: as many as keep the backward's values of a tile in registers and two tiles of every tensor
+// in shared memory with four blocks on an SM.
+template <typename T> constexpr int rows_per_thread(int vec) { return vec == 4 ? (sizeof(T) == 4 ? 4 : 8) : 16; }
+constexpr int kSms = 148, kBlocksPerSm = 4;
 
 int check_shape(const DsbRecurrence& s, bool step) {
     DSB_REQUIRE(s.dtype == DSB_DTYPE_F32 || s.dtype == DSB_DTYPE_F16 || s.dtype == DSB_DTYPE_BF16, "recurrence: unknown dtype %d", s.dtype);
@@ -629,48 +815,59 @@ int check_shape(const DsbRecurrence& s, bool step) {
 }
 
 // The cut depends on the shape alone, never on addresses: the checkpoints of a forward fit every backward of the shape.
-Layout layout_of(const DsbRecurrence& s, int vec) {
-    Layout l;
-    l.vec = vec;
-    const bool shared = s.gate_heads != s.channels;
-    l.heads = shared ? s.gate_heads : 1;
-    l.per_head = s.channels / l.heads;
-    const int wide = (l.per_head + l.vec - 1) / l.vec;
-    l.lg_tx = 0;
-    while (l.lg_tx < 5 && (1 << l.lg_tx) < wide) ++l.lg_tx;
-    l.parts = (wide + (1 << l.lg_tx) - 1) >> l.lg_tx;
-    // A chain per sequence wastes half a tile per sequence on average; a table costs a look at every row.
-    l.table = s.sequence_rows == 0 || s.sequence_rows < tile_rows_of(l, true);
-    l.chains = l.table ? 1 : s.sequences;
-    l.chain_rows = l.table ? s.rows : s.sequence_rows;
-    return l;
-}
 int shape_vec(const DsbRecurrence& s) {
     const bool shared = s.gate_heads != s.channels;
     return (shared ? s.channels / s.gate_heads : s.channels) % 4 == 0 ? 4 : 1;
 }
-int64_t chunks_of(const Layout& l, bool forward) {
-    const int t = tile_rows_of(l, forward);
-    return (l.chain_rows + t - 1) / t;
+Layout layout_of(const DsbRecurrence& s) {
+    Layout l;
+    l.vec = shape_vec(s);
+    const bool shared = s.gate_heads != s.channels;
+    l.heads = shared ? s.gate_heads : 1;
+    l.per_head = s.channels / l.heads;
+    const int wide = (l.per_head + l.vec - 1) / l.vec;
+    const int rows = s.dtype == DSB_DTYPE_F32 ? rows_per_thread<float>(l.vec) : rows_per_thread<__half>(l.vec);
+    l.lg_tx = 0;
+    while (l.lg_tx < 5 && (1 << l.lg_tx) < wide) ++l.lg_tx;
+    for (;;) {
+        l.parts = (wide + (1 << l.lg_tx) - 1) >> l.lg_tx;
+        l.tile_rows = kWarps * (32 >> l.lg_tx) * rows;
+        // A chain per sequence wastes half a tile per sequence on average; a table costs a look at every row.
+        l.table = s.sequence_rows == 0 || s.sequence_rows < l.tile_rows;
+        l.chains = l.table ? 1 : s.sequences;
+        // Narrower channel blocks where wide ones are too few to fill the GPU, down to a 64-byte piece of a row.
+        if (l.lg_tx <= 3 || l.chains * l.heads * l.parts >= kSms * kBlocksPerSm) break;
+        --l.lg_tx;
+    }
+    l.chain_rows = l.table ? s.rows : s.sequence_rows;
+    l.tiles = (l.chain_rows + l.tile_rows - 1) / l.tile_rows;
+    const int64_t blocks = l.chains * l.heads * l.parts;
+    l.segments = 1;
+    if (blocks < kSms * kBlocksPerSm / 2 && l.tiles > 1) {
+        l.segments = kSms * kBlocksPerSm / blocks;
+        if (l.segments > l.tiles) l.segments = l.tiles;
+    }
+    l.segment_tiles = l.tiles ? (l.tiles + l.segments - 1) / l.segments : 0;
+    if (l.tiles) l.segments = (l.tiles + l.segment_tiles - 1) / l.segment_tiles;   // none of them empty
+    return l;
 }
 int64_t up16(int64_t b) { return (b + 15) & ~(int64_t)15; }
 
 int64_t direction_workspace(const DsbRecurrence& s, const Layout& l, bool forward) {
-    const int64_t maps = l.chains * chunks_of(l, forward);
+    const int64_t maps = l.chains * l.segments;
     int64_t bytes = 0;
-    if (chunks_of(l, forward) > 1) bytes += 2 * up16(maps * s.channels * 4) + up16(maps * 4);
+    if (l.segments > 1) bytes += 2 * up16(maps * s.channels * 4) + up16(maps * 4);
     if (!forward && s.gate_heads != s.channels && l.parts > 1) bytes += up16((int64_t)l.parts * s.rows * s.gate_heads * 4);
     return bytes;
 }
 
 bool aligned(const void* p, int64_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
-struct Cut { Layout layout; Args args; int64_t tiles; };
+struct Cut { Layout layout; Args args; int64_t blocks; };
 
 int make_cut(const DsbRecurrence& s, bool forward, void* workspace, int64_t workspace_bytes, float* checkpoints, Cut* out) {
     Cut& c = *out;
-    const int vec = shape_vec(s);
-    c.layout = layout_of(s, vec);
+    c.layout = layout_of(s);
     const Layout& l = c.layout;
     const int64_t need = direction_workspace(s, l, forward);
     if (need > 0 && (!workspace || workspace_bytes < need)) {
@@ -681,8 +878,7 @@ int make_cut(const DsbRecurrence& s, bool forward, void* workspace, int64_t work
     Args& a = c.args;
     a = Args{};
     a.rows = s.rows; a.chain_rows = l.chain_rows; a.chains = l.chains;
-    a.chunks = chunks_of(l, forward);
-    a.checkpoint_rows = tile_rows_of(l, false); a.checkpoint_chunks = chunks_of(l, false);
+    a.tiles = l.tiles; a.segments = l.segments; a.segment_tiles = l.segment_tiles;
     a.checkpoints = checkpoints;
     a.sequences = s.sequences; a.sequence_rows = s.sequence_rows; a.channels = s.channels; a.gate_heads = s.gate_heads;
     a.heads = l.heads; a.per_head = l.per_head; a.parts = l.parts; a.lg_tx = l.lg_tx;
@@ -693,15 +889,15 @@ int make_cut(const DsbRecurrence& s, bool forward, void* workspace, int64_t work
     a.x_stride = sign * s.x_stride; a.gate_stride = sign * s.gate_stride;
     a.h_stride = sign * s.channels; a.gate_out_stride = sign * s.gate_heads;
     unsigned char* w = static_cast<unsigned char*>(workspace);
-    if (a.chunks > 1) {
-        const int64_t maps = l.chains * a.chunks, bytes = up16(maps * s.channels * 4);
+    if (l.segments > 1) {
+        const int64_t maps = l.chains * l.segments, bytes = up16(maps * s.channels * 4);
         a.map_a = reinterpret_cast<float*>(w); w += bytes;
         a.map_b = reinterpret_cast<float*>(w); w += bytes;
         a.map_closed = reinterpret_cast<int*>(w); w += up16(maps * 4);
     }
     if (!forward && a.shared && l.parts > 1) a.gate_parts = reinterpret_cast<float*>(w);
-    c.tiles = l.chains * a.chunks * l.heads * l.parts;
-    DSB_REQUIRE(c.tiles <= kMaxRows, "recurrence: too many tiles for one launch");
+    c.blocks = l.chains * l.segments * l.heads * l.parts;
+    DSB_REQUIRE(c.blocks <= kMaxRows, "recurrence: too many blocks for one launch");
     return device_status_address(&a.device_status);
 }
 
@@ -721,33 +917,35 @@ int pass_states(const float* in, float* out, int64_t count, cudaStream_t s) {
     return DSB_OK;
 }
 
-template <typename T, int V, bool FORWARD>
-int run_tiles(const Cut& c, cudaStream_t s) {
-    const Args& a = c.args;
-    const bool table = c.layout.table;
-    constexpr int L = rows_per_thread(V, FORWARD);
-    const size_t smem = table ? 2 * sizeof(int) * tile_rows_of(c.layout, FORWARD) : 0;
-    const unsigned grid = (unsigned)c.tiles;
-    auto launch = [&](auto apply) {
-        constexpr bool APPLY = decltype(apply)::value;
-        if (FORWARD) {
-            if (table) recurrence_forward_kernel<T, V, L, true, APPLY><<<grid, kThreads, smem, s>>>(a);
-            else recurrence_forward_kernel<T, V, L, false, APPLY><<<grid, kThreads, smem, s>>>(a);
-        } else {
-            if (table) recurrence_backward_kernel<T, V, L, true, APPLY><<<grid, kThreads, smem, s>>>(a);
-            else recurrence_backward_kernel<T, V, L, false, APPLY><<<grid, kThreads, smem, s>>>(a);
-        }
-    };
-    if (a.chunks > 1) {
-        launch(std::false_type{});
-        DSB_LAUNCH_CHECK();
-        const unsigned carry_grid = (unsigned)((a.chains * a.channels + kThreads - 1) / kThreads);
-        recurrence_carry_kernel<FORWARD><<<carry_grid, kThreads, 0, s>>>(a);
-        DSB_LAUNCH_CHECK();
-    }
-    launch(std::true_type{});
+template <typename Kernel>
+int launch_walk(Kernel kernel, unsigned grid, size_t smem, const Args& a, cudaStream_t s) {
+    if (smem > 32 * 1024)   // beside the static part
+        DSB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    kernel<<<grid, kThreads, smem, s>>>(a);
     DSB_LAUNCH_CHECK();
     return DSB_OK;
+}
+
+template <typename T, int V, bool FORWARD>
+int run_walks(const Cut& c, cudaStream_t s) {
+    const Args& a = c.args;
+    const bool table = c.layout.table;
+    constexpr int L = rows_per_thread<T>(V);
+    const size_t smem = kStages * sizeof(Stage<T, V, L, FORWARD ? 2 : 3>) + (table ? kTables * 2 * sizeof(int) * c.layout.tile_rows : 0);
+    const unsigned grid = (unsigned)c.blocks;
+    auto launch = [&](auto apply) {
+        constexpr bool APPLY = decltype(apply)::value;
+        if (FORWARD)
+            return table ? launch_walk(recurrence_forward_kernel<T, V, L, true, APPLY>, grid, smem, a, s)
+                         : launch_walk(recurrence_forward_kernel<T, V, L, false, APPLY>, grid, smem, a, s);
+        return table ? launch_walk(recurrence_backward_kernel<T, V, L, true, APPLY>, grid, smem, a, s)
+                     : launch_walk(recurrence_backward_kernel<T, V, L, false, APPLY>, grid, smem, a, s);
+    };
+    if (a.segments > 1) {
+        const int rc = launch(std::false_type{});
+        if (rc != DSB_OK) return rc;
+    }
+    return launch(std::true_type{});
 }
 
 template <bool FORWARD>
@@ -755,7 +953,7 @@ int run_direction(const DsbRecurrence& shape, const Cut& c, cudaStream_t s) {
     int rc = DSB_OK;
     with_dtype(shape.dtype, [&](auto tag) {
         typedef decltype(tag) T;
-        rc = c.layout.vec == 4 ? run_tiles<T, 4, FORWARD>(c, s) : run_tiles<T, 1, FORWARD>(c, s);
+        rc = c.layout.vec == 4 ? run_walks<T, 4, FORWARD>(c, s) : run_walks<T, 1, FORWARD>(c, s);
         if (rc == DSB_OK && !FORWARD && c.args.gate_parts && c.args.v_gate) {
             const long long n = shape.rows * shape.gate_heads;
             T* out = static_cast<T*>(c.args.v_gate);
@@ -791,15 +989,15 @@ int check_inputs(const DsbRecurrence& s, const void* x, const void* gate) {
 
 int64_t recurrence_workspace_bytes(const DsbRecurrence& s) {
     if (check_shape(s, false) != DSB_OK) return 0;
-    const Layout l = layout_of(s, shape_vec(s));
+    const Layout l = layout_of(s);
     const int64_t f = direction_workspace(s, l, true), b = direction_workspace(s, l, false);
     return f > b ? f : b;
 }
 
 int64_t recurrence_checkpoint_bytes(const DsbRecurrence& s) {
     if (check_shape(s, false) != DSB_OK) return 0;
-    const Layout l = layout_of(s, shape_vec(s));
-    return l.chains * chunks_of(l, false) * s.channels * 4;
+    const Layout l = layout_of(s);
+    return l.chains * l.tiles * s.channels * 4;
 }
 
 int launch_recurrence_forward(const DsbRecurrence& shape, const void* x, const void* gate, const float* state_in, void* h,
