@@ -1,0 +1,870 @@
+// The walk of the gated recurrence (recurrence.cu has its formulas and entry points), forward and backward.
+//
+// A stretch of rows maps the state before it to the state after it as h -> a h + b, and two stretches compose as
+// (a2 a1, a2 b1 + b2); a stretch in which a sequence begins maps every h to b ("closed": its a is never looked at, so
+// that an infinity of the sequence before cannot meet a zero).
+//
+// A block walks along one stretch of rows and a block of channels, tile by tile, and carries the state in registers: it
+// reads everything once and writes everything once.  Inside a tile a thread runs L consecutive rows of V channels, a warp
+// composes its threads' maps with shuffles, the block its warps' through shared memory (one barrier a tile); the next
+// tile's rows are on their way into shared memory meanwhile (each thread copies what it will read itself, so their arrival
+// needs no barrier).  Where sequences and channels alone make too few blocks for the GPU, a sequence is cut into segments:
+// a first launch leaves every segment's map, and each block of the second starts from the composition of those before it.
+// That reads the inputs twice, the second time mostly from L2 where the call is small enough to need it.
+//
+// The backward walks from the last row to the first on q.  It needs h_{t-1}, and recomputes it in 32 bits from states that the
+// forward leaves at every thread's first row (a 32-bit value per L rows and channel): the h that was written out is
+// rounded to the storage type and need not be kept, and no second composition is needed.
+//
+// Every order of composition is fixed by the shape alone, so results do not depend on timing; no block waits for another.
+//
+// What bounds it: instruction issue.  A tile without a sequence border ("plain") therefore has code of its own without any
+// test per row, and the form of the gate, the coupling and shared gates are template parameters.
+#pragma once
+#include <type_traits>
+
+#include "vector_io.cuh"
+
+namespace dsb {
+
+struct RecurrenceArgs {
+    const void *x, *gate, *v_h;
+    void *h, *v_x, *v_gate;
+    const float *state_in, *v_state_out;
+    float *state_out, *v_state_in;
+    float* checkpoints;    // [chains][tiles][groups of L rows][channels]: the state before each group
+    float *map_a, *map_b;  // [chains][segments][channels]
+    int* map_closed;       // [chains][segments]
+    float* gate_parts;     // [parts][rows][heads], when a head spans several channel blocks
+    const int *offsets, *lengths;
+    int* device_status;
+    long long rows, chain_rows, chains;
+    long long x_stride, gate_stride, v_h_stride;   // negative when the scan runs from the last row to the first
+    long long h_stride, gate_out_stride;           // channels / heads of contiguous results, with the same sign
+    long long tiles, segments, segment_tiles;
+    int sequences, sequence_rows, channels, gate_heads, heads, per_head, parts, lg_tx;
+    int reverse, table;    // table: one chain over all rows, with sequence borders anywhere; else one chain per sequence
+    int logit, coupled, shared;
+};
+struct RecurrenceLaunch {
+    RecurrenceArgs args;
+    int vec, tile_rows;
+    unsigned blocks;
+};
+template <typename T> int run_recurrence_forward(const RecurrenceLaunch& c, cudaStream_t s);
+template <typename T> int run_recurrence_backward(const RecurrenceLaunch& c, cudaStream_t s);
+
+constexpr int kWalkThreads = 128;
+constexpr int kWalkWarps = kWalkThreads / 32;
+
+// Consecutive rows of a thread: as many as keep the backward's values of a tile in registers and two tiles of every tensor
+// in shared memory with several blocks on an SM.
+template <typename T> __host__ __device__ constexpr int walk_rows(int vec) { return vec == 4 ? (sizeof(T) == 4 ? 4 : 8) : 16; }
+
+// ---- gates ---------------------------------------------------------------------------------------------------------
+// exp(-|g|) and 1 / (1 + exp(-|g|)): the smaller of f and 1 - f is their product, the other the second.  Both keep full
+// relative precision, however close to 0 or 1 the gate is.
+__device__ __forceinline__ void logistic_parts(float g, float& t, float& r) {
+    float y;
+    asm("max.NaN.f32 %0, %1, 0fC2B40000;" : "=f"(y) : "f"(-fabsf(g)));   // -90: 2^(y log2 e) is flushed to 0; NaN stays NaN
+    const float hi = y * 1.44269502f;                 // exp(y) = 2^(y log2 e), the product's rounding error added back
+    const float lo = fmaf(y, 1.44269502f, -hi);       // to first order
+    t = exp2f(hi);
+    t = fmaf(t, lo * 0.693147181f, t);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + t));
+}
+template <bool LOGIT>
+__device__ __forceinline__ void gate_pair(float g, float& f, float& k) {
+    if (LOGIT) {
+        float t, r;
+        logistic_parts(g, t, r);
+        const float small = t * r;
+        f = g < 0.f ? small : r;
+        k = g < 0.f ? r : small;
+    } else {
+        f = g;
+        k = 1.f - g;
+    }
+}
+// One register that holds both: the smaller one with the sign saying which it is.
+template <bool LOGIT>
+__device__ __forceinline__ float encode_gate(float g) {
+    if (!LOGIT) return g;
+    float t, r;
+    logistic_parts(g, t, r);
+    return copysignf(t * r, g);
+}
+template <bool LOGIT>
+__device__ __forceinline__ void decode_gate(float m, float& f, float& k) {
+    if (LOGIT) {
+        const float rest = 1.f - fabsf(m);
+        const bool small_f = __float_as_int(m) < 0;
+        f = small_f ? fabsf(m) : rest;
+        k = small_f ? rest : fabsf(m);
+    } else {
+        f = m;
+        k = 1.f - m;
+    }
+}
+
+// ---- rows that begin and end sequences ------------------------------------------------------------------------------
+// In the order of the scan: position p is row p, or rows - 1 - p when the scan runs backwards; sequence k of the scan is
+// the tensor's sequence k, or sequences - 1 - k.
+constexpr int kNone = -1, kOutside = -2;
+constexpr int kTables = 3;      // one is read, one was read by the slowest warp, one is written
+
+__device__ __forceinline__ int sequence_id(const RecurrenceArgs& a, int k) { return a.reverse ? a.sequences - 1 - k : k; }
+// Where the scan's packed sequence k begins (k = sequences: where the last one ends).
+__device__ __forceinline__ long long packed_start(const RecurrenceArgs& a, long long k) {
+    return a.reverse ? a.rows - a.offsets[a.sequences - k] : a.offsets[k];
+}
+// How many of packed_start(shift .. shift + sequences - 1) are <= p; called by one whole warp.
+__device__ __forceinline__ int starts_up_to(const RecurrenceArgs& a, int shift, long long p) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, len = a.sequences;
+    while (len > 0) {
+        const int step = (len + 31) / 32;
+        const long long at = (long long)lane * step;
+        const bool below = at < len && packed_start(a, shift + lo + at) <= p;
+        const int below_count = __popc(__ballot_sync(0xffffffffu, below));
+        if (below_count == 0) break;
+        const int skip = (below_count - 1) * step + 1;
+        len = min(step - 1, len - skip);
+        lo += skip;
+    }
+    return lo;
+}
+
+enum TileKind { kPlain, kBorders, kEmpty };   // no border and every row in a sequence; anything; no row in a sequence
+
+// Follows a walk from tile to tile (FORWARD: upwards): what kind of tile comes, and for tiles with borders the tables
+// first[r] / end[r]: the sequence that begins / ends at the tile's row r, kNone, or (first only) kOutside.  Every member is
+// the same in all threads of the block.
+template <bool FORWARD>
+struct Borders {
+    long long lo, hi;      // the sequence last met holds positions [lo, hi)
+    int sequence;          // chain per sequence: its id.  Packed: where to look on, as a sequence of the scan
+    int* tables;
+    int tile_rows;
+
+    __device__ void begin(const RecurrenceArgs& a, int chain, long long p0, int* s_tables, int rows) {
+        tables = s_tables;
+        tile_rows = rows;
+        lo = 1; hi = 0;
+        if (!a.table) {
+            sequence = sequence_id(a, chain);
+            long long len = a.sequence_rows;
+            if (a.lengths) len = min(max(a.lengths[sequence], 0), a.sequence_rows);
+            lo = a.reverse ? a.sequence_rows - len : 0;
+            hi = lo + len;
+        } else if (a.sequence_rows == 0) {
+            // FORWARD: the first sequence to end after p0; else the last to begin before the tile's end
+            __shared__ int s_at;
+            if (threadIdx.x < 32) {
+                const int n = FORWARD ? starts_up_to(a, 1, p0) : starts_up_to(a, 0, p0 + rows - 1) - 1;
+                if (threadIdx.x == 0) s_at = n;
+            }
+            __syncthreads();
+            sequence = s_at;
+            look(a);
+        }
+    }
+    __device__ void look(const RecurrenceArgs& a) {   // packed: the bounds of the sequence the cursor stands at
+        const bool any = sequence >= 0 && sequence < a.sequences;
+        lo = any ? packed_start(a, sequence) : 1;
+        hi = any ? packed_start(a, sequence + 1) : 0;
+    }
+    __device__ int* first(long long t) const { return tables + (int)(t % kTables) * 2 * tile_rows; }
+    __device__ int* end(long long t) const { return first(t) + tile_rows; }
+
+    // Tile t at p0; called by the whole block, tile after tile.  Tables are there after the next barrier.
+    __device__ int prepare(const RecurrenceArgs& a, long long t, long long p0) {
+        const long long p1 = p0 + tile_rows;
+        if (p0 > lo && p1 < hi) return kPlain;
+        if (!a.table && (p1 <= lo || p0 >= hi)) return kEmpty;
+        int *f = first(t), *e = end(t);
+        const int tid = threadIdx.x;
+        if (!a.table) {
+            for (int r = tid; r < tile_rows; r += kWalkThreads) {
+                const long long p = p0 + r;
+                f[r] = p < lo || p >= hi ? kOutside : p == lo ? sequence : kNone;
+                e[r] = p == hi - 1 ? sequence : kNone;
+            }
+            return kBorders;
+        }
+        if (a.sequence_rows > 0) {
+            for (int r = tid; r < tile_rows; r += kWalkThreads) {
+                const long long p = p0 + r;
+                int b = kOutside, c = kNone;
+                if (p < a.rows) {
+                    const int turn = (int)(p / a.sequence_rows), pos = (int)(p - (long long)turn * a.sequence_rows);
+                    const int seq = sequence_id(a, turn);
+                    const int len = a.lengths ? min(max(a.lengths[seq], 0), a.sequence_rows) : a.sequence_rows;
+                    const int at = a.reverse ? a.sequence_rows - len : 0;
+                    if (pos >= at && pos < at + len) {
+                        b = pos == at ? seq : kNone;
+                        c = pos == at + len - 1 ? seq : kNone;
+                    }
+                }
+                f[r] = b;
+                e[r] = c;
+            }
+            return kBorders;
+        }
+        const long long last = min(p1, a.rows);
+        const long long all0 = packed_start(a, 0), all1 = packed_start(a, a.sequences);
+        for (int r = tid; r < tile_rows; r += kWalkThreads) {
+            const long long p = p0 + r;
+            f[r] = p < last && p >= all0 && p < all1 ? kNone : kOutside;
+            e[r] = kNone;
+        }
+        __syncthreads();
+        int done;
+        do {   // offsets out of order may lead this astray, but every access stays where it belongs
+            const long long k = FORWARD ? (long long)sequence + tid : (long long)sequence - tid;
+            bool through = false;
+            if (k >= 0 && k < a.sequences) {
+                const long long o0 = packed_start(a, k), o1 = packed_start(a, k + 1);
+                if (o0 < o1) {
+                    const int id = sequence_id(a, (int)k);
+                    if (o0 >= p0 && o0 < last) f[o0 - p0] = id;
+                    if (o1 > p0 && o1 <= last) e[o1 - 1 - p0] = id;
+                }
+                through = FORWARD ? o1 <= p1 : o0 >= p0;
+            }
+            done = __syncthreads_count(through);
+            sequence += FORWARD ? done : -done;
+        } while (done == kWalkThreads);
+        look(a);
+        return kBorders;
+    }
+};
+
+// Sequences without rows hand their state on; offsets and lengths out of order or range are reported.
+__device__ __forceinline__ void pass_empty_sequences(const RecurrenceArgs& a, const float* in, float* out) {
+    if (!a.offsets && !a.lengths) return;
+    const long long step = (long long)gridDim.x * kWalkThreads;
+    for (long long s = (long long)blockIdx.x * kWalkThreads + threadIdx.x; s < a.sequences; s += step) {
+        bool empty, bad;
+        if (a.offsets) {
+            const long long o0 = a.offsets[s], o1 = a.offsets[s + 1];
+            empty = o1 <= o0;
+            bad = o1 < o0 || o0 < 0 || o1 > a.rows;
+        } else {
+            const int len = a.lengths[s];
+            empty = len <= 0;
+            bad = len < 0 || len > a.sequence_rows;
+        }
+        if (bad) atomicMin(a.device_status, DSB_ERR_INVALID_ARGUMENT);
+        if ((empty || bad) && out)
+            for (int c = 0; c < a.channels; ++c) out[s * a.channels + c] = in ? in[s * a.channels + c] : 0.f;
+    }
+}
+
+// ---- maps and their composition ----------------------------------------------------------------------------------------
+// A is V, or 1 where all channels of a thread share the gate.
+template <int V, int A>
+struct Map {
+    float a[A], b[V];
+    int closed;
+};
+template <int V, int A>
+__device__ __forceinline__ void identity(Map<V, A>& m) {
+#pragma unroll
+    for (int v = 0; v < A; ++v) m.a[v] = 1.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) m.b[v] = 0.f;
+    m.closed = 0;
+}
+// m <- m after e (e comes first along the scan).  PLAIN: neither is closed.
+template <bool PLAIN, int V, int A>
+__device__ __forceinline__ void compose_after(Map<V, A>& m, const Map<V, A>& e) {
+    const bool open = PLAIN || !m.closed;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const float b = fmaf(m.a[v % A], e.b[v], m.b[v]);
+        m.b[v] = open ? b : m.b[v];
+    }
+#pragma unroll
+    for (int v = 0; v < A; ++v) m.a[v] *= e.a[v];
+    if (!PLAIN) m.closed |= e.closed;
+}
+template <bool PLAIN, int V, int A>
+__device__ __forceinline__ void apply_map(float (&h)[V], const Map<V, A>& m) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const float n = fmaf(m.a[v % A], h[v], m.b[v]);
+        h[v] = PLAIN || !m.closed ? n : m.b[v];
+    }
+}
+
+// The warps' maps of one tile.
+template <int V, int A>
+struct alignas(16) WarpMaps {     // read and written V (A) floats at a time
+    float b[kWalkWarps][32 * V];
+    float a[kWalkWarps][32 * A];
+    int closed[kWalkWarps];
+};
+
+// Lanes that hold the same channels on consecutive row groups are tx apart.  From every thread's own map: the warp's
+// total in shared memory, and the map of the warp's rows before this thread's.  FORWARD: rows run with the lane; else
+// against it.
+template <bool FORWARD, bool PLAIN, int V, int A>
+__device__ __forceinline__ Map<V, A> compose_warp(const Map<V, A>& own, int lg_tx, WarpMaps<V, A>& sh) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tx = 1 << lg_tx;
+    Map<V, A> run = own;
+    auto from = [&](auto value, int off) {
+        return FORWARD ? __shfl_up_sync(0xffffffffu, value, off) : __shfl_down_sync(0xffffffffu, value, off);
+    };
+    for (int off = tx; off < 32; off <<= 1) {
+        Map<V, A> e;
+#pragma unroll
+        for (int v = 0; v < A; ++v) e.a[v] = from(run.a[v], off);
+#pragma unroll
+        for (int v = 0; v < V; ++v) e.b[v] = from(run.b[v], off);
+        e.closed = PLAIN ? 0 : from(run.closed, off);
+        if (FORWARD ? lane >= off : lane + off < 32) compose_after<PLAIN>(run, e);
+    }
+    if (FORWARD ? lane >= 32 - tx : lane < tx) {
+        const int at = lane & (tx - 1);
+        store_floats<float, A>(&sh.a[warp][at * A], run.a);
+        store_floats<float, V>(&sh.b[warp][at * V], run.b);
+        if (!PLAIN && at == 0) sh.closed[warp] = run.closed;
+    }
+    Map<V, A> before;
+    identity(before);
+    if (tx < 32) {
+#pragma unroll
+        for (int v = 0; v < A; ++v) before.a[v] = from(run.a[v], tx);
+#pragma unroll
+        for (int v = 0; v < V; ++v) before.b[v] = from(run.b[v], tx);
+        if (!PLAIN) before.closed = from(run.closed, tx);
+        if (FORWARD ? lane < tx : lane >= 32 - tx) identity(before);
+    }
+    return before;
+}
+template <bool PLAIN, int V, int A>
+__device__ __forceinline__ Map<V, A> warp_map(const WarpMaps<V, A>& sh, int warp, int tx) {
+    Map<V, A> m;
+    const Pack<float, A> pa = load_pack<float, A>(&sh.a[warp][tx * A]);
+    const Pack<float, V> pb = load_pack<float, V>(&sh.b[warp][tx * V]);
+#pragma unroll
+    for (int v = 0; v < A; ++v) m.a[v] = pa.e[v];
+#pragma unroll
+    for (int v = 0; v < V; ++v) m.b[v] = pb.e[v];
+    m.closed = PLAIN ? 0 : sh.closed[warp];
+    return m;
+}
+// carry: the state before the tile -> the state after it; mine: the state before this thread's warp.
+template <bool FORWARD, bool PLAIN, int V, int A>
+__device__ __forceinline__ void pass_warps(const WarpMaps<V, A>& sh, int tx, float (&carry)[V], float (&mine)[V]) {
+    const int warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int i = 0; i < kWalkWarps; ++i) {
+        const int w = FORWARD ? i : kWalkWarps - 1 - i;
+        if (w == warp) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) mine[v] = carry[v];
+        }
+        apply_map<PLAIN>(carry, warp_map<PLAIN>(sh, w, tx));
+    }
+}
+
+// ---- a block's place -----------------------------------------------------------------------------------------------------
+struct Place {
+    int chain, head, part, channel, tx;
+    long long segment;
+    int row0, group;       // this thread's first row inside a tile, and which of the tile's groups of rows that is
+    bool active;
+};
+template <int V, int L>
+__device__ __forceinline__ Place place_of(const RecurrenceArgs& a) {
+    Place p;
+    const int blocks = a.heads * a.parts;
+    const long long rest = blockIdx.x / blocks;
+    const int block = (int)(blockIdx.x - rest * blocks);
+    p.chain = (int)(rest % a.chains);
+    p.segment = rest / a.chains;
+    p.head = block / a.parts;
+    p.part = block - p.head * a.parts;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    p.tx = lane & ((1 << a.lg_tx) - 1);
+    p.group = warp * (32 >> a.lg_tx) + (lane >> a.lg_tx);
+    p.row0 = p.group * L;
+    const int c = (p.part << a.lg_tx) * V + p.tx * V;
+    p.active = c < a.per_head;
+    p.channel = p.head * a.per_head + c;
+    return p;
+}
+
+template <int V>
+__device__ __forceinline__ void load_state(const float* states, long long index, int channels, int channel, float (&o)[V]) {
+    if (!states) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] = 0.f;
+        return;
+    }
+    const Pack<float, V> q = load_pack<float, V>(states + index * channels + channel);
+#pragma unroll
+    for (int v = 0; v < V; ++v) o[v] = q.e[v];
+}
+
+// ---- rows on their way through shared memory ---------------------------------------------------------------------------
+template <typename T, int V>
+__device__ __forceinline__ void copy_async(T* to, const T* from, bool there) {
+    constexpr int kBytes = V * sizeof(T);
+    if (kBytes == 2) {                            // below what an asynchronous copy takes
+        T v;
+        memset(&v, 0, kBytes);
+        if (there) v = *from;
+        *to = v;
+    } else {
+        const unsigned at = (unsigned)__cvta_generic_to_shared(to);
+        const int bytes = there ? kBytes : 0;     // what is not copied is filled with zeros
+        if (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(bytes) : "memory");
+        else if (kBytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(at), "l"(from), "r"(bytes) : "memory");
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(at), "l"(from), "r"(bytes) : "memory");
+    }
+}
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_landed() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+// Lanes lie side by side, so that neither the copies nor the reads meet a bank twice.
+template <typename T, int V, int L, int TENSORS>
+struct alignas(16) TileStage {
+    T v[TENSORS][L][kWalkThreads][V];
+};
+
+// This thread's rows of a tile; rows past the chain's end become zeros.  Rows that belong to no sequence but lie within the
+// tensor are copied like the others and masked where they are used.
+template <typename T, int V, int L>
+__device__ __forceinline__ void fetch_rows(T (*to)[kWalkThreads][V], const T* base, long long stride, const RecurrenceArgs& a,
+                                           const Place& p, long long p0) {
+    const long long at = p0 + p.row0;
+    const T* from = base + (p.chain * a.chain_rows + at) * stride;
+    const int left = p.active ? (int)min(a.chain_rows - at, (long long)L) : 0;
+    if (left == L) {
+#pragma unroll
+        for (int l = 0; l < L; ++l, from += stride) copy_async<T, V>(to[l][threadIdx.x], from, true);
+    } else {
+#pragma unroll
+        for (int l = 0; l < L; ++l) copy_async<T, V>(to[l][threadIdx.x], l < left ? from + l * stride : base, l < left);
+    }
+}
+// Gates of their own come like x; a shared one is read directly, as every thread of a row wants the same value.
+template <bool SHARED, typename T, int V, int L>
+__device__ __forceinline__ void fetch_gates(T (*to)[kWalkThreads][V], T (&own)[L], const RecurrenceArgs& a, const Place& p,
+                                            long long p0) {
+    const T* base = static_cast<const T*>(a.gate) + (SHARED ? p.head : p.channel);
+    if (!SHARED) {
+        fetch_rows<T, V, L>(to, base, a.gate_stride, a, p, p0);
+        return;
+    }
+    const long long at = p0 + p.row0;
+    const T* from = base + (p.chain * a.chain_rows + at) * a.gate_stride;
+    const int left = p.active ? (int)min(a.chain_rows - at, (long long)L) : 0;
+#pragma unroll
+    for (int l = 0; l < L; ++l) {
+        memset(&own[l], 0, sizeof(T));
+        if (l < left) own[l] = from[l * a.gate_stride];
+    }
+}
+
+// The state (or q) at the segment's beginning: the maps of the segments before it, each warp a share of them, in order.
+template <bool FORWARD, int V, int A>
+__device__ void carry_of_segment(const RecurrenceArgs& a, const Place& p, WarpMaps<V, A>& sh, float (&carry)[V]) {
+    const long long before = FORWARD ? p.segment : a.segments - 1 - p.segment;
+#pragma unroll
+    for (int v = 0; v < V; ++v) carry[v] = 0.f;
+    if (before == 0) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long share = (before + kWalkWarps - 1) / kWalkWarps;
+    const long long i0 = min(share * warp, before), i1 = min(i0 + share, before);
+    if (lane < (1 << a.lg_tx)) {
+        Map<V, A> all;
+        identity(all);
+#pragma unroll 4
+        for (long long i = i0; i < i1; ++i) {
+            const long long at = p.chain * a.segments + (FORWARD ? i : a.segments - 1 - i);
+            Map<V, A> m;
+            identity(m);
+            m.closed = a.map_closed[at];
+            if (p.active) {
+                const Pack<float, V> pa = load_pack<float, V>(a.map_a + at * a.channels + p.channel);
+                const Pack<float, V> pb = load_pack<float, V>(a.map_b + at * a.channels + p.channel);
+#pragma unroll
+                for (int v = 0; v < A; ++v) m.a[v] = pa.e[v];
+#pragma unroll
+                for (int v = 0; v < V; ++v) m.b[v] = pb.e[v];
+            }
+            compose_after<false>(m, all);
+            all = m;
+        }
+        store_floats<float, A>(&sh.a[warp][p.tx * A], all.a);
+        store_floats<float, V>(&sh.b[warp][p.tx * V], all.b);
+        if (p.tx == 0) sh.closed[warp] = all.closed;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWalkWarps; ++w) apply_map<false>(carry, warp_map<false>(sh, w, p.tx));
+    __syncthreads();
+}
+
+// Leaves the composition of a whole segment's tiles.
+template <int V, int A>
+__device__ __forceinline__ void store_segment_map(const RecurrenceArgs& a, const Place& p, const Map<V, A>& all) {
+    if (threadIdx.x >= (1 << a.lg_tx) || !p.active) return;
+    const long long at = p.chain * a.segments + p.segment;
+    float wide[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) wide[v] = all.a[v % A];
+    store_floats<float, V>(a.map_a + at * a.channels + p.channel, wide);
+    store_floats<float, V>(a.map_b + at * a.channels + p.channel, all.b);
+    if (p.tx == 0) a.map_closed[at] = all.closed;
+}
+
+// A tile of rows that belong to no sequence.
+template <typename T, int V, int L>
+__device__ __forceinline__ void store_zero_rows(T* to, long long stride, int left, bool active) {
+    const float zero[V] = {};
+#pragma unroll
+    for (int l = 0; l < L; ++l)
+        if (active && l < left) store_floats<T, V>(to + l * stride, zero);
+}
+
+template <typename T, int V, bool LOGIT, bool COUPLED, bool SHARED, bool APPLY>
+__global__ void __launch_bounds__(kWalkThreads, 4)
+recurrence_forward_kernel(const RecurrenceArgs a) {
+    constexpr int L = walk_rows<T>(V), A = SHARED ? 1 : V;
+    typedef TileStage<T, V, L, SHARED ? 1 : 2> Ring;
+    extern __shared__ __align__(16) unsigned char s_raw[];
+    Ring* ring = reinterpret_cast<Ring*>(s_raw);
+    __shared__ WarpMaps<V, A> sh[2];
+    const int tile_rows = kWalkWarps * (32 >> a.lg_tx) * L;
+    const Place p = place_of<V, L>(a);
+    const long long t0 = p.segment * a.segment_tiles, t1 = min(t0 + a.segment_tiles, a.tiles);
+    const T* x = static_cast<const T*>(a.x) + p.channel;
+
+    float carry[V];
+    Map<V, A> all;
+    identity(all);
+    if (APPLY) carry_of_segment<true>(a, p, sh[0], carry);
+    Borders<true> borders;
+    borders.begin(a, p.chain, t0 * tile_rows, reinterpret_cast<int*>(s_raw + 2 * sizeof(Ring)), tile_rows);
+    T gate_now[L], gate_next[L];
+    auto fetch = [&](int stage, long long t) {
+        fetch_rows<T, V, L>(ring[stage].v[0], x, a.x_stride, a, p, t * tile_rows);
+        fetch_gates<SHARED, T, V, L>(ring[stage].v[SHARED ? 0 : 1], gate_next, a, p, t * tile_rows);
+    };
+    int kind = borders.prepare(a, t0, t0 * tile_rows), kind_next = kEmpty;
+    if (kind != kEmpty) fetch(0, t0);
+    copies_issued();
+    __syncthreads();
+    for (long long t = t0; t < t1; ++t, kind = kind_next) {
+        const int stage = (int)(t - t0) & 1;
+        const long long p0 = t * tile_rows;
+        if (SHARED) {
+#pragma unroll
+            for (int l = 0; l < L; ++l) gate_now[l] = gate_next[l];
+        }
+        if (t + 1 < t1) {
+            kind_next = borders.prepare(a, t + 1, p0 + tile_rows);
+            if (kind_next != kEmpty) fetch(stage ^ 1, t + 1);
+        }
+        copies_issued();
+        copies_landed<1>();
+        const int left = (int)min(a.chain_rows - p0 - p.row0, (long long)L);
+        T* ph = APPLY && a.h ? static_cast<T*>(a.h) + (p.chain * a.chain_rows + p0 + p.row0) * a.h_stride + p.channel : nullptr;
+        if (kind == kEmpty) {
+            if (ph) store_zero_rows<T, V, L>(ph, a.h_stride, left, p.active);
+            __syncthreads();
+            continue;
+        }
+        auto tile = [&](auto plain) {
+            constexpr bool PLAIN = decltype(plain)::value;
+            const int *first = borders.first(t) + p.row0, *end = borders.end(t) + p.row0;
+            float f[L][A], b[L][V];
+            Map<V, A> own;
+            identity(own);
+#pragma unroll
+            for (int l = 0; l < L; ++l) {
+                const int s = PLAIN ? kNone : first[l];
+                const bool outside = s == kOutside;
+                const Pack<T, V> px = load_pack<T, V>(ring[stage].v[0][l][threadIdx.x]);
+                Pack<T, A> pg;
+                if (SHARED) pg.e[0] = gate_now[l];
+                else pg = load_pack<T, A>(&ring[stage].v[SHARED ? 0 : 1][l][threadIdx.x][0]);
+                if (s >= 0) {          // the state before this row is the sequence's own, whatever came before
+                    load_state<V>(p.active ? a.state_in : nullptr, s, a.channels, p.channel, own.b);
+                    own.closed = 1;
+                }
+                float k[A];
+#pragma unroll
+                for (int v = 0; v < A; ++v) {
+                    gate_pair<LOGIT>(to_float(pg.e[v]), f[l][v], k[v]);
+                    if (outside) f[l][v] = 1.f;
+                    own.a[v] *= f[l][v];
+                }
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const float xv = to_float(px.e[v]);
+                    b[l][v] = outside ? 0.f : COUPLED ? xv * k[v % A] : xv;
+                    own.b[v] = fmaf(f[l][v % A], own.b[v], b[l][v]);
+                }
+            }
+            const Map<V, A> before = compose_warp<true, PLAIN>(own, a.lg_tx, sh[stage]);
+            __syncthreads();
+            if (!APPLY) {
+#pragma unroll
+                for (int w = 0; w < kWalkWarps; ++w) {
+                    Map<V, A> m = warp_map<PLAIN>(sh[stage], w, p.tx);
+                    const int closed = all.closed;
+                    compose_after<PLAIN>(m, all);
+                    if (PLAIN) m.closed = closed;
+                    all = m;
+                }
+                return;
+            }
+            float h[V];
+            pass_warps<true, PLAIN>(sh[stage], p.tx, carry, h);
+            apply_map<PLAIN>(h, before);
+            if (a.checkpoints && p.active)
+                store_floats<float, V>(a.checkpoints + ((p.chain * a.tiles + t) * (kWalkWarps * (32 >> a.lg_tx)) + p.group) * a.channels + p.channel, h);
+            T* to = ph;
+#pragma unroll
+            for (int l = 0; l < L; ++l) {
+                const int s = PLAIN ? kNone : first[l], e = PLAIN ? kNone : end[l];
+                if (s >= 0) load_state<V>(p.active ? a.state_in : nullptr, s, a.channels, p.channel, h);
+                float o[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    h[v] = fmaf(f[l][v % A], h[v], b[l][v]);
+                    o[v] = s == kOutside ? 0.f : h[v];
+                }
+                if (ph && p.active && (PLAIN || l < left)) store_floats<T, V>(to, o);
+                to += a.h_stride;
+                if (e >= 0 && p.active) store_floats<float, V>(a.state_out + (long long)e * a.channels + p.channel, h);
+            }
+        };
+        if (kind == kPlain) tile(std::true_type{});
+        else tile(std::false_type{});
+    }
+    if (APPLY) pass_empty_sequences(a, a.state_in, a.state_out);
+    else store_segment_map(a, p, all);
+}
+
+template <typename T, int V, bool LOGIT, bool COUPLED, bool SHARED, bool APPLY>
+__global__ void __launch_bounds__(kWalkThreads, 3)
+recurrence_backward_kernel(const RecurrenceArgs a) {
+    constexpr int L = walk_rows<T>(V), A = SHARED ? 1 : V;
+    constexpr int kX = 1, kGate = 2;                    // places in a stage; v_h has the first
+    typedef TileStage<T, V, L, 1 + (APPLY ? 1 : 0) + (SHARED ? 0 : 1)> Ring;
+    constexpr int kGateAt = SHARED ? 0 : APPLY ? kGate : 1, kXAt = APPLY ? kX : 0;
+    extern __shared__ __align__(16) unsigned char s_raw[];
+    Ring* ring = reinterpret_cast<Ring*>(s_raw);
+    __shared__ WarpMaps<V, A> sh[2];
+    const int tile_rows = kWalkWarps * (32 >> a.lg_tx) * L;
+    const Place p = place_of<V, L>(a);
+    const long long t0 = p.segment * a.segment_tiles, t1 = min(t0 + a.segment_tiles, a.tiles);
+    const T* x = static_cast<const T*>(a.x) + p.channel;
+    const T* vh = static_cast<const T*>(a.v_h) + p.channel;
+
+    float q_carry[V], start[V], start_next[V];
+    Map<V, A> all;
+    identity(all);
+    if (APPLY) carry_of_segment<false>(a, p, sh[0], q_carry);
+    Borders<false> borders;
+    borders.begin(a, p.chain, (t1 - 1) * tile_rows, reinterpret_cast<int*>(s_raw + 2 * sizeof(Ring)), tile_rows);
+    T gate_now[L], gate_next[L];
+    auto fetch = [&](int stage, long long t) {
+        if (a.v_h) fetch_rows<T, V, L>(ring[stage].v[0], vh, a.v_h_stride, a, p, t * tile_rows);
+        fetch_gates<SHARED, T, V, L>(ring[stage].v[kGateAt], gate_next, a, p, t * tile_rows);
+        if (APPLY) {
+            fetch_rows<T, V, L>(ring[stage].v[kXAt], x, a.x_stride, a, p, t * tile_rows);
+            load_state<V>(p.active ? a.checkpoints : nullptr, (p.chain * a.tiles + t) * (kWalkWarps * (32 >> a.lg_tx)) + p.group,
+                          a.channels, p.channel, start_next);
+        }
+    };
+    int kind = borders.prepare(a, t1 - 1, (t1 - 1) * tile_rows), kind_next = kEmpty;
+    if (kind != kEmpty) fetch(0, t1 - 1);
+    copies_issued();
+    __syncthreads();
+    for (long long t = t1 - 1; t >= t0; --t, kind = kind_next) {
+        const int stage = (int)(t1 - 1 - t) & 1;
+        const long long p0 = t * tile_rows;
+        if (SHARED) {
+#pragma unroll
+            for (int l = 0; l < L; ++l) gate_now[l] = gate_next[l];
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) start[v] = start_next[v];
+        if (t > t0) {
+            kind_next = borders.prepare(a, t - 1, p0 - tile_rows);
+            if (kind_next != kEmpty) fetch(stage ^ 1, t - 1);
+        }
+        copies_issued();
+        copies_landed<1>();
+        const long long row = p.chain * a.chain_rows + p0 + p.row0;
+        const int left = (int)min(a.chain_rows - p0 - p.row0, (long long)L);
+        T* px = APPLY && a.v_x ? static_cast<T*>(a.v_x) + row * a.h_stride + p.channel : nullptr;
+        T* pg = APPLY && a.v_gate && !SHARED ? static_cast<T*>(a.v_gate) + row * a.gate_out_stride + p.channel : nullptr;
+        // a shared gate's sum over this block's channels
+        auto store_gate_sum = [&](int l, float sum) {
+            const long long o = (row + l) * a.gate_out_stride + p.head;
+            if (a.parts == 1) from_float(sum, static_cast<T*>(a.v_gate)[o]);
+            else a.gate_parts[(a.reverse ? (a.rows - 1) * a.gate_heads + o : o) + (long long)p.part * a.rows * a.gate_heads] = sum;
+        };
+        if (kind == kEmpty) {
+            if (px) store_zero_rows<T, V, L>(px, a.h_stride, left, p.active);
+            if (pg) store_zero_rows<T, V, L>(pg, a.gate_out_stride, left, p.active);
+            if (APPLY && SHARED && a.v_gate && p.tx == 0)
+                for (int l = 0; l < left; ++l) store_gate_sum(l, 0.f);
+            __syncthreads();
+            continue;
+        }
+        auto tile = [&](auto plain) {
+            constexpr bool PLAIN = decltype(plain)::value;
+            const int *first = borders.first(t) + p.row0, *end = borders.end(t) + p.row0;
+            float m[L][A], u[L][V];
+            Map<V, A> own;
+            identity(own);
+#pragma unroll
+            for (int l = L - 1; l >= 0; --l) {
+                const bool outside = !PLAIN && first[l] == kOutside;
+                const int e = PLAIN ? kNone : end[l];
+                Pack<T, A> g;
+                if (SHARED) g.e[0] = gate_now[l];
+                else g = load_pack<T, A>(&ring[stage].v[kGateAt][l][threadIdx.x][0]);
+                Pack<T, V> d;
+                if (a.v_h) d = load_pack<T, V>(ring[stage].v[0][l][threadIdx.x]);
+                if (e >= 0) {
+                    load_state<V>(p.active ? a.v_state_out : nullptr, e, a.channels, p.channel, own.b);
+                    own.closed = 1;
+                }
+                float f[A], k;
+#pragma unroll
+                for (int v = 0; v < A; ++v) {
+                    m[l][v] = encode_gate<LOGIT>(to_float(g.e[v]));
+                    decode_gate<LOGIT>(m[l][v], f[v], k);
+                    if (outside) f[v] = 1.f;
+                    own.a[v] *= f[v];
+                }
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    own.b[v] = f[v % A] * ((a.v_h && !outside ? to_float(d.e[v]) : 0.f) + own.b[v]);
+            }
+            const Map<V, A> after = compose_warp<false, PLAIN>(own, a.lg_tx, sh[stage]);
+            if (APPLY) {                       // u_t: h_{t-1}, coupled: h_{t-1} - x_t
+                float h[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) h[v] = start[v];
+#pragma unroll
+                for (int l = 0; l < L; ++l) {
+                    const int s = PLAIN ? kNone : first[l];
+                    if (s >= 0) load_state<V>(p.active ? a.state_in : nullptr, s, a.channels, p.channel, h);
+                    const Pack<T, V> xl = load_pack<T, V>(ring[stage].v[kXAt][l][threadIdx.x]);
+                    float f[A], k[A];
+#pragma unroll
+                    for (int v = 0; v < A; ++v) decode_gate<LOGIT>(m[l][v], f[v], k[v]);
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        const float xv = to_float(xl.e[v]);
+                        u[l][v] = COUPLED ? h[v] - xv : h[v];
+                        const float n = fmaf(f[v % A], h[v], COUPLED ? xv * k[v % A] : xv);
+                        h[v] = s == kOutside ? h[v] : n;
+                    }
+                }
+            }
+            __syncthreads();
+            if (!APPLY) {
+#pragma unroll
+                for (int w = kWalkWarps - 1; w >= 0; --w) {
+                    Map<V, A> n = warp_map<PLAIN>(sh[stage], w, p.tx);
+                    const int closed = all.closed;
+                    compose_after<PLAIN>(n, all);
+                    if (PLAIN) n.closed = closed;
+                    all = n;
+                }
+                return;
+            }
+            float q[V];
+            pass_warps<false, PLAIN>(sh[stage], p.tx, q_carry, q);
+            apply_map<PLAIN>(q, after);
+#pragma unroll
+            for (int l = L - 1; l >= 0; --l) {
+                const int s = PLAIN ? kNone : first[l], e = PLAIN ? kNone : end[l];
+                const bool outside = s == kOutside;
+                if (e >= 0) load_state<V>(p.active ? a.v_state_out : nullptr, e, a.channels, p.channel, q);
+                Pack<T, V> d;
+                if (a.v_h) d = load_pack<T, V>(ring[stage].v[0][l][threadIdx.x]);
+                float f[A], k[A], slope[A], dx[V], dg[V], sum = 0.f;
+#pragma unroll
+                for (int v = 0; v < A; ++v) {
+                    decode_gate<LOGIT>(m[l][v], f[v], k[v]);
+                    slope[v] = LOGIT ? f[v] * k[v] : 1.f;
+                }
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const float g = (a.v_h && !outside ? to_float(d.e[v]) : 0.f) + q[v];
+                    dx[v] = outside ? 0.f : COUPLED ? k[v % A] * g : g;
+                    dg[v] = outside ? 0.f : SHARED ? g * u[l][v] : g * u[l][v] * slope[v % A];
+                    if (SHARED) sum += dg[v];
+                    q[v] = outside ? q[v] : f[v % A] * g;
+                }
+                if (px && p.active && (PLAIN || l < left)) store_floats<T, V>(px + l * a.h_stride, dx);
+                if (s >= 0 && p.active && a.v_state_in) store_floats<float, V>(a.v_state_in + (long long)s * a.channels + p.channel, q);
+                if (!SHARED) {
+                    if (pg && p.active && (PLAIN || l < left)) store_floats<T, V>(pg + l * a.gate_out_stride, dg);
+                } else if (a.v_gate) {
+                    sum = p.active ? sum * slope[0] : 0.f;
+                    for (int off = (1 << a.lg_tx) >> 1; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                    if (p.tx == 0 && (PLAIN || l < left)) store_gate_sum(l, sum);
+                }
+            }
+        };
+        if (kind == kPlain) tile(std::true_type{});
+        else tile(std::false_type{});
+    }
+    if (APPLY) pass_empty_sequences(a, a.v_state_out, a.v_state_in);
+    else store_segment_map(a, p, all);
+}
+
+// ---- launches: one source file per storage type and direction instantiates these ------------------------------------------
+template <typename T, int V, bool FORWARD, bool LOGIT, bool COUPLED, bool SHARED, bool APPLY>
+int launch_walk(const RecurrenceLaunch& c, cudaStream_t s) {
+    constexpr int L = walk_rows<T>(V);
+    constexpr int kTensors = FORWARD ? (SHARED ? 1 : 2) : 1 + (APPLY ? 1 : 0) + (SHARED ? 0 : 1);
+    auto kernel = FORWARD ? recurrence_forward_kernel<T, V, LOGIT, COUPLED, SHARED, APPLY>
+                          : recurrence_backward_kernel<T, V, LOGIT, COUPLED, SHARED, APPLY>;
+    const size_t smem = 2 * sizeof(TileStage<T, V, L, kTensors>) + kTables * 2 * sizeof(int) * c.tile_rows;
+    if (smem > 32 * 1024)   // beside the static part
+        DSB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    kernel<<<c.blocks, kWalkThreads, smem, s>>>(c.args);
+    DSB_LAUNCH_CHECK();
+    return DSB_OK;
+}
+template <typename T, int V, bool FORWARD, bool LOGIT, bool COUPLED, bool SHARED>
+int run_walk(const RecurrenceLaunch& c, cudaStream_t s) {
+    if (c.args.segments > 1) {
+        const int rc = launch_walk<T, V, FORWARD, LOGIT, COUPLED, SHARED, false>(c, s);
+        if (rc != DSB_OK) return rc;
+    }
+    return launch_walk<T, V, FORWARD, LOGIT, COUPLED, SHARED, true>(c, s);
+}
+template <typename T, int V, bool FORWARD, bool LOGIT, bool COUPLED>
+int run_walk(const RecurrenceLaunch& c, cudaStream_t s) {
+    return c.args.shared ? run_walk<T, V, FORWARD, LOGIT, COUPLED, true>(c, s) : run_walk<T, V, FORWARD, LOGIT, COUPLED, false>(c, s);
+}
+template <typename T, int V, bool FORWARD>
+int run_walk(const RecurrenceLaunch& c, cudaStream_t s) {
+    if (c.args.logit)
+        return c.args.coupled ? run_walk<T, V, FORWARD, true, true>(c, s) : run_walk<T, V, FORWARD, true, false>(c, s);
+    return c.args.coupled ? run_walk<T, V, FORWARD, false, true>(c, s) : run_walk<T, V, FORWARD, false, false>(c, s);
+}
+template <typename T, bool FORWARD>
+int run_walk(const RecurrenceLaunch& c, cudaStream_t s) {
+    return c.vec == 4 ? run_walk<T, 4, FORWARD>(c, s) : run_walk<T, 1, FORWARD>(c, s);
+}
+
+}  // namespace dsb

@@ -1,0 +1,9 @@
+// The backward walk of the gated recurrence for one storage type.
+#include "recurrence.cuh"
+
+namespace dsb {
+
+template <>
+int run_recurrence_backward<float>(const RecurrenceLaunch& c, cudaStream_t s) { return run_walk<float, false>(c, s); }
+
+}  // namespace dsb
