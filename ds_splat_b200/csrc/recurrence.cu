@@ -44,12 +44,17 @@ recurrence_step_kernel(const T* x, const T* gate, float* state, T* h, const long
     const Pack<T, V> px = load_pack<T, V>(x + s * x_stride + c);
     const Pack<float, V> ps = load_pack<float, V>(state + i);
     float o[V], f = 0.f, k = 0.f;
+    auto take = [&](T g) {
+        const float e = gate_register<T, LOGIT>(g);
+        f = gate_f<LOGIT>(e);
+        k = gate_k<LOGIT>(e, f);
+    };
     Pack<T, V> pg;
-    if (per_head > 1) gate_pair<LOGIT>(to_float(gate[s * gate_stride + c / per_head]), f, k);
+    if (per_head > 1) take(gate[s * gate_stride + c / per_head]);
     else pg = load_pack<T, V>(gate + s * gate_stride + c);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        if (per_head == 1) gate_pair<LOGIT>(to_float(pg.e[v]), f, k);
+        if (per_head == 1) take(pg.e[v]);
         const float xv = to_float(px.e[v]);
         o[v] = fmaf(f, ps.e[v], coupled ? k * xv : xv);
     }

@@ -62,49 +62,40 @@ constexpr int kWalkWarps = kWalkThreads / 32;
 template <typename T> __host__ __device__ constexpr int walk_rows(int vec) { return vec == 4 ? (sizeof(T) == 4 ? 4 : 8) : 16; }
 
 // ---- gates ---------------------------------------------------------------------------------------------------------
-// exp(-|g|) and 1 / (1 + exp(-|g|)): the smaller of f and 1 - f is their product, the other the second.  Both keep full
-// relative precision, however close to 0 or 1 the gate is.
-__device__ __forceinline__ void logistic_parts(float g, float& t, float& r) {
-    float y;
-    asm("max.NaN.f32 %0, %1, 0fC2B40000;" : "=f"(y) : "f"(-fabsf(g)));   // -90: 2^(y log2 e) is flushed to 0; NaN stays NaN
-    const float hi = y * 1.44269502f;                 // exp(y) = 2^(y log2 e), the product's rounding error added back
-    const float lo = fmaf(y, 1.44269502f, -hi);       // to first order
-    t = exp2f(hi);
-    t = fmaf(t, lo * 0.693147181f, t);
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + t));
-}
-template <bool LOGIT>
-__device__ __forceinline__ void gate_pair(float g, float& f, float& k) {
-    if (LOGIT) {
-        float t, r;
-        logistic_parts(g, t, r);
-        const float small = t * r;
-        f = g < 0.f ? small : r;
-        k = g < 0.f ? r : small;
-    } else {
-        f = g;
-        k = 1.f - g;
-    }
-}
-// One register that holds both: the smaller one with the sign saying which it is.
-template <bool LOGIT>
-__device__ __forceinline__ float encode_gate(float g) {
+// A gate is kept as one register: a decay as itself, a logit g as e = exp(-g), from which f = 1 / (1 + e) and 1 - f = e f
+// follow with full relative precision however close to 0 or 1 they are.  e is kept below 2^126, where 1 / (1 + e) is still a
+// normal number (1.2e-38); a NaN stays one.
+// Errors, with u = 2^-24 and L = log2 e: 2^x by the hardware 4 u, its argument's rounding |g| 1.2 u, the quotient 2 u, 1 + e and
+// the product u each.  32-bit gates get the argument's rounding error back to first order (three instructions more).
+template <typename T, bool LOGIT>
+__device__ __forceinline__ float gate_register(T gate) {
+    const float g = to_float(gate);
     if (!LOGIT) return g;
-    float t, r;
-    logistic_parts(g, t, r);
-    return copysignf(t * r, g);
+    constexpr float kLog2e = 1.44269502f, kLn2 = 0.693147181f;
+    float e;
+    if (sizeof(T) == 4) {
+        float y;
+        asm("{\n\t.reg .f32 t;\n\tmin.NaN.f32 t, %1, 0f42AE0000;\n\tmax.NaN.f32 %0, t, 0fC2AE0000;\n\t}" : "=f"(y) : "f"(-g));   // +-87
+        const float hi = y * kLog2e, lo = fmaf(y, kLog2e, -hi);
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(hi));
+        e = fmaf(e, lo * kLn2, e);
+    } else {
+        float t;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(g * -kLog2e));
+        asm("min.NaN.f32 %0, %1, 0f7E800000;" : "=f"(e) : "f"(t));
+    }
+    return e;
 }
 template <bool LOGIT>
-__device__ __forceinline__ void decode_gate(float m, float& f, float& k) {
-    if (LOGIT) {
-        const float rest = 1.f - fabsf(m);
-        const bool small_f = __float_as_int(m) < 0;
-        f = small_f ? fabsf(m) : rest;
-        k = small_f ? rest : fabsf(m);
-    } else {
-        f = m;
-        k = 1.f - m;
-    }
+__device__ __forceinline__ float gate_f(float e) {
+    if (!LOGIT) return e;
+    float f;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(f) : "f"(1.f + e));
+    return f;
+}
+template <bool LOGIT>
+__device__ __forceinline__ float gate_k(float e, float f) {   // 1 - f
+    return LOGIT ? e * f : 1.f - f;
 }
 
 // ---- rows that begin and end sequences ------------------------------------------------------------------------------
@@ -188,7 +179,7 @@ struct Borders {
             for (int r = tid; r < tile_rows; r += kWalkThreads) {
                 const long long p = p0 + r;
                 f[r] = p < lo || p >= hi ? kOutside : p == lo ? sequence : kNone;
-                e[r] = p == hi - 1 ? sequence : kNone;
+                e[r] = p == hi - 1 && lo < hi ? sequence : kNone;   // a sequence of no rows ends nowhere
             }
             return kBorders;
         }
@@ -602,7 +593,9 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
                 float k[A];
 #pragma unroll
                 for (int v = 0; v < A; ++v) {
-                    gate_pair<LOGIT>(to_float(pg.e[v]), f[l][v], k[v]);
+                    const float e = gate_register<T, LOGIT>(pg.e[v]);
+                    f[l][v] = gate_f<LOGIT>(e);
+                    k[v] = gate_k<LOGIT>(e, f[l][v]);
                     if (outside) f[l][v] = 1.f;
                     own.a[v] *= f[l][v];
                 }
@@ -632,6 +625,7 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
             if (a.checkpoints && p.active)
                 store_floats<float, V>(a.checkpoints + ((p.chain * a.tiles + t) * (kWalkWarps * (32 >> a.lg_tx)) + p.group) * a.channels + p.channel, h);
             T* to = ph;
+            const bool wanted = ph && p.active;
 #pragma unroll
             for (int l = 0; l < L; ++l) {
                 const int s = PLAIN ? kNone : first[l], e = PLAIN ? kNone : end[l];
@@ -642,7 +636,7 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
                     h[v] = fmaf(f[l][v % A], h[v], b[l][v]);
                     o[v] = s == kOutside ? 0.f : h[v];
                 }
-                if (ph && p.active && (PLAIN || l < left)) store_floats<T, V>(to, o);
+                store_floats_if<T, V>(to, o, wanted && (PLAIN || l < left));
                 to += a.h_stride;
                 if (e >= 0 && p.active) store_floats<float, V>(a.state_out + (long long)e * a.channels + p.channel, h);
             }
@@ -742,11 +736,11 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                     load_state<V>(p.active ? a.v_state_out : nullptr, e, a.channels, p.channel, own.b);
                     own.closed = 1;
                 }
-                float f[A], k;
+                float f[A];
 #pragma unroll
                 for (int v = 0; v < A; ++v) {
-                    m[l][v] = encode_gate<LOGIT>(to_float(g.e[v]));
-                    decode_gate<LOGIT>(m[l][v], f[v], k);
+                    m[l][v] = gate_register<T, LOGIT>(g.e[v]);
+                    f[v] = gate_f<LOGIT>(m[l][v]);
                     if (outside) f[v] = 1.f;
                     own.a[v] *= f[v];
                 }
@@ -766,7 +760,10 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                     const Pack<T, V> xl = load_pack<T, V>(ring[stage].v[kXAt][l][threadIdx.x]);
                     float f[A], k[A];
 #pragma unroll
-                    for (int v = 0; v < A; ++v) decode_gate<LOGIT>(m[l][v], f[v], k[v]);
+                    for (int v = 0; v < A; ++v) {
+                        f[v] = gate_f<LOGIT>(m[l][v]);
+                        k[v] = gate_k<LOGIT>(m[l][v], f[v]);
+                    }
 #pragma unroll
                     for (int v = 0; v < V; ++v) {
                         const float xv = to_float(xl.e[v]);
@@ -801,7 +798,8 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                 float f[A], k[A], slope[A], dx[V], dg[V], sum = 0.f;
 #pragma unroll
                 for (int v = 0; v < A; ++v) {
-                    decode_gate<LOGIT>(m[l][v], f[v], k[v]);
+                    f[v] = gate_f<LOGIT>(m[l][v]);
+                    k[v] = gate_k<LOGIT>(m[l][v], f[v]);
                     slope[v] = LOGIT ? f[v] * k[v] : 1.f;
                 }
 #pragma unroll
@@ -812,10 +810,10 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                     if (SHARED) sum += dg[v];
                     q[v] = outside ? q[v] : f[v % A] * g;
                 }
-                if (px && p.active && (PLAIN || l < left)) store_floats<T, V>(px + l * a.h_stride, dx);
+                store_floats_if<T, V>(px + l * a.h_stride, dx, px && p.active && (PLAIN || l < left));
                 if (s >= 0 && p.active && a.v_state_in) store_floats<float, V>(a.v_state_in + (long long)s * a.channels + p.channel, q);
                 if (!SHARED) {
-                    if (pg && p.active && (PLAIN || l < left)) store_floats<T, V>(pg + l * a.gate_out_stride, dg);
+                    store_floats_if<T, V>(pg + l * a.gate_out_stride, dg, pg && p.active && (PLAIN || l < left));
                 } else if (a.v_gate) {
                     sum = p.active ? sum * slope[0] : 0.f;
                     for (int off = (1 << a.lg_tx) >> 1; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);

@@ -45,6 +45,18 @@ __device__ __forceinline__ void store_floats(T* p, const float (&v)[V]) {
     *reinterpret_cast<Raw*>(p) = raw;
 }
 
+// The same under a condition, with only the store itself left out.
+template <typename T, int V>
+__device__ __forceinline__ void store_floats_if(T* p, const float (&v)[V], bool there) {
+    typedef typename RawVec<V * sizeof(T)>::type Raw;
+    Pack<T, V> out;
+#pragma unroll
+    for (int i = 0; i < V; ++i) from_float(v[i], out.e[i]);
+    Raw raw;
+    memcpy(&raw, &out, sizeof(raw));
+    if (there) *reinterpret_cast<Raw*>(p) = raw;
+}
+
 // Calls f with a value of the storage type that `dtype` (DSB_DTYPE_*) names; false for an unknown one.
 template <typename F>
 bool with_dtype(int dtype, F&& f) {
