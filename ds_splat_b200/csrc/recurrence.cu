@@ -21,7 +21,8 @@ template <> int run_recurrence_backward<__nv_bfloat16>(const RecurrenceLaunch&, 
 
 namespace {
 
-constexpr long long kMaxRows = (1ll << 31) - 1;
+constexpr long long kMaxRows = (1ll << 31) - (1 << 16);   // positions are 32-bit, the last tile's end included
+constexpr long long kMaxBlocks = (1ll << 31) - 1;
 
 // v_gate = sum of the channel blocks' shares of it, in their order
 template <typename T>
@@ -82,7 +83,7 @@ int check_shape(const DsbRecurrence& s, bool step) {
     DSB_REQUIRE(s.gate_form == DSB_GATE_DECAY || s.gate_form == DSB_GATE_LOGIT, "recurrence: unknown gate form %d", s.gate_form);
     DSB_REQUIRE(s.channels >= 1 && s.gate_heads >= 1 && s.channels % s.gate_heads == 0,
                 "recurrence: %d channels do not split into %d gate heads", s.channels, s.gate_heads);
-    DSB_REQUIRE(s.rows >= 0 && s.rows <= kMaxRows, "recurrence: at most 2^31 - 1 rows, got %lld", (long long)s.rows);
+    DSB_REQUIRE(s.rows >= 0 && s.rows <= kMaxRows, "recurrence: at most 2^31 - 2^16 rows, got %lld", (long long)s.rows);
     DSB_REQUIRE(s.sequences >= 0, "recurrence: negative number of sequences");
     if (step) {
         DSB_REQUIRE(s.rows == s.sequences, "recurrence: a step takes one row per sequence");
@@ -163,8 +164,8 @@ int make_cut(const DsbRecurrence& s, bool forward, void* workspace, int64_t work
     DSB_REQUIRE(aligned(workspace, 16) && aligned(checkpoints, 16), "recurrence: workspace and checkpoints must be 16-byte aligned");
     RecurrenceArgs& a = c.launch.args;
     a = RecurrenceArgs{};
-    a.rows = s.rows; a.chain_rows = l.chain_rows; a.chains = l.chains;
-    a.tiles = l.tiles; a.segments = l.segments; a.segment_tiles = l.segment_tiles;
+    a.rows = (int)s.rows; a.chain_rows = (int)l.chain_rows; a.chains = (int)l.chains;
+    a.tiles = (int)l.tiles; a.segments = (int)l.segments; a.segment_tiles = (int)l.segment_tiles;
     a.checkpoints = checkpoints;
     a.sequences = s.sequences; a.sequence_rows = s.sequence_rows; a.channels = s.channels; a.gate_heads = s.gate_heads;
     a.heads = l.heads; a.per_head = l.per_head; a.parts = l.parts; a.lg_tx = l.lg_tx;
@@ -183,7 +184,7 @@ int make_cut(const DsbRecurrence& s, bool forward, void* workspace, int64_t work
     }
     if (!forward && a.shared && l.parts > 1) a.gate_parts = reinterpret_cast<float*>(w);
     const int64_t blocks = l.chains * l.segments * l.heads * l.parts;
-    DSB_REQUIRE(blocks <= kMaxRows, "recurrence: too many blocks for one launch");
+    DSB_REQUIRE(blocks <= kMaxBlocks, "recurrence: too many blocks for one launch");
     c.launch.vec = l.vec; c.launch.tile_rows = l.tile_rows; c.launch.blocks = (unsigned)blocks;
     return device_status_address(&a.device_status);
 }
@@ -320,7 +321,7 @@ int launch_recurrence_step(const DsbRecurrence& shape, const void* x, const void
     DSB_TRY(check_alignment(shape, state, shape.channels, 4, wide, "the state"));
     const long long count = shape.rows * shape.channels;
     const long long blocks = (count / (wide ? 4 : 1) + kWalkThreads - 1) / kWalkThreads;
-    DSB_REQUIRE(blocks <= kMaxRows, "recurrence: too many elements for one launch");
+    DSB_REQUIRE(blocks <= kMaxBlocks, "recurrence: too many elements for one launch");
     const int per_head = shape.channels / shape.gate_heads;
     with_dtype(shape.dtype, [&](auto tag) {
         typedef decltype(tag) T;

@@ -38,10 +38,10 @@ struct RecurrenceArgs {
     float* gate_parts;     // [parts][rows][heads], when a head spans several channel blocks
     const int *offsets, *lengths;
     int* device_status;
-    long long rows, chain_rows, chains;
+    int rows, chain_rows, chains;
     long long x_stride, gate_stride, v_h_stride;   // negative when the scan runs from the last row to the first
     long long h_stride, gate_out_stride;           // channels / heads of contiguous results, with the same sign
-    long long tiles, segments, segment_tiles;
+    int tiles, segments, segment_tiles;
     int sequences, sequence_rows, channels, gate_heads, heads, per_head, parts, lg_tx;
     int reverse, table;    // table: one chain over all rows, with sequence borders anywhere; else one chain per sequence
     int logit, coupled, shared;
@@ -106,17 +106,18 @@ constexpr int kTables = 3;      // one is read, one was read by the slowest warp
 
 __device__ __forceinline__ int sequence_id(const RecurrenceArgs& a, int k) { return a.reverse ? a.sequences - 1 - k : k; }
 // Where the scan's packed sequence k begins (k = sequences: where the last one ends).
-__device__ __forceinline__ long long packed_start(const RecurrenceArgs& a, long long k) {
-    return a.reverse ? a.rows - a.offsets[a.sequences - k] : a.offsets[k];
+__device__ __forceinline__ int packed_start(const RecurrenceArgs& a, int k) {
+    const int o = a.reverse ? a.rows - min(max(a.offsets[a.sequences - k], 0), a.rows) : a.offsets[k];
+    return min(max(o, 0), a.rows);   // offsets out of range are reported (pass_empty_sequences); here they must not overflow
 }
 // How many of packed_start(shift .. shift + sequences - 1) are <= p; called by one whole warp.
-__device__ __forceinline__ int starts_up_to(const RecurrenceArgs& a, int shift, long long p) {
+__device__ __forceinline__ int starts_up_to(const RecurrenceArgs& a, int shift, int p) {
     const int lane = threadIdx.x & 31;
     int lo = 0, len = a.sequences;
     while (len > 0) {
         const int step = (len + 31) / 32;
-        const long long at = (long long)lane * step;
-        const bool below = at < len && packed_start(a, shift + lo + at) <= p;
+        const int at = min(lane, len) * step;     // 32 steps may pass 2^31
+        const bool below = at >= 0 && at < len && packed_start(a, shift + lo + at) <= p;
         const int below_count = __popc(__ballot_sync(0xffffffffu, below));
         if (below_count == 0) break;
         const int skip = (below_count - 1) * step + 1;
@@ -133,18 +134,18 @@ enum TileKind { kPlain, kBorders, kEmpty };   // no border and every row in a se
 // the same in all threads of the block.
 template <bool FORWARD>
 struct Borders {
-    long long lo, hi;      // the sequence last met holds positions [lo, hi)
+    int lo, hi;            // the sequence last met holds positions [lo, hi)
     int sequence;          // chain per sequence: its id.  Packed: where to look on, as a sequence of the scan
     int* tables;
     int tile_rows;
 
-    __device__ void begin(const RecurrenceArgs& a, int chain, long long p0, int* s_tables, int rows) {
+    __device__ void begin(const RecurrenceArgs& a, int chain, int p0, int* s_tables, int rows) {
         tables = s_tables;
         tile_rows = rows;
         lo = 1; hi = 0;
         if (!a.table) {
             sequence = sequence_id(a, chain);
-            long long len = a.sequence_rows;
+            int len = a.sequence_rows;
             if (a.lengths) len = min(max(a.lengths[sequence], 0), a.sequence_rows);
             lo = a.reverse ? a.sequence_rows - len : 0;
             hi = lo + len;
@@ -165,19 +166,19 @@ struct Borders {
         lo = any ? packed_start(a, sequence) : 1;
         hi = any ? packed_start(a, sequence + 1) : 0;
     }
-    __device__ int* first(long long t) const { return tables + (int)(t % kTables) * 2 * tile_rows; }
-    __device__ int* end(long long t) const { return first(t) + tile_rows; }
+    __device__ int* first(int t) const { return tables + t % kTables * 2 * tile_rows; }
+    __device__ int* end(int t) const { return first(t) + tile_rows; }
 
     // Tile t at p0; called by the whole block, tile after tile.  Tables are there after the next barrier.
-    __device__ int prepare(const RecurrenceArgs& a, long long t, long long p0) {
-        const long long p1 = p0 + tile_rows;
+    __device__ int prepare(const RecurrenceArgs& a, int t, int p0) {
+        const int p1 = p0 + tile_rows;
         if (p0 > lo && p1 < hi) return kPlain;
         if (!a.table && (p1 <= lo || p0 >= hi)) return kEmpty;
         int *f = first(t), *e = end(t);
         const int tid = threadIdx.x;
         if (!a.table) {
             for (int r = tid; r < tile_rows; r += kWalkThreads) {
-                const long long p = p0 + r;
+                const int p = p0 + r;
                 f[r] = p < lo || p >= hi ? kOutside : p == lo ? sequence : kNone;
                 e[r] = p == hi - 1 && lo < hi ? sequence : kNone;   // a sequence of no rows ends nowhere
             }
@@ -185,10 +186,10 @@ struct Borders {
         }
         if (a.sequence_rows > 0) {
             for (int r = tid; r < tile_rows; r += kWalkThreads) {
-                const long long p = p0 + r;
+                const int p = p0 + r;
                 int b = kOutside, c = kNone;
                 if (p < a.rows) {
-                    const int turn = (int)(p / a.sequence_rows), pos = (int)(p - (long long)turn * a.sequence_rows);
+                    const int turn = p / a.sequence_rows, pos = p - turn * a.sequence_rows;
                     const int seq = sequence_id(a, turn);
                     const int len = a.lengths ? min(max(a.lengths[seq], 0), a.sequence_rows) : a.sequence_rows;
                     const int at = a.reverse ? a.sequence_rows - len : 0;
@@ -202,22 +203,22 @@ struct Borders {
             }
             return kBorders;
         }
-        const long long last = min(p1, a.rows);
-        const long long all0 = packed_start(a, 0), all1 = packed_start(a, a.sequences);
+        const int last = min(p1, a.rows);
+        const int all0 = packed_start(a, 0), all1 = packed_start(a, a.sequences);
         for (int r = tid; r < tile_rows; r += kWalkThreads) {
-            const long long p = p0 + r;
+            const int p = p0 + r;
             f[r] = p < last && p >= all0 && p < all1 ? kNone : kOutside;
             e[r] = kNone;
         }
         __syncthreads();
         int done;
         do {   // offsets out of order may lead this astray, but every access stays where it belongs
-            const long long k = FORWARD ? (long long)sequence + tid : (long long)sequence - tid;
+            const int k = FORWARD ? sequence + tid : sequence - tid;
             bool through = false;
             if (k >= 0 && k < a.sequences) {
-                const long long o0 = packed_start(a, k), o1 = packed_start(a, k + 1);
+                const int o0 = packed_start(a, k), o1 = packed_start(a, k + 1);
                 if (o0 < o1) {
-                    const int id = sequence_id(a, (int)k);
+                    const int id = sequence_id(a, k);
                     if (o0 >= p0 && o0 < last) f[o0 - p0] = id;
                     if (o1 > p0 && o1 <= last) e[o1 - 1 - p0] = id;
                 }
@@ -363,19 +364,19 @@ __device__ __forceinline__ void pass_warps(const WarpMaps<V, A>& sh, int tx, flo
 
 // ---- a block's place -----------------------------------------------------------------------------------------------------
 struct Place {
-    int chain, head, part, channel, tx;
-    long long segment;
+    int chain, segment, head, part, channel, tx;
     int row0, group;       // this thread's first row inside a tile, and which of the tile's groups of rows that is
-    bool active;
+    bool active;           // false beyond the head's last channel
+    int read_channel;      // what to read all the same where a thread has no channel
 };
 template <int V, int L>
 __device__ __forceinline__ Place place_of(const RecurrenceArgs& a) {
     Place p;
     const int blocks = a.heads * a.parts;
-    const long long rest = blockIdx.x / blocks;
-    const int block = (int)(blockIdx.x - rest * blocks);
-    p.chain = (int)(rest % a.chains);
+    const int rest = (int)(blockIdx.x / (unsigned)blocks);
+    const int block = (int)(blockIdx.x - (unsigned)rest * blocks);
     p.segment = rest / a.chains;
+    p.chain = rest - p.segment * a.chains;
     p.head = block / a.parts;
     p.part = block - p.head * a.parts;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -385,6 +386,7 @@ __device__ __forceinline__ Place place_of(const RecurrenceArgs& a) {
     const int c = (p.part << a.lg_tx) * V + p.tx * V;
     p.active = c < a.per_head;
     p.channel = p.head * a.per_head + c;
+    p.read_channel = p.active ? p.channel : p.head * a.per_head;
     return p;
 }
 
@@ -402,19 +404,17 @@ __device__ __forceinline__ void load_state(const float* states, long long index,
 
 // ---- rows on their way through shared memory ---------------------------------------------------------------------------
 template <typename T, int V>
-__device__ __forceinline__ void copy_async(T* to, const T* from, bool there) {
+__device__ __forceinline__ void copy_async(unsigned to, const T* from, bool there) {
     constexpr int kBytes = V * sizeof(T);
     if (kBytes == 2) {                            // below what an asynchronous copy takes
-        T v;
-        memset(&v, 0, kBytes);
-        if (there) v = *from;
-        *to = v;
+        unsigned short v = 0;
+        if (there) v = *reinterpret_cast<const unsigned short*>(from);
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(v) : "memory");
     } else {
-        const unsigned at = (unsigned)__cvta_generic_to_shared(to);
         const int bytes = there ? kBytes : 0;     // what is not copied is filled with zeros
-        if (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(bytes) : "memory");
-        else if (kBytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(at), "l"(from), "r"(bytes) : "memory");
-        else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(at), "l"(from), "r"(bytes) : "memory");
+        if (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+        else if (kBytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
     }
 }
 __device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -427,57 +427,58 @@ struct alignas(16) TileStage {
     T v[TENSORS][L][kWalkThreads][V];
 };
 
-// This thread's rows of a tile; rows past the chain's end become zeros.  Rows that belong to no sequence but lie within the
-// tensor are copied like the others and masked where they are used.
+// A thread's view of one tensor: its first row of the tile that is fetched next.  The walk moves it from tile to tile.
+template <typename T>
+struct RowPointer {
+    const T* at;
+    long long stride, step;    // to the next row, to the same row of the next tile of the walk
+    __device__ __forceinline__ RowPointer(const T* base, int channel, long long row_stride, const RecurrenceArgs& a, const Place& p,
+                                          int tile, int tile_rows, bool forward) {
+        stride = row_stride;
+        step = forward ? tile_rows * row_stride : -(tile_rows * row_stride);
+        at = base + ((long long)p.chain * a.chain_rows + (long long)tile * tile_rows + p.row0) * row_stride + channel;
+    }
+};
+// The thread's rows of a tile, `left` of them within the chain (L: all, known to the whole block); the others become zeros.
+// Rows that belong to no sequence but lie within the tensor are copied like the others and masked where they are used.
 template <typename T, int V, int L>
-__device__ __forceinline__ void fetch_rows(T (*to)[kWalkThreads][V], const T* base, long long stride, const RecurrenceArgs& a,
-                                           const Place& p, long long p0) {
-    const long long at = p0 + p.row0;
-    const T* from = base + (p.chain * a.chain_rows + at) * stride;
-    const int left = p.active ? (int)min(a.chain_rows - at, (long long)L) : 0;
-    if (left == L) {
+__device__ __forceinline__ void fetch_rows(unsigned to, const RowPointer<T>& r, bool full, int left) {
+    constexpr unsigned kRow = kWalkThreads * V * sizeof(T);
+    const T* from = r.at;
+    if (full) {
 #pragma unroll
-        for (int l = 0; l < L; ++l, from += stride) copy_async<T, V>(to[l][threadIdx.x], from, true);
+        for (int l = 0; l < L; ++l, from += r.stride) copy_async<T, V>(to + l * kRow, from, true);
     } else {
-#pragma unroll
-        for (int l = 0; l < L; ++l) copy_async<T, V>(to[l][threadIdx.x], l < left ? from + l * stride : base, l < left);
+#pragma unroll 1
+        for (int l = 0; l < L; ++l) copy_async<T, V>(to + l * kRow, l < left ? from + l * r.stride : static_cast<const T*>(from), l < left);
     }
 }
-// Gates of their own come like x; a shared one is read directly, as every thread of a row wants the same value.
-template <bool SHARED, typename T, int V, int L>
-__device__ __forceinline__ void fetch_gates(T (*to)[kWalkThreads][V], T (&own)[L], const RecurrenceArgs& a, const Place& p,
-                                            long long p0) {
-    const T* base = static_cast<const T*>(a.gate) + (SHARED ? p.head : p.channel);
-    if (!SHARED) {
-        fetch_rows<T, V, L>(to, base, a.gate_stride, a, p, p0);
-        return;
-    }
-    const long long at = p0 + p.row0;
-    const T* from = base + (p.chain * a.chain_rows + at) * a.gate_stride;
-    const int left = p.active ? (int)min(a.chain_rows - at, (long long)L) : 0;
+// A gate that channels share is read directly, as every thread of a row wants the same value.
+template <typename T, int L>
+__device__ __forceinline__ void fetch_shared_gates(T (&own)[L], const RowPointer<T>& r, int left) {
 #pragma unroll
     for (int l = 0; l < L; ++l) {
         memset(&own[l], 0, sizeof(T));
-        if (l < left) own[l] = from[l * a.gate_stride];
+        if (l < left) own[l] = r.at[l * r.stride];
     }
 }
 
 // The state (or q) at the segment's beginning: the maps of the segments before it, each warp a share of them, in order.
 template <bool FORWARD, int V, int A>
 __device__ void carry_of_segment(const RecurrenceArgs& a, const Place& p, WarpMaps<V, A>& sh, float (&carry)[V]) {
-    const long long before = FORWARD ? p.segment : a.segments - 1 - p.segment;
+    const int before = FORWARD ? p.segment : a.segments - 1 - p.segment;
 #pragma unroll
     for (int v = 0; v < V; ++v) carry[v] = 0.f;
     if (before == 0) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long share = (before + kWalkWarps - 1) / kWalkWarps;
-    const long long i0 = min(share * warp, before), i1 = min(i0 + share, before);
+    const int share = (before + kWalkWarps - 1) / kWalkWarps;
+    const int i0 = min(share * warp, before), i1 = min(i0 + share, before);
     if (lane < (1 << a.lg_tx)) {
         Map<V, A> all;
         identity(all);
 #pragma unroll 4
-        for (long long i = i0; i < i1; ++i) {
-            const long long at = p.chain * a.segments + (FORWARD ? i : a.segments - 1 - i);
+        for (int i = i0; i < i1; ++i) {
+            const long long at = (long long)p.chain * a.segments + (FORWARD ? i : a.segments - 1 - i);
             Map<V, A> m;
             identity(m);
             m.closed = a.map_closed[at];
@@ -506,7 +507,7 @@ __device__ void carry_of_segment(const RecurrenceArgs& a, const Place& p, WarpMa
 template <int V, int A>
 __device__ __forceinline__ void store_segment_map(const RecurrenceArgs& a, const Place& p, const Map<V, A>& all) {
     if (threadIdx.x >= (1 << a.lg_tx) || !p.active) return;
-    const long long at = p.chain * a.segments + p.segment;
+    const long long at = (long long)p.chain * a.segments + p.segment;
     float wide[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) wide[v] = all.a[v % A];
@@ -517,11 +518,11 @@ __device__ __forceinline__ void store_segment_map(const RecurrenceArgs& a, const
 
 // A tile of rows that belong to no sequence.
 template <typename T, int V, int L>
-__device__ __forceinline__ void store_zero_rows(T* to, long long stride, int left, bool active) {
+__device__ __forceinline__ void store_zero_rows(T* to, long long stride, int left) {
     const float zero[V] = {};
-#pragma unroll
+#pragma unroll 1
     for (int l = 0; l < L; ++l)
-        if (active && l < left) store_floats<T, V>(to + l * stride, zero);
+        if (l < left) store_floats<T, V>(to + l * stride, zero);
 }
 
 template <typename T, int V, bool LOGIT, bool COUPLED, bool SHARED, bool APPLY>
@@ -534,8 +535,16 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
     __shared__ WarpMaps<V, A> sh[2];
     const int tile_rows = kWalkWarps * (32 >> a.lg_tx) * L;
     const Place p = place_of<V, L>(a);
-    const long long t0 = p.segment * a.segment_tiles, t1 = min(t0 + a.segment_tiles, a.tiles);
-    const T* x = static_cast<const T*>(a.x) + p.channel;
+    const int t0 = p.segment * a.segment_tiles, t1 = min(t0 + a.segment_tiles, a.tiles);
+    RowPointer<T> x(static_cast<const T*>(a.x), p.read_channel, a.x_stride, a, p, t0, tile_rows, true);
+    RowPointer<T> gate(static_cast<const T*>(a.gate), SHARED ? p.head : p.read_channel, a.gate_stride, a, p, t0, tile_rows, true);
+    const unsigned s_ring = (unsigned)__cvta_generic_to_shared(s_raw) + threadIdx.x * V * sizeof(T);
+    constexpr unsigned kTensor = L * kWalkThreads * V * sizeof(T);
+    const int groups = kWalkWarps * (32 >> a.lg_tx);
+    const bool wanted = APPLY && a.h && p.active;
+    T* to_h = static_cast<T*>(a.h) + ((long long)p.chain * a.chain_rows + (long long)t0 * tile_rows + p.row0) * a.h_stride + p.channel;
+    const bool keep = APPLY && a.checkpoints && p.active;
+    float* to_start = a.checkpoints + (((long long)p.chain * a.tiles + t0) * groups + p.group) * a.channels + p.channel;
 
     float carry[V];
     Map<V, A> all;
@@ -544,31 +553,39 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
     Borders<true> borders;
     borders.begin(a, p.chain, t0 * tile_rows, reinterpret_cast<int*>(s_raw + 2 * sizeof(Ring)), tile_rows);
     T gate_now[L], gate_next[L];
-    auto fetch = [&](int stage, long long t) {
-        fetch_rows<T, V, L>(ring[stage].v[0], x, a.x_stride, a, p, t * tile_rows);
-        fetch_gates<SHARED, T, V, L>(ring[stage].v[SHARED ? 0 : 1], gate_next, a, p, t * tile_rows);
+    // Fetches tile t, the next of the walk, and moves on; tiles without rows of a sequence are only passed.
+    auto fetch = [&](int stage, int t, int kind) {
+        if (kind != kEmpty) {
+            const int rest = a.chain_rows - t * tile_rows;
+            const int left = min(rest - p.row0, L);
+            fetch_rows<T, V, L>(s_ring + stage * sizeof(Ring), x, rest >= tile_rows, left);
+            if (SHARED) fetch_shared_gates<T, L>(gate_next, gate, left);
+            else fetch_rows<T, V, L>(s_ring + stage * sizeof(Ring) + kTensor, gate, rest >= tile_rows, left);
+        }
+        x.at += x.step;
+        gate.at += gate.step;
+        copies_issued();
     };
     int kind = borders.prepare(a, t0, t0 * tile_rows), kind_next = kEmpty;
-    if (kind != kEmpty) fetch(0, t0);
-    copies_issued();
+    fetch(0, t0, kind);
     __syncthreads();
-    for (long long t = t0; t < t1; ++t, kind = kind_next) {
-        const int stage = (int)(t - t0) & 1;
-        const long long p0 = t * tile_rows;
+    for (int t = t0; t < t1; ++t, kind = kind_next, to_h += tile_rows * a.h_stride, to_start += (long long)groups * a.channels) {
+        const int stage = (t - t0) & 1;
+        const int p0 = t * tile_rows;
         if (SHARED) {
 #pragma unroll
             for (int l = 0; l < L; ++l) gate_now[l] = gate_next[l];
         }
         if (t + 1 < t1) {
             kind_next = borders.prepare(a, t + 1, p0 + tile_rows);
-            if (kind_next != kEmpty) fetch(stage ^ 1, t + 1);
+            fetch(stage ^ 1, t + 1, kind_next);
+            copies_landed<1>();
+        } else {
+            copies_landed<0>();
         }
-        copies_issued();
-        copies_landed<1>();
-        const int left = (int)min(a.chain_rows - p0 - p.row0, (long long)L);
-        T* ph = APPLY && a.h ? static_cast<T*>(a.h) + (p.chain * a.chain_rows + p0 + p.row0) * a.h_stride + p.channel : nullptr;
+        const int left = min(a.chain_rows - p0 - p.row0, L);
         if (kind == kEmpty) {
-            if (ph) store_zero_rows<T, V, L>(ph, a.h_stride, left, p.active);
+            if (wanted) store_zero_rows<T, V, L>(to_h, a.h_stride, left);
             __syncthreads();
             continue;
         }
@@ -622,10 +639,8 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
             float h[V];
             pass_warps<true, PLAIN>(sh[stage], p.tx, carry, h);
             apply_map<PLAIN>(h, before);
-            if (a.checkpoints && p.active)
-                store_floats<float, V>(a.checkpoints + ((p.chain * a.tiles + t) * (kWalkWarps * (32 >> a.lg_tx)) + p.group) * a.channels + p.channel, h);
-            T* to = ph;
-            const bool wanted = ph && p.active;
+            store_floats_if<float, V>(to_start, h, keep);
+            T* to = to_h;
 #pragma unroll
             for (int l = 0; l < L; ++l) {
                 const int s = PLAIN ? kNone : first[l], e = PLAIN ? kNone : end[l];
@@ -660,9 +675,19 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
     __shared__ WarpMaps<V, A> sh[2];
     const int tile_rows = kWalkWarps * (32 >> a.lg_tx) * L;
     const Place p = place_of<V, L>(a);
-    const long long t0 = p.segment * a.segment_tiles, t1 = min(t0 + a.segment_tiles, a.tiles);
-    const T* x = static_cast<const T*>(a.x) + p.channel;
-    const T* vh = static_cast<const T*>(a.v_h) + p.channel;
+    const int t0 = p.segment * a.segment_tiles, t1 = min(t0 + a.segment_tiles, a.tiles);
+    RowPointer<T> vh(static_cast<const T*>(a.v_h), p.read_channel, a.v_h_stride, a, p, t1 - 1, tile_rows, false);
+    RowPointer<T> x(static_cast<const T*>(a.x), p.read_channel, a.x_stride, a, p, t1 - 1, tile_rows, false);
+    RowPointer<T> gate(static_cast<const T*>(a.gate), SHARED ? p.head : p.read_channel, a.gate_stride, a, p, t1 - 1, tile_rows, false);
+    const unsigned s_ring = (unsigned)__cvta_generic_to_shared(s_raw) + threadIdx.x * V * sizeof(T);
+    constexpr unsigned kTensor = L * kWalkThreads * V * sizeof(T);
+    const int groups = kWalkWarps * (32 >> a.lg_tx);
+    const long long row_first = (long long)p.chain * a.chain_rows + (long long)(t1 - 1) * tile_rows + p.row0;
+    const bool want_x = APPLY && a.v_x && p.active, want_gate = APPLY && a.v_gate && !SHARED && p.active;
+    T* to_x = static_cast<T*>(a.v_x) + row_first * a.h_stride + p.channel;
+    T* to_gate = static_cast<T*>(a.v_gate) + row_first * a.gate_out_stride + (SHARED ? p.head : p.channel);
+    float* to_part = a.gate_parts + ((a.reverse ? a.rows - 1 - row_first : row_first) + (long long)p.part * a.rows) * a.gate_heads + p.head;
+    const float* from_start = a.checkpoints + (((long long)p.chain * a.tiles + t1 - 1) * groups + p.group) * a.channels + p.read_channel;
 
     float q_carry[V], start[V], start_next[V];
     Map<V, A> all;
@@ -671,22 +696,34 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
     Borders<false> borders;
     borders.begin(a, p.chain, (t1 - 1) * tile_rows, reinterpret_cast<int*>(s_raw + 2 * sizeof(Ring)), tile_rows);
     T gate_now[L], gate_next[L];
-    auto fetch = [&](int stage, long long t) {
-        if (a.v_h) fetch_rows<T, V, L>(ring[stage].v[0], vh, a.v_h_stride, a, p, t * tile_rows);
-        fetch_gates<SHARED, T, V, L>(ring[stage].v[kGateAt], gate_next, a, p, t * tile_rows);
-        if (APPLY) {
-            fetch_rows<T, V, L>(ring[stage].v[kXAt], x, a.x_stride, a, p, t * tile_rows);
-            load_state<V>(p.active ? a.checkpoints : nullptr, (p.chain * a.tiles + t) * (kWalkWarps * (32 >> a.lg_tx)) + p.group,
-                          a.channels, p.channel, start_next);
+    auto fetch = [&](int stage, int t, int kind) {
+        if (kind != kEmpty) {
+            const int rest = a.chain_rows - t * tile_rows;
+            const int left = min(rest - p.row0, L);
+            const unsigned to = s_ring + stage * sizeof(Ring);
+            if (a.v_h) fetch_rows<T, V, L>(to, vh, rest >= tile_rows, left);
+            if (SHARED) fetch_shared_gates<T, L>(gate_next, gate, left);
+            else fetch_rows<T, V, L>(to + kGateAt * kTensor, gate, rest >= tile_rows, left);
+            if (APPLY) {
+                fetch_rows<T, V, L>(to + kXAt * kTensor, x, rest >= tile_rows, left);
+                const Pack<float, V> pack = load_pack<float, V>(from_start);
+#pragma unroll
+                for (int v = 0; v < V; ++v) start_next[v] = pack.e[v];
+            }
         }
+        vh.at += vh.step;
+        x.at += x.step;
+        gate.at += gate.step;
+        from_start -= (long long)groups * a.channels;
+        copies_issued();
     };
     int kind = borders.prepare(a, t1 - 1, (t1 - 1) * tile_rows), kind_next = kEmpty;
-    if (kind != kEmpty) fetch(0, t1 - 1);
-    copies_issued();
+    fetch(0, t1 - 1, kind);
     __syncthreads();
-    for (long long t = t1 - 1; t >= t0; --t, kind = kind_next) {
-        const int stage = (int)(t1 - 1 - t) & 1;
-        const long long p0 = t * tile_rows;
+    for (int t = t1 - 1; t >= t0; --t, kind = kind_next, to_x -= tile_rows * a.h_stride, to_gate -= tile_rows * a.gate_out_stride,
+             to_part -= tile_rows * a.gate_out_stride) {
+        const int stage = (t1 - 1 - t) & 1;
+        const int p0 = t * tile_rows;
         if (SHARED) {
 #pragma unroll
             for (int l = 0; l < L; ++l) gate_now[l] = gate_next[l];
@@ -695,23 +732,20 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
         for (int v = 0; v < V; ++v) start[v] = start_next[v];
         if (t > t0) {
             kind_next = borders.prepare(a, t - 1, p0 - tile_rows);
-            if (kind_next != kEmpty) fetch(stage ^ 1, t - 1);
+            fetch(stage ^ 1, t - 1, kind_next);
+            copies_landed<1>();
+        } else {
+            copies_landed<0>();
         }
-        copies_issued();
-        copies_landed<1>();
-        const long long row = p.chain * a.chain_rows + p0 + p.row0;
-        const int left = (int)min(a.chain_rows - p0 - p.row0, (long long)L);
-        T* px = APPLY && a.v_x ? static_cast<T*>(a.v_x) + row * a.h_stride + p.channel : nullptr;
-        T* pg = APPLY && a.v_gate && !SHARED ? static_cast<T*>(a.v_gate) + row * a.gate_out_stride + p.channel : nullptr;
+        const int left = min(a.chain_rows - p0 - p.row0, L);
         // a shared gate's sum over this block's channels
         auto store_gate_sum = [&](int l, float sum) {
-            const long long o = (row + l) * a.gate_out_stride + p.head;
-            if (a.parts == 1) from_float(sum, static_cast<T*>(a.v_gate)[o]);
-            else a.gate_parts[(a.reverse ? (a.rows - 1) * a.gate_heads + o : o) + (long long)p.part * a.rows * a.gate_heads] = sum;
+            if (a.parts == 1) from_float(sum, to_gate[l * a.gate_out_stride]);
+            else to_part[l * a.gate_out_stride] = sum;
         };
         if (kind == kEmpty) {
-            if (px) store_zero_rows<T, V, L>(px, a.h_stride, left, p.active);
-            if (pg) store_zero_rows<T, V, L>(pg, a.gate_out_stride, left, p.active);
+            if (want_x) store_zero_rows<T, V, L>(to_x, a.h_stride, left);
+            if (want_gate) store_zero_rows<T, V, L>(to_gate, a.gate_out_stride, left);
             if (APPLY && SHARED && a.v_gate && p.tx == 0)
                 for (int l = 0; l < left; ++l) store_gate_sum(l, 0.f);
             __syncthreads();
@@ -810,10 +844,10 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                     if (SHARED) sum += dg[v];
                     q[v] = outside ? q[v] : f[v % A] * g;
                 }
-                store_floats_if<T, V>(px + l * a.h_stride, dx, px && p.active && (PLAIN || l < left));
+                store_floats_if<T, V>(to_x + l * a.h_stride, dx, want_x && (PLAIN || l < left));
                 if (s >= 0 && p.active && a.v_state_in) store_floats<float, V>(a.v_state_in + (long long)s * a.channels + p.channel, q);
                 if (!SHARED) {
-                    store_floats_if<T, V>(pg + l * a.gate_out_stride, dg, pg && p.active && (PLAIN || l < left));
+                    store_floats_if<T, V>(to_gate + l * a.gate_out_stride, dg, want_gate && (PLAIN || l < left));
                 } else if (a.v_gate) {
                     sum = p.active ? sum * slope[0] : 0.f;
                     for (int off = (1 << a.lg_tx) >> 1; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);

@@ -164,7 +164,7 @@ def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, state: Optional[torch.
 
     x        [B, T, D]: B sequences of T rows; with ``lengths`` (int32 [B]) only the first ``lengths[b]`` of them belong to
              sequence b.  [N, D] with ``offsets`` (int32 [S + 1], nondecreasing, within [0, N]): sequence s is rows
-             ``offsets[s] .. offsets[s + 1]`` (a tile's ``ranges`` of the rasterizer are such offsets).  At most 2^31 - 1 rows.
+             ``offsets[s] .. offsets[s + 1]`` (a tile's ``ranges`` of the rasterizer are such offsets).  At most 2^31 - 2^16 rows.
     gate     x's shape with H for D: each of the H gates of a row is shared by D / H consecutive channels.  As logits
              (``form="logit"``) decays near 1 keep their precision in 16-bit types; as ``"decay"`` they are taken as they
              are and are meant to lie in [-1, 1].
