@@ -8,6 +8,8 @@
 //
 // recurrence.cuh holds the kernels that walk along sequences, recurrence_<direction>_<type>.cu instantiate them; here are the
 // single-row kernel, the argument checks and the rules by which a call is cut into blocks.
+#include <cmath>
+
 #include "recurrence.cuh"
 
 namespace dsb {
@@ -46,9 +48,14 @@ recurrence_step_kernel(const T* x, const T* gate, float* state, T* h, const long
     const Pack<float, V> ps = load_pack<float, V>(state + i);
     float o[V], f = 0.f, k = 0.f;
     auto take = [&](T g) {
-        const float e = gate_register<T, LOGIT>(g);
-        f = gate_f<LOGIT>(e);
-        k = gate_k<LOGIT>(e, f);
+        Pack<T, 1> one;
+        one.e[0] = g;
+        float e1[1], f1[1], k1[1];
+        gate_registers<T, LOGIT>(one, e1);
+        gate_f<LOGIT>(e1, f1);
+        gate_k<LOGIT>(e1, f1, k1);
+        f = f1[0];
+        k = k1[0];
     };
     Pack<T, V> pg;
     if (per_head > 1) take(gate[s * gate_stride + c / per_head]);
@@ -76,7 +83,7 @@ struct Layout {            // how a call is cut; the same for the forward and th
     int64_t chains, chain_rows, tiles;     // tiles of a chain
     int64_t segments, segment_tiles;       // of a chain
 };
-constexpr int kSms = 148, kBlocksPerSm = 4;
+constexpr int kSms = 148, kBlocksPerSm = 3;   // blocks: what the registers allow
 
 int check_shape(const DsbRecurrence& s, bool step) {
     DSB_REQUIRE(s.dtype == DSB_DTYPE_F32 || s.dtype == DSB_DTYPE_F16 || s.dtype == DSB_DTYPE_BF16, "recurrence: unknown dtype %d", s.dtype);
@@ -116,22 +123,36 @@ Layout layout_of(const DsbRecurrence& s) {
     const int rows = s.dtype == DSB_DTYPE_F32 ? walk_rows<float>(l.vec) : walk_rows<__half>(l.vec);
     l.lg_tx = 0;
     while (l.lg_tx < 5 && (1 << l.lg_tx) < wide) ++l.lg_tx;
-    for (;;) {
-        l.parts = (wide + (1 << l.lg_tx) - 1) >> l.lg_tx;
-        l.tile_rows = kWalkWarps * (32 >> l.lg_tx) * rows;
+    // How many threads share a row: as many as its channels fill, or fewer (down to a 64-byte piece of a row) where that
+    // spreads the blocks better over the SMs.  An SM holds kBlocksPerSm of them and is kept busy by two.
+    Layout pick = l;
+    int64_t blocks = 0;
+    double best = 0;
+    for (int lg = l.lg_tx, least = lg < 3 ? lg : 3; lg >= least; --lg) {
+        Layout c = l;
+        c.lg_tx = lg;
+        c.parts = (wide + (1 << lg) - 1) >> lg;
+        c.tile_rows = kWalkWarps * (32 >> lg) * rows;
         // A chain per sequence wastes half a tile per sequence on average; a table costs a look at every row.
-        l.table = s.sequence_rows == 0 || s.sequence_rows < l.tile_rows;
-        l.chains = l.table ? 1 : s.sequences;
-        // Narrower channel blocks where wide ones are too few to fill the GPU, down to a 64-byte piece of a row.
-        if (l.lg_tx <= 3 || l.chains * l.heads * l.parts >= kSms * kBlocksPerSm) break;
-        --l.lg_tx;
+        c.table = s.sequence_rows == 0 || s.sequence_rows < c.tile_rows;
+        c.chains = c.table ? 1 : s.sequences;
+        const int64_t these = c.chains * c.heads * c.parts;
+        const double per_sm = (double)these / kSms;
+        const double rounds = per_sm <= 2 ? 2 : per_sm <= kBlocksPerSm ? std::ceil(per_sm) : std::ceil(per_sm / kBlocksPerSm) * kBlocksPerSm;
+        const double even = per_sm / rounds;     // the share of the time that the average SM works
+        if (lg == l.lg_tx || even > best * 1.05) {
+            best = even;
+            blocks = these;
+            pick = c;
+        }
     }
+    l = pick;
     l.chain_rows = l.table ? s.rows : s.sequence_rows;
     l.tiles = (l.chain_rows + l.tile_rows - 1) / l.tile_rows;
-    const int64_t blocks = l.chains * l.heads * l.parts;
     l.segments = 1;
-    if (blocks < kSms * kBlocksPerSm / 2 && l.tiles > 1) {
+    if (best < 0.6 && l.tiles > 1) {   // cut the sequences: the inputs are then read twice
         l.segments = kSms * kBlocksPerSm / blocks;
+        if (l.segments < 1) l.segments = 1;
         if (l.segments > l.tiles) l.segments = l.tiles;
     }
     l.segment_tiles = l.tiles ? (l.tiles + l.segments - 1) / l.segments : 0;
@@ -172,9 +193,11 @@ int make_cut(const DsbRecurrence& s, bool forward, void* workspace, int64_t work
     a.logit = s.gate_form == DSB_GATE_LOGIT; a.coupled = s.coupled != 0; a.reverse = s.reverse != 0;
     a.shared = s.gate_heads != s.channels; a.table = l.table;
     a.offsets = s.offsets; a.lengths = s.lengths;
-    const int64_t sign = a.reverse ? -1 : 1;
+    const int64_t sign = (a.reverse ? -1 : 1) * dtype_bytes(s.dtype);
     a.x_stride = sign * s.x_stride; a.gate_stride = sign * s.gate_stride;
     a.h_stride = sign * s.channels; a.gate_out_stride = sign * s.gate_heads;
+    a.x_step = l.tile_rows * a.x_stride; a.gate_step = l.tile_rows * a.gate_stride;
+    a.h_step = l.tile_rows * a.h_stride; a.gate_out_step = l.tile_rows * a.gate_out_stride;
     unsigned char* w = static_cast<unsigned char*>(workspace);
     if (l.segments > 1) {
         const int64_t maps = l.chains * l.segments, bytes = up16(maps * s.channels * 4);
@@ -303,7 +326,8 @@ int launch_recurrence_backward(const DsbRecurrence& shape, const void* x, const 
     c.launch.args.x = scan_base(x, r, shape.rows, shape.x_stride, elem);
     c.launch.args.gate = scan_base(gate, r, shape.rows, shape.gate_stride, elem);
     c.launch.args.v_h = scan_base(v_h, r, shape.rows, v_h_stride, elem);
-    c.launch.args.v_h_stride = r ? -v_h_stride : v_h_stride;
+    c.launch.args.v_h_stride = (r ? -v_h_stride : v_h_stride) * elem;
+    c.launch.args.v_h_step = c.layout.tile_rows * c.launch.args.v_h_stride;
     c.launch.args.v_x = scan_base(v_x, r, shape.rows, shape.channels, elem);
     c.launch.args.v_gate = scan_base(v_gate, r, shape.rows, shape.gate_heads, elem);
     c.launch.args.state_in = state_in; c.launch.args.v_state_out = v_state_out; c.launch.args.v_state_in = v_state_in;

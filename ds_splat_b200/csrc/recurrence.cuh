@@ -39,8 +39,10 @@ struct RecurrenceArgs {
     const int *offsets, *lengths;
     int* device_status;
     int rows, chain_rows, chains;
-    long long x_stride, gate_stride, v_h_stride;   // negative when the scan runs from the last row to the first
-    long long h_stride, gate_out_stride;           // channels / heads of contiguous results, with the same sign
+    // In bytes; negative when the scan runs from the last row to the first.
+    long long x_stride, gate_stride, v_h_stride;   // from row to row
+    long long h_stride, gate_out_stride;           // contiguous results of channels / heads
+    long long x_step, gate_step, v_h_step, h_step, gate_out_step;   // from tile to tile
     int tiles, segments, segment_tiles;
     int sequences, sequence_rows, channels, gate_heads, heads, per_head, parts, lg_tx;
     int reverse, table;    // table: one chain over all rows, with sequence borders anywhere; else one chain per sequence
@@ -59,7 +61,58 @@ constexpr int kWalkWarps = kWalkThreads / 32;
 
 // Consecutive rows of a thread: as many as keep the backward's values of a tile in registers and two tiles of every tensor
 // in shared memory with several blocks on an SM.
-template <typename T> __host__ __device__ constexpr int walk_rows(int vec) { return vec == 4 ? (sizeof(T) == 4 ? 4 : 8) : 16; }
+template <typename T> __host__ __device__ constexpr int walk_rows(int vec) { return vec == 4 ? (sizeof(T) == 4 ? 4 : 6) : 16; }
+
+// ---- V channels at a time -------------------------------------------------------------------------------------------
+// Two channels an instruction where the hardware has one; `a` may be a single value for all channels.
+__device__ __forceinline__ u64 pair_of(float lo, float hi) {
+    u64 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void split_pair(u64 r, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(r)); }
+template <int V, int A>
+__device__ __forceinline__ void mul_add(float (&r)[V], const float (&a)[A], const float (&b)[V], const float (&c)[V]) {
+    if constexpr (V % 2 == 0) {
+#pragma unroll
+        for (int v = 0; v < V; v += 2) {
+            u64 o;
+            asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(o) : "l"(pair_of(a[v % A], a[(v + 1) % A])), "l"(pair_of(b[v], b[v + 1])), "l"(pair_of(c[v], c[v + 1])));
+            split_pair(o, r[v], r[v + 1]);
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) r[v] = fmaf(a[v % A], b[v], c[v]);
+    }
+}
+template <int V, int A>
+__device__ __forceinline__ void mul(float (&r)[V], const float (&a)[A], const float (&b)[V]) {
+    if constexpr (V % 2 == 0) {
+#pragma unroll
+        for (int v = 0; v < V; v += 2) {
+            u64 o;
+            asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(o) : "l"(pair_of(a[v % A], a[(v + 1) % A])), "l"(pair_of(b[v], b[v + 1])));
+            split_pair(o, r[v], r[v + 1]);
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) r[v] = a[v % A] * b[v];
+    }
+}
+template <int V, int A>
+__device__ __forceinline__ void add(float (&r)[V], const float (&a)[A], const float (&b)[V]) {
+    if constexpr (V % 2 == 0) {
+#pragma unroll
+        for (int v = 0; v < V; v += 2) {
+            u64 o;
+            asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(o) : "l"(pair_of(a[v % A], a[(v + 1) % A])), "l"(pair_of(b[v], b[v + 1])));
+            split_pair(o, r[v], r[v + 1]);
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) r[v] = a[v % A] + b[v];
+    }
+}
 
 // ---- gates ---------------------------------------------------------------------------------------------------------
 // A gate is kept as one register: a decay as itself, a logit g as e = exp(-g), from which f = 1 / (1 + e) and 1 - f = e f
@@ -67,42 +120,67 @@ template <typename T> __host__ __device__ constexpr int walk_rows(int vec) { ret
 // normal number (1.2e-38); a NaN stays one.
 // Errors, with u = 2^-24 and L = log2 e: 2^x by the hardware 4 u, its argument's rounding |g| 1.2 u, the quotient 2 u, 1 + e and
 // the product u each.  32-bit gates get the argument's rounding error back to first order (three instructions more).
-template <typename T, bool LOGIT>
-__device__ __forceinline__ float gate_register(T gate) {
-    const float g = to_float(gate);
-    if (!LOGIT) return g;
+template <typename T, bool LOGIT, int A>
+__device__ __forceinline__ void gate_registers(const Pack<T, A>& gate, float (&e)[A]) {
+    float g[A];
+#pragma unroll
+    for (int v = 0; v < A; ++v) g[v] = to_float(gate.e[v]);
     constexpr float kLog2e = 1.44269502f, kLn2 = 0.693147181f;
-    float e;
-    if (sizeof(T) == 4) {
-        float y;
-        asm("{\n\t.reg .f32 t;\n\tmin.NaN.f32 t, %1, 0f42AE0000;\n\tmax.NaN.f32 %0, t, 0fC2AE0000;\n\t}" : "=f"(y) : "f"(-g));   // +-87
-        const float hi = y * kLog2e, lo = fmaf(y, kLog2e, -hi);
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(hi));
-        e = fmaf(e, lo * kLn2, e);
+    if constexpr (!LOGIT) {
+#pragma unroll
+        for (int v = 0; v < A; ++v) e[v] = g[v];
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int v = 0; v < A; ++v) {
+            float y;
+            asm("{\n\t.reg .f32 t;\n\tmin.NaN.f32 t, %1, 0f42AE0000;\n\tmax.NaN.f32 %0, t, 0fC2AE0000;\n\t}" : "=f"(y) : "f"(-g[v]));   // +-87
+            const float hi = y * kLog2e, lo = fmaf(y, kLog2e, -hi);
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[v]) : "f"(hi));
+            e[v] = fmaf(e[v], lo * kLn2, e[v]);
+        }
     } else {
-        float t;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(g * -kLog2e));
-        asm("min.NaN.f32 %0, %1, 0f7E800000;" : "=f"(e) : "f"(t));
+        const float scale[1] = {-kLog2e};
+        float y[A];
+        mul(y, scale, g);
+#pragma unroll
+        for (int v = 0; v < A; ++v) {
+            float t;
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(y[v]));
+            asm("min.NaN.f32 %0, %1, 0f7E800000;" : "=f"(e[v]) : "f"(t));
+        }
     }
-    return e;
 }
-template <bool LOGIT>
-__device__ __forceinline__ float gate_f(float e) {
-    if (!LOGIT) return e;
-    float f;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(f) : "f"(1.f + e));
-    return f;
+// f and k = 1 - f.  volatile: worked out again where they are used again, rather than kept in a register per element (the
+// backward's values of a tile then fit the registers of more blocks on an SM).
+template <bool LOGIT, int A>
+__device__ __forceinline__ void gate_f(const float (&e)[A], float (&f)[A]) {
+    if constexpr (!LOGIT) {
+#pragma unroll
+        for (int v = 0; v < A; ++v) f[v] = e[v];
+    } else {
+        const float one[1] = {1.f};
+        float d[A];
+        add(d, one, e);
+#pragma unroll
+        for (int v = 0; v < A; ++v) asm volatile("rcp.approx.ftz.f32 %0, %1;" : "=f"(f[v]) : "f"(d[v]));
+    }
 }
-template <bool LOGIT>
-__device__ __forceinline__ float gate_k(float e, float f) {   // 1 - f
-    return LOGIT ? e * f : 1.f - f;
+template <bool LOGIT, int A>
+__device__ __forceinline__ void gate_k(const float (&e)[A], const float (&f)[A], float (&k)[A]) {
+    if constexpr (LOGIT) {
+        mul(k, e, f);
+    } else {
+#pragma unroll
+        for (int v = 0; v < A; ++v) k[v] = 1.f - f[v];
+    }
 }
 
 // ---- rows that begin and end sequences ------------------------------------------------------------------------------
 // In the order of the scan: position p is row p, or rows - 1 - p when the scan runs backwards; sequence k of the scan is
 // the tensor's sequence k, or sequences - 1 - k.
 constexpr int kNone = -1, kOutside = -2;
-constexpr int kTables = 3;      // one is read, one was read by the slowest warp, one is written
+constexpr int kStages = 2;              // tiles in shared memory: one is worked on, the others are on their way
+constexpr int kTables = kStages + 1;    // border tables: besides, the slowest warp may still read the tile before
 
 __device__ __forceinline__ int sequence_id(const RecurrenceArgs& a, int k) { return a.reverse ? a.sequences - 1 - k : k; }
 // Where the scan's packed sequence k begins (k = sequences: where the last one ends).
@@ -272,22 +350,19 @@ __device__ __forceinline__ void identity(Map<V, A>& m) {
 template <bool PLAIN, int V, int A>
 __device__ __forceinline__ void compose_after(Map<V, A>& m, const Map<V, A>& e) {
     const bool open = PLAIN || !m.closed;
+    float b[V];
+    mul_add(b, m.a, e.b, m.b);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const float b = fmaf(m.a[v % A], e.b[v], m.b[v]);
-        m.b[v] = open ? b : m.b[v];
-    }
-#pragma unroll
-    for (int v = 0; v < A; ++v) m.a[v] *= e.a[v];
+    for (int v = 0; v < V; ++v) m.b[v] = open ? b[v] : m.b[v];
+    mul(m.a, e.a, m.a);
     if (!PLAIN) m.closed |= e.closed;
 }
 template <bool PLAIN, int V, int A>
 __device__ __forceinline__ void apply_map(float (&h)[V], const Map<V, A>& m) {
+    float n[V];
+    mul_add(n, m.a, h, m.b);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const float n = fmaf(m.a[v % A], h[v], m.b[v]);
-        h[v] = PLAIN || !m.closed ? n : m.b[v];
-    }
+    for (int v = 0; v < V; ++v) h[v] = PLAIN || !m.closed ? n[v] : m.b[v];
 }
 
 // The warps' maps of one tile.
@@ -350,7 +425,7 @@ __device__ __forceinline__ Map<V, A> warp_map(const WarpMaps<V, A>& sh, int warp
 // carry: the state before the tile -> the state after it; mine: the state before this thread's warp.
 template <bool FORWARD, bool PLAIN, int V, int A>
 __device__ __forceinline__ void pass_warps(const WarpMaps<V, A>& sh, int tx, float (&carry)[V], float (&mine)[V]) {
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);   // the same in the whole warp: no divergence below
 #pragma unroll
     for (int i = 0; i < kWalkWarps; ++i) {
         const int w = FORWARD ? i : kWalkWarps - 1 - i;
@@ -427,39 +502,32 @@ struct alignas(16) TileStage {
     T v[TENSORS][L][kWalkThreads][V];
 };
 
-// A thread's view of one tensor: its first row of the tile that is fetched next.  The walk moves it from tile to tile.
-template <typename T>
-struct RowPointer {
-    const T* at;
-    long long stride, step;    // to the next row, to the same row of the next tile of the walk
-    __device__ __forceinline__ RowPointer(const T* base, int channel, long long row_stride, const RecurrenceArgs& a, const Place& p,
-                                          int tile, int tile_rows, bool forward) {
-        stride = row_stride;
-        step = forward ? tile_rows * row_stride : -(tile_rows * row_stride);
-        at = base + ((long long)p.chain * a.chain_rows + (long long)tile * tile_rows + p.row0) * row_stride + channel;
-    }
-};
+// A thread's first element of a tile, as a byte address.
+template <typename T, typename Byte>
+__device__ __forceinline__ Byte* row_pointer(Byte* base, int channel, long long stride, const RecurrenceArgs& a, const Place& p, int tile,
+                                             int tile_rows) {
+    return base + ((long long)p.chain * a.chain_rows + (long long)tile * tile_rows + p.row0) * stride + channel * (long long)sizeof(T);
+}
 // The thread's rows of a tile, `left` of them within the chain (L: all, known to the whole block); the others become zeros.
 // Rows that belong to no sequence but lie within the tensor are copied like the others and masked where they are used.
 template <typename T, int V, int L>
-__device__ __forceinline__ void fetch_rows(unsigned to, const RowPointer<T>& r, bool full, int left) {
+__device__ __forceinline__ void fetch_rows(unsigned to, const char* from, const long long& stride, bool full, int left, const char* base) {
     constexpr unsigned kRow = kWalkThreads * V * sizeof(T);
-    const T* from = r.at;
     if (full) {
 #pragma unroll
-        for (int l = 0; l < L; ++l, from += r.stride) copy_async<T, V>(to + l * kRow, from, true);
+        for (int l = 0; l < L; ++l, from += stride) copy_async<T, V>(to + l * kRow, reinterpret_cast<const T*>(from), true);
     } else {
 #pragma unroll 1
-        for (int l = 0; l < L; ++l) copy_async<T, V>(to + l * kRow, l < left ? from + l * r.stride : static_cast<const T*>(from), l < left);
+        for (int l = 0; l < L; ++l) copy_async<T, V>(to + l * kRow, reinterpret_cast<const T*>(l < left ? from + l * stride : base), l < left);
     }
 }
 // A gate that channels share is read directly, as every thread of a row wants the same value.
 template <typename T, int L>
-__device__ __forceinline__ void fetch_shared_gates(T (&own)[L], const RowPointer<T>& r, int left) {
+__device__ __forceinline__ void fetch_shared_gates(T (&own)[L], const char* from, const long long& stride, int left) {
 #pragma unroll
     for (int l = 0; l < L; ++l) {
         memset(&own[l], 0, sizeof(T));
-        if (l < left) own[l] = r.at[l * r.stride];
+        if (l < left) own[l] = *reinterpret_cast<const T*>(from + l * stride);
     }
 }
 
@@ -518,15 +586,15 @@ __device__ __forceinline__ void store_segment_map(const RecurrenceArgs& a, const
 
 // A tile of rows that belong to no sequence.
 template <typename T, int V, int L>
-__device__ __forceinline__ void store_zero_rows(T* to, long long stride, int left) {
+__device__ __forceinline__ void store_zero_rows(char* to, long long stride, int left) {
     const float zero[V] = {};
 #pragma unroll 1
     for (int l = 0; l < L; ++l)
-        if (l < left) store_floats<T, V>(to + l * stride, zero);
+        if (l < left) store_floats<T, V>(reinterpret_cast<T*>(to + l * stride), zero);
 }
 
 template <typename T, int V, bool LOGIT, bool COUPLED, bool SHARED, bool APPLY>
-__global__ void __launch_bounds__(kWalkThreads, 4)
+__global__ void __launch_bounds__(kWalkThreads)
 recurrence_forward_kernel(const RecurrenceArgs a) {
     constexpr int L = walk_rows<T>(V), A = SHARED ? 1 : V;
     typedef TileStage<T, V, L, SHARED ? 1 : 2> Ring;
@@ -536,13 +604,13 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
     const int tile_rows = kWalkWarps * (32 >> a.lg_tx) * L;
     const Place p = place_of<V, L>(a);
     const int t0 = p.segment * a.segment_tiles, t1 = min(t0 + a.segment_tiles, a.tiles);
-    RowPointer<T> x(static_cast<const T*>(a.x), p.read_channel, a.x_stride, a, p, t0, tile_rows, true);
-    RowPointer<T> gate(static_cast<const T*>(a.gate), SHARED ? p.head : p.read_channel, a.gate_stride, a, p, t0, tile_rows, true);
+    const char* x = row_pointer<T>(static_cast<const char*>(a.x), p.read_channel, a.x_stride, a, p, t0, tile_rows);
+    const char* gate = row_pointer<T>(static_cast<const char*>(a.gate), SHARED ? p.head : p.read_channel, a.gate_stride, a, p, t0, tile_rows);
     const unsigned s_ring = (unsigned)__cvta_generic_to_shared(s_raw) + threadIdx.x * V * sizeof(T);
     constexpr unsigned kTensor = L * kWalkThreads * V * sizeof(T);
     const int groups = kWalkWarps * (32 >> a.lg_tx);
     const bool wanted = APPLY && a.h && p.active;
-    T* to_h = static_cast<T*>(a.h) + ((long long)p.chain * a.chain_rows + (long long)t0 * tile_rows + p.row0) * a.h_stride + p.channel;
+    char* to_h = row_pointer<T>(static_cast<char*>(a.h), p.channel, a.h_stride, a, p, t0, tile_rows);
     const bool keep = APPLY && a.checkpoints && p.active;
     float* to_start = a.checkpoints + (((long long)p.chain * a.tiles + t0) * groups + p.group) * a.channels + p.channel;
 
@@ -551,38 +619,49 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
     identity(all);
     if (APPLY) carry_of_segment<true>(a, p, sh[0], carry);
     Borders<true> borders;
-    borders.begin(a, p.chain, t0 * tile_rows, reinterpret_cast<int*>(s_raw + 2 * sizeof(Ring)), tile_rows);
+    borders.begin(a, p.chain, t0 * tile_rows, reinterpret_cast<int*>(s_raw + kStages * sizeof(Ring)), tile_rows);
     T gate_now[L], gate_next[L];
-    // Fetches tile t, the next of the walk, and moves on; tiles without rows of a sequence are only passed.
-    auto fetch = [&](int stage, int t, int kind) {
-        if (kind != kEmpty) {
-            const int rest = a.chain_rows - t * tile_rows;
-            const int left = min(rest - p.row0, L);
-            fetch_rows<T, V, L>(s_ring + stage * sizeof(Ring), x, rest >= tile_rows, left);
-            if (SHARED) fetch_shared_gates<T, L>(gate_next, gate, left);
-            else fetch_rows<T, V, L>(s_ring + stage * sizeof(Ring) + kTensor, gate, rest >= tile_rows, left);
+    // Fetches tile t, the next of the walk, into the stage `fetched` and moves on; tiles without rows of a sequence are only
+    // passed.  Their kinds wait in `kinds`, two bits each, the tile that is worked on lowest.
+    unsigned kinds = 0;
+    int fetched = 0;
+    auto fetch = [&](int t, int ahead) {
+        if (t < t1) {
+            const int kind = borders.prepare(a, t, t * tile_rows);
+            kinds |= (unsigned)kind << (2 * ahead);
+            if (kind != kEmpty) {
+                const int rest = a.chain_rows - t * tile_rows;
+                const int left = min(rest - p.row0, L);
+                const unsigned to = s_ring + fetched * sizeof(Ring);
+                fetch_rows<T, V, L>(to, x, a.x_stride, rest >= tile_rows, left, static_cast<const char*>(a.x));
+                if (!SHARED) fetch_rows<T, V, L>(to + kTensor, gate, a.gate_stride, rest >= tile_rows, left, static_cast<const char*>(a.gate));
+            }
+            x += a.x_step;
+            if (!SHARED) gate += a.gate_step;
         }
-        x.at += x.step;
-        gate.at += gate.step;
+        fetched = fetched + 1 == kStages ? 0 : fetched + 1;
         copies_issued();
     };
-    int kind = borders.prepare(a, t0, t0 * tile_rows), kind_next = kEmpty;
-    fetch(0, t0, kind);
+    auto fetch_gates = [&](int t) {
+        fetch_shared_gates<T, L>(gate_next, gate, a.gate_stride, t < t1 ? min(a.chain_rows - t * tile_rows - p.row0, L) : 0);
+        gate += a.gate_step;
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) fetch(t0 + i, i);
+    if (SHARED) fetch_gates(t0);
     __syncthreads();
-    for (int t = t0; t < t1; ++t, kind = kind_next, to_h += tile_rows * a.h_stride, to_start += (long long)groups * a.channels) {
-        const int stage = (t - t0) & 1;
+    int stage = 0;
+    for (int t = t0; t < t1; ++t, kinds >>= 2, stage = stage + 1 == kStages ? 0 : stage + 1, to_h += a.h_step,
+             to_start += (long long)groups * a.channels) {
+        const int kind = kinds & 3u;
         const int p0 = t * tile_rows;
         if (SHARED) {
 #pragma unroll
             for (int l = 0; l < L; ++l) gate_now[l] = gate_next[l];
+            fetch_gates(t + 1);
         }
-        if (t + 1 < t1) {
-            kind_next = borders.prepare(a, t + 1, p0 + tile_rows);
-            fetch(stage ^ 1, t + 1, kind_next);
-            copies_landed<1>();
-        } else {
-            copies_landed<0>();
-        }
+        fetch(t + kStages - 1, kStages - 1);
+        copies_landed<kStages - 1>();
         const int left = min(a.chain_rows - p0 - p.row0, L);
         if (kind == kEmpty) {
             if (wanted) store_zero_rows<T, V, L>(to_h, a.h_stride, left);
@@ -607,28 +686,33 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
                     load_state<V>(p.active ? a.state_in : nullptr, s, a.channels, p.channel, own.b);
                     own.closed = 1;
                 }
-                float k[A];
+                float e[A], k[A], xv[V];
+                gate_registers<T, LOGIT>(pg, e);
+                gate_f<LOGIT>(e, f[l]);
 #pragma unroll
-                for (int v = 0; v < A; ++v) {
-                    const float e = gate_register<T, LOGIT>(pg.e[v]);
-                    f[l][v] = gate_f<LOGIT>(e);
-                    k[v] = gate_k<LOGIT>(e, f[l][v]);
-                    if (outside) f[l][v] = 1.f;
-                    own.a[v] *= f[l][v];
-                }
+                for (int v = 0; v < V; ++v) xv[v] = to_float(px.e[v]);
+                if (COUPLED) {
+                    gate_k<LOGIT>(e, f[l], k);
+                    mul(b[l], k, xv);
+                } else {
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const float xv = to_float(px.e[v]);
-                    b[l][v] = outside ? 0.f : COUPLED ? xv * k[v % A] : xv;
-                    own.b[v] = fmaf(f[l][v % A], own.b[v], b[l][v]);
+                    for (int v = 0; v < V; ++v) b[l][v] = xv[v];
                 }
+                if (outside) {
+#pragma unroll
+                    for (int v = 0; v < A; ++v) f[l][v] = 1.f;
+#pragma unroll
+                    for (int v = 0; v < V; ++v) b[l][v] = 0.f;
+                }
+                mul(own.a, f[l], own.a);
+                mul_add(own.b, f[l], own.b, b[l]);
             }
-            const Map<V, A> before = compose_warp<true, PLAIN>(own, a.lg_tx, sh[stage]);
+            const Map<V, A> before = compose_warp<true, PLAIN>(own, a.lg_tx, sh[t & 1]);
             __syncthreads();
             if (!APPLY) {
 #pragma unroll
                 for (int w = 0; w < kWalkWarps; ++w) {
-                    Map<V, A> m = warp_map<PLAIN>(sh[stage], w, p.tx);
+                    Map<V, A> m = warp_map<PLAIN>(sh[t & 1], w, p.tx);
                     const int closed = all.closed;
                     compose_after<PLAIN>(m, all);
                     if (PLAIN) m.closed = closed;
@@ -637,21 +721,19 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
                 return;
             }
             float h[V];
-            pass_warps<true, PLAIN>(sh[stage], p.tx, carry, h);
+            pass_warps<true, PLAIN>(sh[t & 1], p.tx, carry, h);
             apply_map<PLAIN>(h, before);
             store_floats_if<float, V>(to_start, h, keep);
-            T* to = to_h;
+            char* to = to_h;
 #pragma unroll
             for (int l = 0; l < L; ++l) {
                 const int s = PLAIN ? kNone : first[l], e = PLAIN ? kNone : end[l];
                 if (s >= 0) load_state<V>(p.active ? a.state_in : nullptr, s, a.channels, p.channel, h);
                 float o[V];
+                mul_add(h, f[l], h, b[l]);
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    h[v] = fmaf(f[l][v % A], h[v], b[l][v]);
-                    o[v] = s == kOutside ? 0.f : h[v];
-                }
-                store_floats_if<T, V>(to, o, wanted && (PLAIN || l < left));
+                for (int v = 0; v < V; ++v) o[v] = s == kOutside ? 0.f : h[v];
+                store_floats_if<T, V>(reinterpret_cast<T*>(to), o, wanted && (PLAIN || l < left));
                 to += a.h_stride;
                 if (e >= 0 && p.active) store_floats<float, V>(a.state_out + (long long)e * a.channels + p.channel, h);
             }
@@ -664,7 +746,7 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
 }
 
 template <typename T, int V, bool LOGIT, bool COUPLED, bool SHARED, bool APPLY>
-__global__ void __launch_bounds__(kWalkThreads, 3)
+__global__ void __launch_bounds__(kWalkThreads)
 recurrence_backward_kernel(const RecurrenceArgs a) {
     constexpr int L = walk_rows<T>(V), A = SHARED ? 1 : V;
     constexpr int kX = 1, kGate = 2;                    // places in a stage; v_h has the first
@@ -676,17 +758,18 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
     const int tile_rows = kWalkWarps * (32 >> a.lg_tx) * L;
     const Place p = place_of<V, L>(a);
     const int t0 = p.segment * a.segment_tiles, t1 = min(t0 + a.segment_tiles, a.tiles);
-    RowPointer<T> vh(static_cast<const T*>(a.v_h), p.read_channel, a.v_h_stride, a, p, t1 - 1, tile_rows, false);
-    RowPointer<T> x(static_cast<const T*>(a.x), p.read_channel, a.x_stride, a, p, t1 - 1, tile_rows, false);
-    RowPointer<T> gate(static_cast<const T*>(a.gate), SHARED ? p.head : p.read_channel, a.gate_stride, a, p, t1 - 1, tile_rows, false);
+    const char* vh = row_pointer<T>(static_cast<const char*>(a.v_h), p.read_channel, a.v_h_stride, a, p, t1 - 1, tile_rows);
+    const char* x = row_pointer<T>(static_cast<const char*>(a.x), p.read_channel, a.x_stride, a, p, t1 - 1, tile_rows);
+    const char* gate = row_pointer<T>(static_cast<const char*>(a.gate), SHARED ? p.head : p.read_channel, a.gate_stride, a, p, t1 - 1, tile_rows);
     const unsigned s_ring = (unsigned)__cvta_generic_to_shared(s_raw) + threadIdx.x * V * sizeof(T);
     constexpr unsigned kTensor = L * kWalkThreads * V * sizeof(T);
     const int groups = kWalkWarps * (32 >> a.lg_tx);
     const long long row_first = (long long)p.chain * a.chain_rows + (long long)(t1 - 1) * tile_rows + p.row0;
     const bool want_x = APPLY && a.v_x && p.active, want_gate = APPLY && a.v_gate && !SHARED && p.active;
-    T* to_x = static_cast<T*>(a.v_x) + row_first * a.h_stride + p.channel;
-    T* to_gate = static_cast<T*>(a.v_gate) + row_first * a.gate_out_stride + (SHARED ? p.head : p.channel);
+    char* to_x = row_pointer<T>(static_cast<char*>(a.v_x), p.channel, a.h_stride, a, p, t1 - 1, tile_rows);
+    char* to_gate = row_pointer<T>(static_cast<char*>(a.v_gate), SHARED ? p.head : p.channel, a.gate_out_stride, a, p, t1 - 1, tile_rows);
     float* to_part = a.gate_parts + ((a.reverse ? a.rows - 1 - row_first : row_first) + (long long)p.part * a.rows) * a.gate_heads + p.head;
+    const int part_stride = a.reverse ? -a.gate_heads : a.gate_heads;
     const float* from_start = a.checkpoints + (((long long)p.chain * a.tiles + t1 - 1) * groups + p.group) * a.channels + p.read_channel;
 
     float q_carry[V], start[V], start_next[V];
@@ -694,35 +777,54 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
     identity(all);
     if (APPLY) carry_of_segment<false>(a, p, sh[0], q_carry);
     Borders<false> borders;
-    borders.begin(a, p.chain, (t1 - 1) * tile_rows, reinterpret_cast<int*>(s_raw + 2 * sizeof(Ring)), tile_rows);
+    borders.begin(a, p.chain, (t1 - 1) * tile_rows, reinterpret_cast<int*>(s_raw + kStages * sizeof(Ring)), tile_rows);
     T gate_now[L], gate_next[L];
-    auto fetch = [&](int stage, int t, int kind) {
-        if (kind != kEmpty) {
-            const int rest = a.chain_rows - t * tile_rows;
-            const int left = min(rest - p.row0, L);
-            const unsigned to = s_ring + stage * sizeof(Ring);
-            if (a.v_h) fetch_rows<T, V, L>(to, vh, rest >= tile_rows, left);
-            if (SHARED) fetch_shared_gates<T, L>(gate_next, gate, left);
-            else fetch_rows<T, V, L>(to + kGateAt * kTensor, gate, rest >= tile_rows, left);
-            if (APPLY) {
-                fetch_rows<T, V, L>(to + kXAt * kTensor, x, rest >= tile_rows, left);
-                const Pack<float, V> pack = load_pack<float, V>(from_start);
-#pragma unroll
-                for (int v = 0; v < V; ++v) start_next[v] = pack.e[v];
+    unsigned kinds = 0;    // as in the forward
+    int fetched = 0;
+    auto fetch = [&](int t, int ahead) {
+        if (t >= t0) {
+            const int kind = borders.prepare(a, t, t * tile_rows);
+            kinds |= (unsigned)kind << (2 * ahead);
+            if (kind != kEmpty) {
+                const int rest = a.chain_rows - t * tile_rows;
+                const int left = min(rest - p.row0, L);
+                const unsigned to = s_ring + fetched * sizeof(Ring);
+                if (a.v_h) fetch_rows<T, V, L>(to, vh, a.v_h_stride, rest >= tile_rows, left, static_cast<const char*>(a.v_h));   // else zeros, put there before
+                if (!SHARED) fetch_rows<T, V, L>(to + kGateAt * kTensor, gate, a.gate_stride, rest >= tile_rows, left, static_cast<const char*>(a.gate));
+                if (APPLY) fetch_rows<T, V, L>(to + kXAt * kTensor, x, a.x_stride, rest >= tile_rows, left, static_cast<const char*>(a.x));
             }
+            vh -= a.v_h_step;
+            x -= a.x_step;
+            if (!SHARED) gate -= a.gate_step;
         }
-        vh.at += vh.step;
-        x.at += x.step;
-        gate.at += gate.step;
-        from_start -= (long long)groups * a.channels;
+        fetched = fetched + 1 == kStages ? 0 : fetched + 1;
         copies_issued();
     };
-    int kind = borders.prepare(a, t1 - 1, (t1 - 1) * tile_rows), kind_next = kEmpty;
-    fetch(0, t1 - 1, kind);
+    // what goes through registers: one tile ahead
+    auto fetch_next = [&](int t) {
+        if (SHARED) {
+            fetch_shared_gates<T, L>(gate_next, gate, a.gate_stride, t >= t0 ? min(a.chain_rows - t * tile_rows - p.row0, L) : 0);
+            gate -= a.gate_step;
+        }
+        if (APPLY && t >= t0) {
+            const Pack<float, V> pack = load_pack<float, V>(from_start);
+#pragma unroll
+            for (int v = 0; v < V; ++v) start_next[v] = pack.e[v];
+            from_start -= (long long)groups * a.channels;
+        }
+    };
+    if (!a.v_h) {
+#pragma unroll 1
+        for (int i = 0; i < kStages * L; ++i) memset(ring[i / L].v[0][i % L][threadIdx.x], 0, V * sizeof(T));
+    }
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) fetch(t1 - 1 - i, i);
+    fetch_next(t1 - 1);
     __syncthreads();
-    for (int t = t1 - 1; t >= t0; --t, kind = kind_next, to_x -= tile_rows * a.h_stride, to_gate -= tile_rows * a.gate_out_stride,
-             to_part -= tile_rows * a.gate_out_stride) {
-        const int stage = (t1 - 1 - t) & 1;
+    int stage = 0;
+    for (int t = t1 - 1; t >= t0; --t, kinds >>= 2, stage = stage + 1 == kStages ? 0 : stage + 1, to_x -= a.h_step,
+             to_gate -= a.gate_out_step, to_part -= (long long)tile_rows * part_stride) {
+        const int kind = kinds & 3u;
         const int p0 = t * tile_rows;
         if (SHARED) {
 #pragma unroll
@@ -730,18 +832,14 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) start[v] = start_next[v];
-        if (t > t0) {
-            kind_next = borders.prepare(a, t - 1, p0 - tile_rows);
-            fetch(stage ^ 1, t - 1, kind_next);
-            copies_landed<1>();
-        } else {
-            copies_landed<0>();
-        }
+        fetch_next(t - 1);
+        fetch(t - kStages + 1, kStages - 1);
+        copies_landed<kStages - 1>();
         const int left = min(a.chain_rows - p0 - p.row0, L);
         // a shared gate's sum over this block's channels
         auto store_gate_sum = [&](int l, float sum) {
-            if (a.parts == 1) from_float(sum, to_gate[l * a.gate_out_stride]);
-            else to_part[l * a.gate_out_stride] = sum;
+            if (a.parts == 1) from_float(sum, *reinterpret_cast<T*>(to_gate + l * a.gate_out_stride));
+            else to_part[(long long)l * part_stride] = sum;
         };
         if (kind == kEmpty) {
             if (want_x) store_zero_rows<T, V, L>(to_x, a.h_stride, left);
@@ -764,25 +862,25 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                 Pack<T, A> g;
                 if (SHARED) g.e[0] = gate_now[l];
                 else g = load_pack<T, A>(&ring[stage].v[kGateAt][l][threadIdx.x][0]);
-                Pack<T, V> d;
-                if (a.v_h) d = load_pack<T, V>(ring[stage].v[0][l][threadIdx.x]);
+                const Pack<T, V> d = load_pack<T, V>(ring[stage].v[0][l][threadIdx.x]);
                 if (e >= 0) {
                     load_state<V>(p.active ? a.v_state_out : nullptr, e, a.channels, p.channel, own.b);
                     own.closed = 1;
                 }
-                float f[A];
+                float f[A], dv[V];
+                gate_registers<T, LOGIT>(g, m[l]);
+                gate_f<LOGIT>(m[l], f);
 #pragma unroll
-                for (int v = 0; v < A; ++v) {
-                    m[l][v] = gate_register<T, LOGIT>(g.e[v]);
-                    f[v] = gate_f<LOGIT>(m[l][v]);
-                    if (outside) f[v] = 1.f;
-                    own.a[v] *= f[v];
+                for (int v = 0; v < V; ++v) dv[v] = outside ? 0.f : to_float(d.e[v]);
+                if (outside) {
+#pragma unroll
+                    for (int v = 0; v < A; ++v) f[v] = 1.f;
                 }
-#pragma unroll
-                for (int v = 0; v < V; ++v)
-                    own.b[v] = f[v % A] * ((a.v_h && !outside ? to_float(d.e[v]) : 0.f) + own.b[v]);
+                mul(own.a, f, own.a);
+                add(own.b, dv, own.b);
+                mul(own.b, f, own.b);
             }
-            const Map<V, A> after = compose_warp<false, PLAIN>(own, a.lg_tx, sh[stage]);
+            const Map<V, A> after = compose_warp<false, PLAIN>(own, a.lg_tx, sh[t & 1]);
             if (APPLY) {                       // u_t: h_{t-1}, coupled: h_{t-1} - x_t
                 float h[V];
 #pragma unroll
@@ -792,26 +890,29 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                     const int s = PLAIN ? kNone : first[l];
                     if (s >= 0) load_state<V>(p.active ? a.state_in : nullptr, s, a.channels, p.channel, h);
                     const Pack<T, V> xl = load_pack<T, V>(ring[stage].v[kXAt][l][threadIdx.x]);
-                    float f[A], k[A];
+                    float f[A], k[A], xv[V], n[V];
+                    gate_f<LOGIT>(m[l], f);
 #pragma unroll
-                    for (int v = 0; v < A; ++v) {
-                        f[v] = gate_f<LOGIT>(m[l][v]);
-                        k[v] = gate_k<LOGIT>(m[l][v], f[v]);
-                    }
+                    for (int v = 0; v < V; ++v) xv[v] = to_float(xl.e[v]);
+                    if (COUPLED) {
+                        const float minus[1] = {-1.f};
+                        mul_add(u[l], minus, xv, h);
+                        gate_k<LOGIT>(m[l], f, k);
+                        mul(xv, k, xv);
+                    } else {
 #pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        const float xv = to_float(xl.e[v]);
-                        u[l][v] = COUPLED ? h[v] - xv : h[v];
-                        const float n = fmaf(f[v % A], h[v], COUPLED ? xv * k[v % A] : xv);
-                        h[v] = s == kOutside ? h[v] : n;
+                        for (int v = 0; v < V; ++v) u[l][v] = h[v];
                     }
+                    mul_add(n, f, h, xv);
+#pragma unroll
+                    for (int v = 0; v < V; ++v) h[v] = s == kOutside ? h[v] : n[v];
                 }
             }
             __syncthreads();
             if (!APPLY) {
 #pragma unroll
                 for (int w = kWalkWarps - 1; w >= 0; --w) {
-                    Map<V, A> n = warp_map<PLAIN>(sh[stage], w, p.tx);
+                    Map<V, A> n = warp_map<PLAIN>(sh[t & 1], w, p.tx);
                     const int closed = all.closed;
                     compose_after<PLAIN>(n, all);
                     if (PLAIN) n.closed = closed;
@@ -820,34 +921,45 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                 return;
             }
             float q[V];
-            pass_warps<false, PLAIN>(sh[stage], p.tx, q_carry, q);
+            pass_warps<false, PLAIN>(sh[t & 1], p.tx, q_carry, q);
             apply_map<PLAIN>(q, after);
+            char *row_x = to_x + (L - 1) * a.h_stride, *row_gate = to_gate + (L - 1) * a.gate_out_stride;
 #pragma unroll
             for (int l = L - 1; l >= 0; --l) {
                 const int s = PLAIN ? kNone : first[l], e = PLAIN ? kNone : end[l];
                 const bool outside = s == kOutside;
                 if (e >= 0) load_state<V>(p.active ? a.v_state_out : nullptr, e, a.channels, p.channel, q);
-                Pack<T, V> d;
-                if (a.v_h) d = load_pack<T, V>(ring[stage].v[0][l][threadIdx.x]);
-                float f[A], k[A], slope[A], dx[V], dg[V], sum = 0.f;
+                const Pack<T, V> d = load_pack<T, V>(ring[stage].v[0][l][threadIdx.x]);
+                float f[A], k[A], slope[A], dx[V], dg[V], g[V], n[V], sum = 0.f;
+                gate_f<LOGIT>(m[l], f);
+                gate_k<LOGIT>(m[l], f, k);
+                if (LOGIT) mul(slope, f, k);
+                else slope[0] = 1.f;
 #pragma unroll
-                for (int v = 0; v < A; ++v) {
-                    f[v] = gate_f<LOGIT>(m[l][v]);
-                    k[v] = gate_k<LOGIT>(m[l][v], f[v]);
-                    slope[v] = LOGIT ? f[v] * k[v] : 1.f;
+                for (int v = 0; v < V; ++v) g[v] = outside ? 0.f : to_float(d.e[v]);
+                add(g, g, q);
+                if (COUPLED) {
+                    mul(dx, k, g);
+                } else {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) dx[v] = g[v];
                 }
+                mul(dg, g, u[l]);
+                if (!SHARED && LOGIT) mul(dg, slope, dg);
+                mul(n, f, g);
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    const float g = (a.v_h && !outside ? to_float(d.e[v]) : 0.f) + q[v];
-                    dx[v] = outside ? 0.f : COUPLED ? k[v % A] * g : g;
-                    dg[v] = outside ? 0.f : SHARED ? g * u[l][v] : g * u[l][v] * slope[v % A];
+                    dx[v] = outside ? 0.f : dx[v];
+                    dg[v] = outside ? 0.f : dg[v];
                     if (SHARED) sum += dg[v];
-                    q[v] = outside ? q[v] : f[v % A] * g;
+                    q[v] = outside ? q[v] : n[v];
                 }
-                store_floats_if<T, V>(to_x + l * a.h_stride, dx, want_x && (PLAIN || l < left));
+                store_floats_if<T, V>(reinterpret_cast<T*>(row_x), dx, want_x && (PLAIN || l < left));
+                row_x -= a.h_stride;
                 if (s >= 0 && p.active && a.v_state_in) store_floats<float, V>(a.v_state_in + (long long)s * a.channels + p.channel, q);
                 if (!SHARED) {
-                    store_floats_if<T, V>(to_gate + l * a.gate_out_stride, dg, want_gate && (PLAIN || l < left));
+                    store_floats_if<T, V>(reinterpret_cast<T*>(row_gate), dg, want_gate && (PLAIN || l < left));
+                    row_gate -= a.gate_out_stride;
                 } else if (a.v_gate) {
                     sum = p.active ? sum * slope[0] : 0.f;
                     for (int off = (1 << a.lg_tx) >> 1; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
@@ -867,9 +979,11 @@ template <typename T, int V, bool FORWARD, bool LOGIT, bool COUPLED, bool SHARED
 int launch_walk(const RecurrenceLaunch& c, cudaStream_t s) {
     constexpr int L = walk_rows<T>(V);
     constexpr int kTensors = FORWARD ? (SHARED ? 1 : 2) : 1 + (APPLY ? 1 : 0) + (SHARED ? 0 : 1);
-    auto kernel = FORWARD ? recurrence_forward_kernel<T, V, LOGIT, COUPLED, SHARED, APPLY>
-                          : recurrence_backward_kernel<T, V, LOGIT, COUPLED, SHARED, APPLY>;
-    const size_t smem = 2 * sizeof(TileStage<T, V, L, kTensors>) + kTables * 2 * sizeof(int) * c.tile_rows;
+    auto kernel = [] {
+        if constexpr (FORWARD) return recurrence_forward_kernel<T, V, LOGIT, COUPLED, SHARED, APPLY>;
+        else return recurrence_backward_kernel<T, V, LOGIT, COUPLED, SHARED, APPLY>;
+    }();
+    const size_t smem = kStages * sizeof(TileStage<T, V, L, kTensors>) + kTables * 2 * sizeof(int) * c.tile_rows;
     if (smem > 32 * 1024)   // beside the static part
         DSB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     kernel<<<c.blocks, kWalkThreads, smem, s>>>(c.args);
