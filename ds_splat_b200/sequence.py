@@ -22,18 +22,21 @@ device.  There is no fallback for other devices.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 from typing import Optional, Tuple, Union
 
 import torch
+from torch._C import _cuda_getCurrentRawStream as _raw_stream   # the current stream's handle without an object around it
 
 from . import _capi
 
 
-def _on(device):
-    """Context with ``device`` current (the library launches on the current device)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _on(device, call, *args):
+    """``call(*args)`` with ``device`` current (the library launches on the current device)."""
+    if torch.cuda.current_device() == device.index:
+        return call(*args)
+    with torch.cuda.device(device):
+        return call(*args)
 
 
 def _require(t, name, device=None, dtype=None):
@@ -51,16 +54,18 @@ def _rows(t: torch.Tensor, lanes: int):
     """(tensor, elements between rows): ``t`` as rows of its last dimension, as it is where one stride leads from row to row
     and, for loads of ``lanes`` elements, the rows start on such boundaries; a contiguous copy otherwise."""
     width = t.shape[-1]
-    stride, rows = width, 1
-    plain = t.stride(-1) == 1 or width == 1
-    for size, step in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
-        if size == 1:
-            continue
-        if rows == 1:
-            stride = step
-        elif step != stride * rows:
-            plain = False
-        rows *= size
+    if t.is_contiguous():
+        plain, stride = True, width
+    else:
+        plain, stride, rows = t.stride(-1) == 1 or width == 1, width, 1
+        for size, step in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if size == 1:
+                continue
+            if rows == 1:
+                stride = step
+            elif step != stride * rows:
+                plain = False
+            rows *= size
     if plain and (lanes == 1 or (stride % lanes == 0 and t.data_ptr() % (lanes * t.element_size()) == 0)):
         return t, stride
     return t.clone(memory_format=torch.contiguous_format), width
@@ -70,21 +75,9 @@ def _state(t: Optional[torch.Tensor], shape, device, name):
     if t is None:
         return None
     _require(t, name, device, torch.float32)
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have the shape {list(shape)}, got {list(t.shape)}")
     return _rows(t, 4 if shape[-1] % 4 == 0 else 1)[0].contiguous()
-
-
-def _describe(x, gate, sequences, sequence_rows, form, coupled, reverse, offsets, lengths):
-    """The call's DsbRecurrence and the tensors it points into."""
-    d, heads = x.shape[-1], gate.shape[-1]
-    lanes = 4 if (d // heads if heads != d else d) % 4 == 0 else 1
-    x, x_stride = _rows(x, lanes)
-    gate, gate_stride = _rows(gate, lanes if heads == d else 1)
-    shape = _capi.DsbRecurrence(x.numel() // d, sequences, sequence_rows, d, heads, _capi.DTYPES[x.dtype], _capi.GATE_FORMS[form],
-                                1 if coupled else 0, 1 if reverse else 0, x_stride, gate_stride, _capi.ptr(offsets),
-                                _capi.ptr(lengths))
-    return shape, x, gate, lanes
 
 
 def _check_gate(x, gate, form):
@@ -94,65 +87,92 @@ def _check_gate(x, gate, form):
     _require(gate, "gate", x.device, x.dtype)
     if form not in _capi.GATE_FORMS:
         raise ValueError(f"form must be 'decay' or 'logit', got {form!r}")
-    if gate.dim() != x.dim() or gate.shape[:-1] != x.shape[:-1]:
-        raise ValueError(f"gate must have one row per row of x: {list(gate.shape)} against {list(x.shape)}")
-    d, heads = x.shape[-1], gate.shape[-1]
-    if d < 1 or heads < 1 or d % heads != 0:
-        raise ValueError(f"{d} channels do not split into {heads} gate heads")
+    if gate.shape != x.shape:
+        if gate.dim() != x.dim() or gate.shape[:-1] != x.shape[:-1]:
+            raise ValueError(f"gate must have one row per row of x: {list(gate.shape)} against {list(x.shape)}")
+        d, heads = x.shape[-1], gate.shape[-1]
+        if heads < 1 or d % heads != 0:
+            raise ValueError(f"{d} channels do not split into {heads} gate heads")
+    elif x.shape[-1] < 1:
+        raise ValueError("x must have a channel at least")
+
+
+class _Call:
+    """What a call's forward and backward pass have in common: the DsbRecurrence (for ``x`` and ``gate`` as they are kept
+    here, copied where their rows do not lie as the kernels need them) and the sizes that follow from it."""
+    __slots__ = ("shape", "ref", "lanes", "x", "gate", "sequences", "final_only", "workspace_bytes")
+
+    def __init__(self, x, gate, sequences, sequence_rows, form, coupled, reverse, offsets, lengths, final_only=False):
+        d, heads = x.shape[-1], gate.shape[-1]
+        self.lanes = lanes = 4 if (d // heads if heads != d else d) % 4 == 0 else 1
+        self.x, x_stride = _rows(x, lanes)
+        self.gate, gate_stride = _rows(gate, lanes if heads == d else 1)
+        self.sequences, self.final_only = sequences, final_only
+        self.shape = _capi.DsbRecurrence(
+            x.numel() // d, sequences, sequence_rows, d, heads, _capi.DTYPES[x.dtype], _capi.GATE_FORMS[form], 1 if coupled else 0,
+            1 if reverse else 0, x_stride, gate_stride, _capi.ptr(offsets), _capi.ptr(lengths))
+        self.ref = C.byref(self.shape)
+
+    def workspace(self, lib, device):
+        n = self.workspace_bytes
+        return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+    def run(self, state, keep):
+        """(h or None, last, checkpoints or None)"""
+        lib, x = _capi.lib(), self.x
+        dev, d = x.device, x.shape[-1]
+        h = None if self.final_only else torch.empty(x.shape, dtype=x.dtype, device=dev)
+        last = torch.empty((self.sequences, d), dtype=torch.float32, device=dev)
+        checkpoints = None
+        if keep:
+            checkpoints = torch.empty(lib.dsb_recurrence_checkpoint_bytes(self.ref), dtype=torch.uint8, device=dev)
+        self.workspace_bytes = lib.dsb_recurrence_workspace_bytes(self.ref)
+        workspace = self.workspace(lib, dev)
+        rc = lib.dsb_recurrence_forward(
+            self.ref, x.data_ptr(), self.gate.data_ptr(), _capi.ptr(state), _capi.ptr(h), last.data_ptr(), _capi.ptr(checkpoints),
+            _capi.ptr(workspace), self.workspace_bytes, _raw_stream(dev.index))
+        if rc:
+            _capi.check(rc)
+        return h, last, checkpoints
+
+    def run_backward(self, x, gate, state, checkpoints, v_h, v_last, need):
+        lib, dev, d = _capi.lib(), x.device, x.shape[-1]
+        v_h, v_h_stride = _rows(v_h, self.lanes) if v_h is not None else (None, d)
+        v_last = _state(v_last, (self.sequences, d), dev, "the last state's gradient")
+        v_x = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
+        v_gate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if need[1] else None
+        v_state = torch.empty((self.sequences, d), dtype=torch.float32, device=dev) if need[2] else None
+        workspace = self.workspace(lib, dev)
+        rc = lib.dsb_recurrence_backward(
+            self.ref, x.data_ptr(), gate.data_ptr(), _capi.ptr(state), _capi.ptr(checkpoints), _capi.ptr(v_h), v_h_stride,
+            _capi.ptr(v_last), _capi.ptr(v_x), _capi.ptr(v_gate), _capi.ptr(v_state), _capi.ptr(workspace), self.workspace_bytes,
+            _raw_stream(dev.index))
+        if rc:
+            _capi.check(rc)
+        return v_x, v_gate, v_state
 
 
 class _GatedRecurrence(torch.autograd.Function):
+    """Over (x, gate, state) and a ``_Call`` with the offsets or lengths it points at."""
+
     @staticmethod
-    def forward(ctx, x, gate, state, offsets, lengths, form, coupled, reverse, final_only):
-        lib = _capi.lib()
-        dev, lead, d = x.device, x.shape[:-1], x.shape[-1]
-        sequences = offsets.numel() - 1 if offsets is not None else x.shape[0]
-        sequence_rows = 0 if offsets is not None else x.shape[1]
-        state = _state(state, (sequences, d), dev, "state")
-        with _on(dev):
-            shape, x, gate, _ = _describe(x, gate, sequences, sequence_rows, form, coupled, reverse, offsets, lengths)
-            keep = any(ctx.needs_input_grad[:3])
-            h = None if final_only else torch.empty((*lead, d), dtype=x.dtype, device=dev)
-            last = torch.empty((sequences, d), dtype=torch.float32, device=dev)
-            checkpoints = None
-            if keep:
-                checkpoints = torch.empty(int(lib.dsb_recurrence_checkpoint_bytes(C.byref(shape))), dtype=torch.uint8, device=dev)
-            nbytes = int(lib.dsb_recurrence_workspace_bytes(C.byref(shape)))
-            workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-            _capi.check(lib.dsb_recurrence_forward(
-                C.byref(shape), x.data_ptr(), gate.data_ptr(), _capi.ptr(state), _capi.ptr(h), last.data_ptr(),
-                _capi.ptr(checkpoints), _capi.ptr(workspace), nbytes, _capi.stream_ptr()))
-        ctx.call = (sequences, sequence_rows, form, coupled, reverse)
-        if keep:
-            ctx.save_for_backward(x, gate, state, checkpoints, offsets, lengths)
+    def forward(ctx, x, gate, state, call, borders):
+        h, last, checkpoints = _on(x.device, call.run, state, True)
+        ctx.save_for_backward(call.x, call.gate, state, checkpoints, borders)
+        call.x = call.gate = None          # saved above
+        ctx.call = call
         ctx.set_materialize_grads(False)
-        return last if final_only else (h, last)
+        return last if call.final_only else (h, last)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
-        lib = _capi.lib()
-        x, gate, state, checkpoints, offsets, lengths = ctx.saved_tensors
+        x, gate, state, checkpoints, _ = ctx.saved_tensors
         v_h, v_last = (None, grads[0]) if len(grads) == 1 else grads
         if v_h is None and v_last is None:
-            return (None,) * 9
-        sequences, sequence_rows, form, coupled, reverse = ctx.call
-        dev, d = x.device, x.shape[-1]
-        need = ctx.needs_input_grad
-        with _on(dev):
-            shape, x, gate, lanes = _describe(x, gate, sequences, sequence_rows, form, coupled, reverse, offsets, lengths)
-            v_h, v_h_stride = _rows(v_h, lanes) if v_h is not None else (None, d)
-            v_last = _state(v_last, (sequences, d), dev, "the last state's gradient")
-            v_x = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
-            v_gate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if need[1] else None
-            v_state = torch.empty((sequences, d), dtype=torch.float32, device=dev) if need[2] else None
-            nbytes = int(lib.dsb_recurrence_workspace_bytes(C.byref(shape)))
-            workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-            _capi.check(lib.dsb_recurrence_backward(
-                C.byref(shape), x.data_ptr(), gate.data_ptr(), _capi.ptr(state), _capi.ptr(checkpoints), _capi.ptr(v_h), v_h_stride,
-                _capi.ptr(v_last), _capi.ptr(v_x), _capi.ptr(v_gate), _capi.ptr(v_state), _capi.ptr(workspace), nbytes,
-                _capi.stream_ptr()))
-        return v_x, v_gate, v_state, None, None, None, None, None, None
+            return (None,) * 5
+        v = _on(x.device, ctx.call.run_backward, x, gate, state, checkpoints, v_h, v_last, ctx.needs_input_grad)
+        return (*v, None, None)
 
 
 def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, state: Optional[torch.Tensor] = None, *,
@@ -193,8 +213,13 @@ def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, state: Optional[torch.
             if tuple(lengths.shape) != (x.shape[0],):
                 raise ValueError(f"lengths must have one entry per sequence: {list(lengths.shape)} against {x.shape[0]}")
             lengths = lengths.contiguous()
-    out = _GatedRecurrence.apply(x, gate, state, offsets, lengths, form, bool(coupled), bool(reverse), bool(final_only))
-    return (None, out) if final_only else out
+    sequences = x.shape[0] if offsets is None else offsets.numel() - 1
+    state = _state(state, (sequences, x.shape[-1]), x.device, "state")
+    call = _Call(x, gate, sequences, x.shape[1] if offsets is None else 0, form, coupled, reverse, offsets, lengths, final_only)
+    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (state is not None and state.requires_grad)):
+        out = _GatedRecurrence.apply(call.x, call.gate, state, call, offsets if offsets is not None else lengths)
+        return (None, out) if final_only else out
+    return _on(x.device, call.run, state, False)[:2]
 
 
 def gated_recurrence_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, *, form: str = "logit",
@@ -211,13 +236,18 @@ def gated_recurrence_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tens
         raise ValueError("state is updated in place and must be contiguous")
     if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or state.requires_grad):
         raise RuntimeError("gated_recurrence_step has no backward pass: use gated_recurrence, or torch.no_grad()")
-    with _on(x.device):
-        shape, x, gate, _ = _describe(x, gate, x.shape[0], 0, form, coupled, False, None, None)
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        if h.numel():
-            _capi.check(_capi.lib().dsb_recurrence_step(C.byref(shape), x.data_ptr(), gate.data_ptr(), state.data_ptr(),
-                                                        h.data_ptr(), _capi.stream_ptr()))
-            torch.autograd.graph.increment_version(state)
+    return _on(x.device, _run_step, _Call(x, gate, x.shape[0], 0, form, coupled, False, None, None), state)
+
+
+def _run_step(call, state):
+    x = call.x
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if h.numel():
+        rc = _capi.lib().dsb_recurrence_step(call.ref, x.data_ptr(), call.gate.data_ptr(), state.data_ptr(), h.data_ptr(),
+                                             _raw_stream(x.device.index))
+        if rc:
+            _capi.check(rc)
+        torch.autograd.graph.increment_version(state)
     return h
 
 
@@ -232,32 +262,28 @@ def _launch_dropout(x, residual, p, seed, step, rng, rng_used):
         cols = residual_stride = x.shape[-1]
         if residual is not None:
             residual, residual_stride = _rows(residual, 1)
-    _capi.check(_capi.lib().dsb_dropout(
+    rc = _capi.lib().dsb_dropout(
         x.data_ptr(), _capi.ptr(residual), out.data_ptr(), out.numel() // cols, cols, x_stride, residual_stride, cols,
-        _capi.DTYPES[x.dtype], p, seed, step, _capi.ptr(rng), _capi.ptr(rng_used), _capi.stream_ptr()))
+        _capi.DTYPES[x.dtype], p, seed, step, _capi.ptr(rng), _capi.ptr(rng_used), _raw_stream(x.device.index))
+    if rc:
+        _capi.check(rc)
     return out
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, p, seed, step, rng):
-        with _on(x.device):
-            used = torch.empty(2, dtype=torch.int64, device=x.device) if rng is not None else None
-            out = _launch_dropout(x, residual, p, seed, step, rng, used)
-        ctx.call = (p, seed, step)
-        ctx.save_for_backward(used)     # the pair as it was: the caller may advance rng before the backward pass
-        return out
+    def forward(ctx, x, residual, call):
+        p, seed, step, rng = call
+        used = torch.empty(2, dtype=torch.int64, device=x.device) if rng is not None else None
+        ctx.call = (p, seed, step, used)   # the pair as it was: the caller may advance rng before the backward pass
+        return _on(x.device, _launch_dropout, x, residual, p, seed, step, rng, used)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, v_out):
-        used, = ctx.saved_tensors
-        p, seed, step = ctx.call
-        v_x = None
-        if ctx.needs_input_grad[0]:
-            with _on(v_out.device):
-                v_x = _launch_dropout(v_out, None, p, seed, step, used, None)
-        return v_x, (v_out if ctx.needs_input_grad[1] else None), None, None, None, None
+        p, seed, step, used = ctx.call
+        v_x = _on(v_out.device, _launch_dropout, v_out, None, p, seed, step, used, None) if ctx.needs_input_grad[0] else None
+        return v_x, (v_out if ctx.needs_input_grad[1] else None), None
 
 
 def dropout(x: torch.Tensor, p: float, rng: Union[Tuple[int, int], torch.Tensor], *,
@@ -286,8 +312,12 @@ def dropout(x: torch.Tensor, p: float, rng: Union[Tuple[int, int], torch.Tensor]
         _require(rng, "rng", x.device, torch.int64)
         if rng.numel() != 2 or not rng.is_contiguous():
             raise ValueError("rng must hold two elements, (seed, step)")
-        return _Dropout.apply(x, residual, p, 0, 0, rng)
-    seed, step = (int(v) for v in rng)
-    if not (0 <= seed < 1 << 64 and 0 <= step < 1 << 64):
-        raise ValueError("seed and step must lie in [0, 2^64)")
-    return _Dropout.apply(x, residual, p, seed, step, None)
+        seed = step = 0
+    else:
+        seed, step = rng
+        seed, step, rng = int(seed), int(step), None
+        if not (0 <= seed < 1 << 64 and 0 <= step < 1 << 64):
+            raise ValueError("seed and step must lie in [0, 2^64)")
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+        return _Dropout.apply(x, residual, (p, seed, step, rng))
+    return _on(x.device, _launch_dropout, x, residual, p, seed, step, rng, None)
