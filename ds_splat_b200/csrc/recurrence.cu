@@ -74,7 +74,8 @@ recurrence_step_kernel(const T* x, const T* gate, float* state, T* h, const long
 
 struct Layout {            // how a call is cut; the same for the forward and the backward of one shape
     int vec;               // channels per thread: 4 or 1
-    int lg_tx;             // log2 of the threads side by side on one row
+    int tx, groups;        // threads side by side on one row; groups of rows in a tile
+    bool shuffle;
     int per_head;          // channels that share a gate; all of them when every channel has its own
     int heads;             // 1 when every channel has its own gate
     int parts;             // channel blocks per head
@@ -83,7 +84,7 @@ struct Layout {            // how a call is cut; the same for the forward and th
     int64_t chains, chain_rows, tiles;     // tiles of a chain
     int64_t segments, segment_tiles;       // of a chain
 };
-constexpr int kSms = 148, kBlocksPerSm = 3;   // blocks: what the registers allow
+constexpr int kSms = 148, kBlocksPerSm = 2;
 
 int check_shape(const DsbRecurrence& s, bool step) {
     DSB_REQUIRE(s.dtype == DSB_DTYPE_F32 || s.dtype == DSB_DTYPE_F16 || s.dtype == DSB_DTYPE_BF16, "recurrence: unknown dtype %d", s.dtype);
@@ -114,50 +115,66 @@ int shape_vec(const DsbRecurrence& s) {
     return (shared ? s.channels / s.gate_heads : s.channels) % 4 == 0 ? 4 : 1;
 }
 Layout layout_of(const DsbRecurrence& s) {
-    Layout l;
+    Layout l = {};
+    if (s.rows == 0) return l;
     l.vec = shape_vec(s);
     const bool shared = s.gate_heads != s.channels;
     l.heads = shared ? s.gate_heads : 1;
     l.per_head = s.channels / l.heads;
     const int wide = (l.per_head + l.vec - 1) / l.vec;
     const int rows = s.dtype == DSB_DTYPE_F32 ? walk_rows<float>(l.vec) : walk_rows<__half>(l.vec);
-    l.lg_tx = 0;
-    while (l.lg_tx < 5 && (1 << l.lg_tx) < wide) ++l.lg_tx;
-    // How many threads share a row: as many as its channels fill, or fewer (down to a 64-byte piece of a row) where that
-    // spreads the blocks better over the SMs.  An SM holds kBlocksPerSm of them and is kept busy by two.
-    Layout pick = l;
-    int64_t blocks = 0;
-    double best = 0;
-    for (int lg = l.lg_tx, least = lg < 3 ? lg : 3; lg >= least; --lg) {
+    const int piece = l.vec * dtype_bytes(s.dtype);
+    auto fill_in = [&](int tx) {
         Layout c = l;
-        c.lg_tx = lg;
-        c.parts = (wide + (1 << lg) - 1) >> lg;
-        c.tile_rows = kWalkWarps * (32 >> lg) * rows;
+        c.tx = tx;
+        c.shuffle = tx <= 8;
+        c.groups = kWalkThreads / tx;
+        c.parts = (wide + tx - 1) / tx;
+        c.tile_rows = c.groups * rows;
         // A chain per sequence wastes half a tile per sequence on average; a table costs a look at every row.
         c.table = s.sequence_rows == 0 || s.sequence_rows < c.tile_rows;
         c.chains = c.table ? 1 : s.sequences;
-        const int64_t these = c.chains * c.heads * c.parts;
-        const double per_sm = (double)these / kSms;
-        const double rounds = per_sm <= 2 ? 2 : per_sm <= kBlocksPerSm ? std::ceil(per_sm) : std::ceil(per_sm / kBlocksPerSm) * kBlocksPerSm;
-        const double even = per_sm / rounds;     // the share of the time that the average SM works
-        if (lg == l.lg_tx || even > best * 1.05) {
-            best = even;
-            blocks = these;
-            pick = c;
+        c.chain_rows = c.table ? s.rows : s.sequence_rows;
+        c.tiles = (c.chain_rows + c.tile_rows - 1) / c.tile_rows;
+        c.segments = 1;
+        return c;
+    };
+    Layout best = {};
+    if (wide <= 8) {
+        int tx = 1;
+        while (tx < wide) tx *= 2;
+        best = fill_in(tx);
+        const int64_t blocks = best.chains * best.heads;
+        if (2 * blocks < kSms * kBlocksPerSm) best.segments = kSms * kBlocksPerSm / blocks;
+    } else {
+        // The number of threads that share a row, and whether sequences are cut (which reads the inputs twice), by what share
+        // of the threads' time goes into elements: threads without channels, SMs without their two blocks, pieces of a row that
+        // end inside a 32-byte sector, and the composition of a tile's maps (20 instructions an element; 60 and 9 per
+        // group of rows for a thread's part of a tile) all take from it.  A shared gate's sum over its channels takes a
+        // power of two of threads.
+        double most = 0;
+        for (int lanes = 9; lanes <= 64; ++lanes) {
+            const int parts = (wide + lanes - 1) / lanes, tx = shared ? lanes : (wide + parts - 1) / parts;
+            if (tx < 9 || (shared && lanes != 16 && lanes != 32)) continue;
+            Layout c = fill_in(tx);
+            const double elements = 20.0 * rows * l.vec;
+            double share = (double)wide / (c.parts * tx) * (c.groups * tx) / kWalkThreads * elements / (elements + 60 + 9 * c.groups);
+            if (c.parts > 1 && tx * piece % 32 != 0) share *= 0.93;
+            const double per_sm = (double)(c.chains * c.heads * c.parts) / kSms;
+            const double whole = share * (per_sm <= 1 ? 0.65 * per_sm : per_sm / (kBlocksPerSm * std::ceil(per_sm / kBlocksPerSm)));
+            int64_t segments = (int64_t)(kBlocksPerSm / per_sm);
+            if (segments > c.tiles) segments = c.tiles;
+            const double cut = segments > 1 ? share * per_sm * segments / kBlocksPerSm / 1.6 : 0;
+            if (whole > most) { most = whole; best = c; }
+            if (cut > most) { most = cut; best = c; best.segments = segments; }
         }
     }
-    l = pick;
-    l.chain_rows = l.table ? s.rows : s.sequence_rows;
-    l.tiles = (l.chain_rows + l.tile_rows - 1) / l.tile_rows;
-    l.segments = 1;
-    if (best < 0.6 && l.tiles > 1) {   // cut the sequences: the inputs are then read twice
-        l.segments = kSms * kBlocksPerSm / blocks;
-        if (l.segments < 1) l.segments = 1;
-        if (l.segments > l.tiles) l.segments = l.tiles;
+    if (best.segments > best.tiles) best.segments = best.tiles;
+    if (best.tiles > 0) {
+        best.segment_tiles = (best.tiles + best.segments - 1) / best.segments;
+        best.segments = (best.tiles + best.segment_tiles - 1) / best.segment_tiles;   // none of them empty
     }
-    l.segment_tiles = l.tiles ? (l.tiles + l.segments - 1) / l.segments : 0;
-    if (l.tiles) l.segments = (l.tiles + l.segment_tiles - 1) / l.segment_tiles;   // none of them empty
-    return l;
+    return best;
 }
 int64_t up16(int64_t b) { return (b + 15) & ~(int64_t)15; }
 
@@ -189,7 +206,8 @@ int make_cut(const DsbRecurrence& s, bool forward, void* workspace, int64_t work
     a.tiles = (int)l.tiles; a.segments = (int)l.segments; a.segment_tiles = (int)l.segment_tiles;
     a.checkpoints = checkpoints;
     a.sequences = s.sequences; a.sequence_rows = s.sequence_rows; a.channels = s.channels; a.gate_heads = s.gate_heads;
-    a.heads = l.heads; a.per_head = l.per_head; a.parts = l.parts; a.lg_tx = l.lg_tx;
+    a.heads = l.heads; a.per_head = l.per_head; a.parts = l.parts;
+    a.tx = l.tx; a.groups = l.groups; a.shuffle = l.shuffle; a.entries = l.shuffle ? kWalkWarps : l.groups;
     a.logit = s.gate_form == DSB_GATE_LOGIT; a.coupled = s.coupled != 0; a.reverse = s.reverse != 0;
     a.shared = s.gate_heads != s.channels; a.table = l.table;
     a.offsets = s.offsets; a.lengths = s.lengths;
@@ -277,7 +295,7 @@ int64_t recurrence_workspace_bytes(const DsbRecurrence& s) {
 int64_t recurrence_checkpoint_bytes(const DsbRecurrence& s) {
     if (check_shape(s, false) != DSB_OK) return 0;
     const Layout l = layout_of(s);
-    return l.chains * l.tiles * (kWalkWarps * (32 >> l.lg_tx)) * s.channels * 4;
+    return l.chains * l.tiles * l.groups * s.channels * 4;
 }
 
 int launch_recurrence_forward(const DsbRecurrence& shape, const void* x, const void* gate, const float* state_in, void* h,

@@ -21,6 +21,7 @@
 // What bounds it: instruction issue.  A tile without a sequence border ("plain") therefore has code of its own without any
 // test per row, and the form of the gate, the coupling and shared gates are template parameters.
 #pragma once
+#include <atomic>
 #include <type_traits>
 
 #include "vector_io.cuh"
@@ -44,7 +45,9 @@ struct RecurrenceArgs {
     long long h_stride, gate_out_stride;           // contiguous results of channels / heads
     long long x_step, gate_step, v_h_step, h_step, gate_out_step;   // from tile to tile
     int tiles, segments, segment_tiles;
-    int sequences, sequence_rows, channels, gate_heads, heads, per_head, parts, lg_tx;
+    int sequences, sequence_rows, channels, gate_heads, heads, per_head, parts;
+    int tx, groups;        // threads side by side on one row, groups of L rows in a tile
+    int shuffle, entries;  // whether a warp composes its maps by itself, and how many maps a tile leaves in shared memory
     int reverse, table;    // table: one chain over all rows, with sequence borders anywhere; else one chain per sequence
     int logit, coupled, shared;
 };
@@ -56,12 +59,13 @@ struct RecurrenceLaunch {
 template <typename T> int run_recurrence_forward(const RecurrenceLaunch& c, cudaStream_t s);
 template <typename T> int run_recurrence_backward(const RecurrenceLaunch& c, cudaStream_t s);
 
-constexpr int kWalkThreads = 128;
+constexpr int kWalkThreads = 256;
 constexpr int kWalkWarps = kWalkThreads / 32;
+constexpr int kMaxEntries = 32;
 
 // Consecutive rows of a thread: as many as keep the backward's values of a tile in registers and two tiles of every tensor
 // in shared memory with several blocks on an SM.
-template <typename T> __host__ __device__ constexpr int walk_rows(int vec) { return vec == 4 ? (sizeof(T) == 4 ? 4 : 6) : 16; }
+template <typename T> __host__ __device__ constexpr int walk_rows(int vec) { return vec == 4 ? (sizeof(T) == 4 ? 3 : 5) : 16; }
 
 // ---- V channels at a time -------------------------------------------------------------------------------------------
 // Two channels an instruction where the hardware has one; `a` may be a single value for all channels.
@@ -365,83 +369,42 @@ __device__ __forceinline__ void apply_map(float (&h)[V], const Map<V, A>& m) {
     for (int v = 0; v < V; ++v) h[v] = PLAIN || !m.closed ? n[v] : m.b[v];
 }
 
-// The warps' maps of one tile.
+// The maps of one tile in shared memory, in the order of its rows: one per group of rows, or one per warp.
 template <int V, int A>
-struct alignas(16) WarpMaps {     // read and written V (A) floats at a time
-    float b[kWalkWarps][32 * V];
-    float a[kWalkWarps][32 * A];
-    int closed[kWalkWarps];
+struct alignas(16) TileMaps {     // read and written V (A) floats at a time
+    float b[kWalkThreads * V];
+    float a[kWalkThreads * A];
+    int closed[kMaxEntries];
 };
-
-// Lanes that hold the same channels on consecutive row groups are tx apart.  From every thread's own map: the warp's
-// total in shared memory, and the map of the warp's rows before this thread's.  FORWARD: rows run with the lane; else
-// against it.
-template <bool FORWARD, bool PLAIN, int V, int A>
-__device__ __forceinline__ Map<V, A> compose_warp(const Map<V, A>& own, int lg_tx, WarpMaps<V, A>& sh) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tx = 1 << lg_tx;
-    Map<V, A> run = own;
-    auto from = [&](auto value, int off) {
-        return FORWARD ? __shfl_up_sync(0xffffffffu, value, off) : __shfl_down_sync(0xffffffffu, value, off);
-    };
-    for (int off = tx; off < 32; off <<= 1) {
-        Map<V, A> e;
-#pragma unroll
-        for (int v = 0; v < A; ++v) e.a[v] = from(run.a[v], off);
-#pragma unroll
-        for (int v = 0; v < V; ++v) e.b[v] = from(run.b[v], off);
-        e.closed = PLAIN ? 0 : from(run.closed, off);
-        if (FORWARD ? lane >= off : lane + off < 32) compose_after<PLAIN>(run, e);
-    }
-    if (FORWARD ? lane >= 32 - tx : lane < tx) {
-        const int at = lane & (tx - 1);
-        store_floats<float, A>(&sh.a[warp][at * A], run.a);
-        store_floats<float, V>(&sh.b[warp][at * V], run.b);
-        if (!PLAIN && at == 0) sh.closed[warp] = run.closed;
-    }
-    Map<V, A> before;
-    identity(before);
-    if (tx < 32) {
-#pragma unroll
-        for (int v = 0; v < A; ++v) before.a[v] = from(run.a[v], tx);
-#pragma unroll
-        for (int v = 0; v < V; ++v) before.b[v] = from(run.b[v], tx);
-        if (!PLAIN) before.closed = from(run.closed, tx);
-        if (FORWARD ? lane < tx : lane >= 32 - tx) identity(before);
-    }
-    return before;
+template <bool PLAIN, int V, int A>
+__device__ __forceinline__ void put_map(TileMaps<V, A>& sh, int entry, int tx_count, int tx, const Map<V, A>& m) {
+    const int at = entry * tx_count + tx;
+    store_floats<float, A>(&sh.a[at * A], m.a);
+    store_floats<float, V>(&sh.b[at * V], m.b);
+    if (!PLAIN && tx == 0) sh.closed[entry] = m.closed;
 }
 template <bool PLAIN, int V, int A>
-__device__ __forceinline__ Map<V, A> warp_map(const WarpMaps<V, A>& sh, int warp, int tx) {
+__device__ __forceinline__ Map<V, A> get_map(const TileMaps<V, A>& sh, int entry, int tx_count, int tx) {
     Map<V, A> m;
-    const Pack<float, A> pa = load_pack<float, A>(&sh.a[warp][tx * A]);
-    const Pack<float, V> pb = load_pack<float, V>(&sh.b[warp][tx * V]);
+    const int at = entry * tx_count + tx;
+    const Pack<float, A> pa = load_pack<float, A>(&sh.a[at * A]);
+    const Pack<float, V> pb = load_pack<float, V>(&sh.b[at * V]);
 #pragma unroll
     for (int v = 0; v < A; ++v) m.a[v] = pa.e[v];
 #pragma unroll
     for (int v = 0; v < V; ++v) m.b[v] = pb.e[v];
-    m.closed = PLAIN ? 0 : sh.closed[warp];
+    m.closed = PLAIN ? 0 : sh.closed[entry];
     return m;
-}
-// carry: the state before the tile -> the state after it; mine: the state before this thread's warp.
-template <bool FORWARD, bool PLAIN, int V, int A>
-__device__ __forceinline__ void pass_warps(const WarpMaps<V, A>& sh, int tx, float (&carry)[V], float (&mine)[V]) {
-    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);   // the same in the whole warp: no divergence below
-#pragma unroll
-    for (int i = 0; i < kWalkWarps; ++i) {
-        const int w = FORWARD ? i : kWalkWarps - 1 - i;
-        if (w == warp) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) mine[v] = carry[v];
-        }
-        apply_map<PLAIN>(carry, warp_map<PLAIN>(sh, w, tx));
-    }
 }
 
 // ---- a block's place -----------------------------------------------------------------------------------------------------
+// Where many threads share a row, every group of rows leaves its map in shared memory (any number of threads a row, so that
+// the blocks can be made as many as the SMs hold).  Where few do (1, 2, 4 or 8), groups are many: a warp composes its own.
 struct Place {
     int chain, segment, head, part, channel, tx;
     int row0, group;       // this thread's first row inside a tile, and which of the tile's groups of rows that is
-    bool active;           // false beyond the head's last channel
+    int entry;             // whose map in shared memory includes this thread's rows
+    bool there, active;    // there: one of the tile's groups; active: and not beyond the head's last channel
     int read_channel;      // what to read all the same where a thread has no channel
 };
 template <int V, int L>
@@ -454,15 +417,88 @@ __device__ __forceinline__ Place place_of(const RecurrenceArgs& a) {
     p.chain = rest - p.segment * a.chains;
     p.head = block / a.parts;
     p.part = block - p.head * a.parts;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    p.tx = lane & ((1 << a.lg_tx) - 1);
-    p.group = warp * (32 >> a.lg_tx) + (lane >> a.lg_tx);
+    const int tid = threadIdx.x;
+    p.group = tid / a.tx;
+    p.tx = tid - p.group * a.tx;
+    p.there = p.group < a.groups;
+    if (!p.there) p.group = 0;
+    p.entry = a.shuffle ? tid >> 5 : p.group;
     p.row0 = p.group * L;
-    const int c = (p.part << a.lg_tx) * V + p.tx * V;
-    p.active = c < a.per_head;
+    const int c = (p.part * a.tx + p.tx) * V;
+    p.active = p.there && c < a.per_head;
     p.channel = p.head * a.per_head + c;
     p.read_channel = p.active ? p.channel : p.head * a.per_head;
     return p;
+}
+
+// From every thread's own map: the tile's maps in shared memory (to be read after the next barrier), and the map of the rows
+// of its entry before its own.  FORWARD: rows run with the lanes; else against them.
+template <bool FORWARD, bool PLAIN, int V, int A>
+__device__ __forceinline__ Map<V, A> publish_map(const RecurrenceArgs& a, const Place& p, const Map<V, A>& own, TileMaps<V, A>& sh) {
+    Map<V, A> before;
+    identity(before);
+    if (!a.shuffle) {
+        if (p.there) put_map<PLAIN>(sh, p.entry, a.tx, p.tx, own);
+        return before;
+    }
+    const int lane = threadIdx.x & 31, tx = a.tx;
+    Map<V, A> run = own;
+    auto from = [&](auto value, int off) {
+        return FORWARD ? __shfl_up_sync(0xffffffffu, value, off) : __shfl_down_sync(0xffffffffu, value, off);
+    };
+#pragma unroll 1
+    for (int off = tx; off < 32; off <<= 1) {
+        Map<V, A> e;
+#pragma unroll
+        for (int v = 0; v < A; ++v) e.a[v] = from(run.a[v], off);
+#pragma unroll
+        for (int v = 0; v < V; ++v) e.b[v] = from(run.b[v], off);
+        e.closed = PLAIN ? 0 : from(run.closed, off);
+        if (FORWARD ? lane >= off : lane + off < 32) compose_after<PLAIN>(run, e);
+    }
+    if (FORWARD ? lane >= 32 - tx : lane < tx) put_map<PLAIN>(sh, p.entry, tx, p.tx, run);
+#pragma unroll
+    for (int v = 0; v < A; ++v) before.a[v] = from(run.a[v], tx);
+#pragma unroll
+    for (int v = 0; v < V; ++v) before.b[v] = from(run.b[v], tx);
+    if (!PLAIN) before.closed = from(run.closed, tx);
+    if (FORWARD ? lane < tx : lane >= 32 - tx) identity(before);
+    return before;
+}
+// Once a tile's maps are published: the first `tx` threads carry the state through them in their order and leave every entry's
+// starting state in the place of its b.  Nobody else needs the state between tiles.  Two barriers a tile, but the
+// composition costs the block one thread's work per channel instead of every thread's.
+template <bool FORWARD, bool PLAIN, int V, int A>
+__device__ __forceinline__ void pass_entries(const RecurrenceArgs& a, const Place& p, TileMaps<V, A>& sh, float (&carry)[V]) {
+    if (threadIdx.x < a.tx) {
+#pragma unroll 4
+        for (int i = 0; i < a.entries; ++i) {
+            const int w = FORWARD ? i : a.entries - 1 - i;
+            const Map<V, A> m = get_map<PLAIN>(sh, w, a.tx, p.tx);
+            store_floats<float, V>(&sh.b[(w * a.tx + p.tx) * V], carry);
+            apply_map<PLAIN>(carry, m);
+        }
+    }
+    __syncthreads();
+}
+template <int V, int A>
+__device__ __forceinline__ void entry_state(const RecurrenceArgs& a, const Place& p, const TileMaps<V, A>& sh, float (&h)[V]) {
+    const Pack<float, V> q = load_pack<float, V>(&sh.b[(p.entry * a.tx + p.tx) * V]);
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = q.e[v];
+}
+// all: the map of the tiles before (along the scan) -> that of this one as well.
+template <bool FORWARD, bool PLAIN, int V, int A>
+__device__ __forceinline__ void pass_entries(const RecurrenceArgs& a, const Place& p, const TileMaps<V, A>& sh, Map<V, A>& all) {
+    if (threadIdx.x >= a.tx) return;
+    const int closed = all.closed;
+#pragma unroll 2
+    for (int i = 0; i < a.entries; ++i) {
+        Map<V, A> m = get_map<PLAIN>(sh, FORWARD ? i : a.entries - 1 - i, a.tx, p.tx);
+        compose_after<PLAIN>(m, all);
+        all = m;
+    }
+    if (PLAIN) all.closed = closed;
 }
 
 template <int V>
@@ -531,50 +567,42 @@ __device__ __forceinline__ void fetch_shared_gates(T (&own)[L], const char* from
     }
 }
 
-// The state (or q) at the segment's beginning: the maps of the segments before it, each warp a share of them, in order.
+// The state (or q) at the segment's beginning: the maps of the segments before it, each entry a share of them, in order.
 template <bool FORWARD, int V, int A>
-__device__ void carry_of_segment(const RecurrenceArgs& a, const Place& p, WarpMaps<V, A>& sh, float (&carry)[V]) {
+__device__ void carry_of_segment(const RecurrenceArgs& a, const Place& p, TileMaps<V, A>& sh, float (&carry)[V]) {
     const int before = FORWARD ? p.segment : a.segments - 1 - p.segment;
 #pragma unroll
     for (int v = 0; v < V; ++v) carry[v] = 0.f;
     if (before == 0) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int share = (before + kWalkWarps - 1) / kWalkWarps;
-    const int i0 = min(share * warp, before), i1 = min(i0 + share, before);
-    if (lane < (1 << a.lg_tx)) {
+    const int share = (before + a.entries - 1) / a.entries;
+    const int i0 = min(share * p.entry, before), i1 = min(i0 + share, before);
+    if (p.there && (!a.shuffle || (threadIdx.x & 31) < a.tx)) {
         Map<V, A> all;
         identity(all);
 #pragma unroll 4
         for (int i = i0; i < i1; ++i) {
             const long long at = (long long)p.chain * a.segments + (FORWARD ? i : a.segments - 1 - i);
             Map<V, A> m;
-            identity(m);
+            const Pack<float, V> pa = load_pack<float, V>(a.map_a + at * a.channels + p.read_channel);
+            const Pack<float, V> pb = load_pack<float, V>(a.map_b + at * a.channels + p.read_channel);
+#pragma unroll
+            for (int v = 0; v < A; ++v) m.a[v] = pa.e[v];
+#pragma unroll
+            for (int v = 0; v < V; ++v) m.b[v] = pb.e[v];
             m.closed = a.map_closed[at];
-            if (p.active) {
-                const Pack<float, V> pa = load_pack<float, V>(a.map_a + at * a.channels + p.channel);
-                const Pack<float, V> pb = load_pack<float, V>(a.map_b + at * a.channels + p.channel);
-#pragma unroll
-                for (int v = 0; v < A; ++v) m.a[v] = pa.e[v];
-#pragma unroll
-                for (int v = 0; v < V; ++v) m.b[v] = pb.e[v];
-            }
             compose_after<false>(m, all);
             all = m;
         }
-        store_floats<float, A>(&sh.a[warp][p.tx * A], all.a);
-        store_floats<float, V>(&sh.b[warp][p.tx * V], all.b);
-        if (p.tx == 0) sh.closed[warp] = all.closed;
+        put_map<false>(sh, p.entry, a.tx, p.tx, all);
     }
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWalkWarps; ++w) apply_map<false>(carry, warp_map<false>(sh, w, p.tx));
-    __syncthreads();
+    pass_entries<true, false>(a, p, sh, carry);   // only the first threads' carry counts
 }
 
 // Leaves the composition of a whole segment's tiles.
 template <int V, int A>
 __device__ __forceinline__ void store_segment_map(const RecurrenceArgs& a, const Place& p, const Map<V, A>& all) {
-    if (threadIdx.x >= (1 << a.lg_tx) || !p.active) return;
+    if (threadIdx.x >= a.tx || !p.active) return;
     const long long at = (long long)p.chain * a.segments + p.segment;
     float wide[V];
 #pragma unroll
@@ -594,21 +622,21 @@ __device__ __forceinline__ void store_zero_rows(char* to, long long stride, int 
 }
 
 template <typename T, int V, bool LOGIT, bool COUPLED, bool SHARED, bool APPLY>
-__global__ void __launch_bounds__(kWalkThreads)
+__global__ void __launch_bounds__(kWalkThreads, 2)
 recurrence_forward_kernel(const RecurrenceArgs a) {
     constexpr int L = walk_rows<T>(V), A = SHARED ? 1 : V;
     typedef TileStage<T, V, L, SHARED ? 1 : 2> Ring;
     extern __shared__ __align__(16) unsigned char s_raw[];
     Ring* ring = reinterpret_cast<Ring*>(s_raw);
-    __shared__ WarpMaps<V, A> sh[2];
-    const int tile_rows = kWalkWarps * (32 >> a.lg_tx) * L;
+    __shared__ TileMaps<V, A> sh[2];
+    const int tile_rows = a.groups * L;
     const Place p = place_of<V, L>(a);
     const int t0 = p.segment * a.segment_tiles, t1 = min(t0 + a.segment_tiles, a.tiles);
     const char* x = row_pointer<T>(static_cast<const char*>(a.x), p.read_channel, a.x_stride, a, p, t0, tile_rows);
     const char* gate = row_pointer<T>(static_cast<const char*>(a.gate), SHARED ? p.head : p.read_channel, a.gate_stride, a, p, t0, tile_rows);
     const unsigned s_ring = (unsigned)__cvta_generic_to_shared(s_raw) + threadIdx.x * V * sizeof(T);
     constexpr unsigned kTensor = L * kWalkThreads * V * sizeof(T);
-    const int groups = kWalkWarps * (32 >> a.lg_tx);
+    const int groups = a.groups;
     const bool wanted = APPLY && a.h && p.active;
     char* to_h = row_pointer<T>(static_cast<char*>(a.h), p.channel, a.h_stride, a, p, t0, tile_rows);
     const bool keep = APPLY && a.checkpoints && p.active;
@@ -707,22 +735,16 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
                 mul(own.a, f[l], own.a);
                 mul_add(own.b, f[l], own.b, b[l]);
             }
-            const Map<V, A> before = compose_warp<true, PLAIN>(own, a.lg_tx, sh[t & 1]);
+            const Map<V, A> before = publish_map<true, PLAIN>(a, p, own, sh[t & 1]);
             __syncthreads();
             if (!APPLY) {
-#pragma unroll
-                for (int w = 0; w < kWalkWarps; ++w) {
-                    Map<V, A> m = warp_map<PLAIN>(sh[t & 1], w, p.tx);
-                    const int closed = all.closed;
-                    compose_after<PLAIN>(m, all);
-                    if (PLAIN) m.closed = closed;
-                    all = m;
-                }
+                pass_entries<true, PLAIN>(a, p, sh[t & 1], all);
                 return;
             }
             float h[V];
-            pass_warps<true, PLAIN>(sh[t & 1], p.tx, carry, h);
-            apply_map<PLAIN>(h, before);
+            pass_entries<true, PLAIN>(a, p, sh[t & 1], carry);
+            entry_state(a, p, sh[t & 1], h);
+            if (a.shuffle) apply_map<PLAIN>(h, before);
             store_floats_if<float, V>(to_start, h, keep);
             char* to = to_h;
 #pragma unroll
@@ -746,7 +768,7 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
 }
 
 template <typename T, int V, bool LOGIT, bool COUPLED, bool SHARED, bool APPLY>
-__global__ void __launch_bounds__(kWalkThreads)
+__global__ void __launch_bounds__(kWalkThreads, 2)
 recurrence_backward_kernel(const RecurrenceArgs a) {
     constexpr int L = walk_rows<T>(V), A = SHARED ? 1 : V;
     constexpr int kX = 1, kGate = 2;                    // places in a stage; v_h has the first
@@ -754,8 +776,8 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
     constexpr int kGateAt = SHARED ? 0 : APPLY ? kGate : 1, kXAt = APPLY ? kX : 0;
     extern __shared__ __align__(16) unsigned char s_raw[];
     Ring* ring = reinterpret_cast<Ring*>(s_raw);
-    __shared__ WarpMaps<V, A> sh[2];
-    const int tile_rows = kWalkWarps * (32 >> a.lg_tx) * L;
+    __shared__ TileMaps<V, A> sh[2];
+    const int tile_rows = a.groups * L;
     const Place p = place_of<V, L>(a);
     const int t0 = p.segment * a.segment_tiles, t1 = min(t0 + a.segment_tiles, a.tiles);
     const char* vh = row_pointer<T>(static_cast<const char*>(a.v_h), p.read_channel, a.v_h_stride, a, p, t1 - 1, tile_rows);
@@ -763,7 +785,7 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
     const char* gate = row_pointer<T>(static_cast<const char*>(a.gate), SHARED ? p.head : p.read_channel, a.gate_stride, a, p, t1 - 1, tile_rows);
     const unsigned s_ring = (unsigned)__cvta_generic_to_shared(s_raw) + threadIdx.x * V * sizeof(T);
     constexpr unsigned kTensor = L * kWalkThreads * V * sizeof(T);
-    const int groups = kWalkWarps * (32 >> a.lg_tx);
+    const int groups = a.groups;
     const long long row_first = (long long)p.chain * a.chain_rows + (long long)(t1 - 1) * tile_rows + p.row0;
     const bool want_x = APPLY && a.v_x && p.active, want_gate = APPLY && a.v_gate && !SHARED && p.active;
     char* to_x = row_pointer<T>(static_cast<char*>(a.v_x), p.channel, a.h_stride, a, p, t1 - 1, tile_rows);
@@ -844,7 +866,7 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
         if (kind == kEmpty) {
             if (want_x) store_zero_rows<T, V, L>(to_x, a.h_stride, left);
             if (want_gate) store_zero_rows<T, V, L>(to_gate, a.gate_out_stride, left);
-            if (APPLY && SHARED && a.v_gate && p.tx == 0)
+            if (APPLY && SHARED && a.v_gate && p.there && p.tx == 0)
                 for (int l = 0; l < left; ++l) store_gate_sum(l, 0.f);
             __syncthreads();
             continue;
@@ -880,7 +902,7 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                 add(own.b, dv, own.b);
                 mul(own.b, f, own.b);
             }
-            const Map<V, A> after = compose_warp<false, PLAIN>(own, a.lg_tx, sh[t & 1]);
+            const Map<V, A> after = publish_map<false, PLAIN>(a, p, own, sh[t & 1]);
             if (APPLY) {                       // u_t: h_{t-1}, coupled: h_{t-1} - x_t
                 float h[V];
 #pragma unroll
@@ -910,19 +932,13 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
             }
             __syncthreads();
             if (!APPLY) {
-#pragma unroll
-                for (int w = kWalkWarps - 1; w >= 0; --w) {
-                    Map<V, A> n = warp_map<PLAIN>(sh[t & 1], w, p.tx);
-                    const int closed = all.closed;
-                    compose_after<PLAIN>(n, all);
-                    if (PLAIN) n.closed = closed;
-                    all = n;
-                }
+                pass_entries<false, PLAIN>(a, p, sh[t & 1], all);
                 return;
             }
             float q[V];
-            pass_warps<false, PLAIN>(sh[t & 1], p.tx, q_carry, q);
-            apply_map<PLAIN>(q, after);
+            pass_entries<false, PLAIN>(a, p, sh[t & 1], q_carry);
+            entry_state(a, p, sh[t & 1], q);
+            if (a.shuffle) apply_map<PLAIN>(q, after);
             char *row_x = to_x + (L - 1) * a.h_stride, *row_gate = to_gate + (L - 1) * a.gate_out_stride;
 #pragma unroll
             for (int l = L - 1; l >= 0; --l) {
@@ -962,8 +978,8 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                     row_gate -= a.gate_out_stride;
                 } else if (a.v_gate) {
                     sum = p.active ? sum * slope[0] : 0.f;
-                    for (int off = (1 << a.lg_tx) >> 1; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-                    if (p.tx == 0 && (PLAIN || l < left)) store_gate_sum(l, sum);
+                    for (int off = a.tx >> 1; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                    if (p.there && p.tx == 0 && (PLAIN || l < left)) store_gate_sum(l, sum);
                 }
             }
         };
@@ -984,8 +1000,16 @@ int launch_walk(const RecurrenceLaunch& c, cudaStream_t s) {
         else return recurrence_backward_kernel<T, V, LOGIT, COUPLED, SHARED, APPLY>;
     }();
     const size_t smem = kStages * sizeof(TileStage<T, V, L, kTensors>) + kTables * 2 * sizeof(int) * c.tile_rows;
-    if (smem > 32 * 1024)   // beside the static part
-        DSB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (smem > 31 * 1024) {   // 48 KB with the static part: asked for once per device
+        static std::atomic<u64> asked{0};
+        int device = 0;
+        DSB_CUDA_CHECK(cudaGetDevice(&device));
+        const u64 bit = device < 64 ? 1ull << device : 0;
+        if (!bit || !(asked.load(std::memory_order_relaxed) & bit)) {
+            DSB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 208 * 1024));
+            asked.fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
     kernel<<<c.blocks, kWalkThreads, smem, s>>>(c.args);
     DSB_LAUNCH_CHECK();
     return DSB_OK;
