@@ -43,10 +43,24 @@ __device__ __forceinline__ uint4 philox4x32_10(u32 c0, u32 c1, u32 c2, u32 c3, u
     return make_uint4(c0, c1, c2, c3);
 }
 
-// Each thread takes V consecutive elements (V a multiple of 4: whole counter blocks).  VEC: they lie in one row, at
-// addresses that allow one transaction; else every element finds its own row.
-template <typename T, int V, bool VEC>
-__global__ void __launch_bounds__(kThreads)
+template <int V>
+__device__ __forceinline__ void philox_words_at(u64 first_block, u32 step_lo, u32 step_hi, u32 seed_lo, u32 seed_hi, u32 (&word)[V]) {
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) {
+        const u64 block = first_block + q;
+        const uint4 w = philox4x32_10((u32)block, (u32)(block >> 32), step_lo, step_hi, seed_lo, seed_hi);
+        word[4 * q] = w.x; word[4 * q + 1] = w.y; word[4 * q + 2] = w.z; word[4 * q + 3] = w.w;
+    }
+}
+
+// Each thread takes V consecutive elements a trip (V a multiple of 4: whole counter blocks).  VEC: they lie in one row, at
+// addresses that allow one transaction; else every element finds its own row.  The loads of a trip are issued before its
+// random words are worked out.  What bounds it, on 84M elements: with 32-bit tensors memory (77 us with a residual, 59 without,
+// 0.93 of the copy rate each); with 16-bit ones the generator (87 and 85 us, the same with and without the residual's bytes):
+// five 32 x 32 -> 64 bit products an element, which the multiplier takes four cycles each for.  Six blocks an SM (40
+// registers) were the fastest of 4, 6 and 8; one trip per thread instead of a few loses a fifth.
+template <typename T, int V, bool VEC, bool RESIDUAL>
+__global__ void __launch_bounds__(kThreads, 6)
 dropout_kernel(const T* x, const T* residual, T* out, const DropoutArgs a) {
     u32 seed_lo = a.seed_lo, seed_hi = a.seed_hi, step_lo = a.step_lo, step_hi = a.step_hi;
     if (a.rng) {
@@ -54,43 +68,40 @@ dropout_kernel(const T* x, const T* residual, T* out, const DropoutArgs a) {
         seed_lo = (u32)seed; seed_hi = (u32)(seed >> 32); step_lo = (u32)step; step_hi = (u32)(step >> 32);
         if (a.rng_used && blockIdx.x == 0 && threadIdx.x == 0) { a.rng_used[0] = (long long)seed; a.rng_used[1] = (long long)step; }
     }
-    const long long stride = (long long)gridDim.x * kThreads;
+    const u32 threshold = a.threshold;
+    const float scale = a.scale;
+    const long long stride = (long long)gridDim.x * kThreads * V;
     const bool flat = a.x_stride == a.cols && a.residual_stride == a.cols && a.out_stride == a.cols;
-    for (long long g = (long long)blockIdx.x * kThreads + threadIdx.x; g * V < a.count; g += stride) {
-        const long long i = g * V;
-        u32 word[V];
-#pragma unroll
-        for (int q = 0; q < V / 4; ++q) {
-            const u64 block = (u64)(i >> 2) + q;
-            const uint4 w = philox4x32_10((u32)block, (u32)(block >> 32), step_lo, step_hi, seed_lo, seed_hi);
-            word[4 * q] = w.x; word[4 * q + 1] = w.y; word[4 * q + 2] = w.z; word[4 * q + 3] = w.w;
-        }
-        if (VEC && i + V <= a.count) {
+    long long i = ((long long)blockIdx.x * kThreads + threadIdx.x) * V;
+    if (VEC) {
+        for (; i + V <= a.count; i += stride) {
             long long row = 0, col = i;
             if (!flat) { row = i / a.cols; col = i - row * a.cols; }
             const Pack<T, V> xv = load_pack<T, V>(x + row * a.x_stride + col);
             Pack<T, V> rv;
-            if (residual) rv = load_pack<T, V>(residual + row * a.residual_stride + col);
+            if (RESIDUAL) rv = load_pack<T, V>(residual + row * a.residual_stride + col);
+            u32 word[V];
+            philox_words_at<V>((u64)(i >> 2), step_lo, step_hi, seed_lo, seed_hi, word);
             float o[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const bool keep = word[e] >= a.threshold && !a.drop_all;
-                const float r = residual ? to_float(rv.e[e]) : 0.f;
-                o[e] = keep ? (residual ? fmaf(to_float(xv.e[e]), a.scale, r) : to_float(xv.e[e]) * a.scale) : r;
+                const float v = to_float(xv.e[e]), r = RESIDUAL ? to_float(rv.e[e]) : 0.f;
+                o[e] = word[e] >= threshold && !a.drop_all ? (RESIDUAL ? fmaf(v, scale, r) : v * scale) : r;
             }
             store_floats<T, V>(out + row * a.out_stride + col, o);
-        } else {
+        }
+    }
+    for (; i < a.count; i += stride) {
+        u32 word[V];
+        philox_words_at<V>((u64)(i >> 2), step_lo, step_hi, seed_lo, seed_hi, word);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const long long at = i + e;
-                if (at >= a.count) break;
-                const long long row = flat ? 0 : at / a.cols, col = at - row * a.cols;
-                const bool keep = word[e] >= a.threshold && !a.drop_all;
-                const float r = residual ? to_float(residual[row * a.residual_stride + col]) : 0.f;
-                const float v = to_float(x[row * a.x_stride + col]);
-                const float o = keep ? (residual ? fmaf(v, a.scale, r) : v * a.scale) : r;
-                from_float(o, out[row * a.out_stride + col]);
-            }
+        for (int e = 0; e < V; ++e) {
+            const long long at = i + e;
+            if (at >= a.count) break;
+            const long long row = flat ? 0 : at / a.cols, col = at - row * a.cols;
+            const float v = to_float(x[row * a.x_stride + col]), r = RESIDUAL ? to_float(residual[row * a.residual_stride + col]) : 0.f;
+            const float o = word[e] >= threshold && !a.drop_all ? (RESIDUAL ? fmaf(v, scale, r) : v * scale) : r;
+            from_float(o, out[row * a.out_stride + col]);
         }
     }
 }
@@ -127,8 +138,11 @@ int launch_dropout(const void* x, const void* residual, void* out, int64_t rows,
         const T* tx = static_cast<const T*>(x);
         const T* tr = static_cast<const T*>(residual);
         T* to = static_cast<T*>(out);
-        if (vec) dropout_kernel<T, V, true><<<(unsigned)blocks, kThreads, 0, s>>>(tx, tr, to, a);
-        else dropout_kernel<T, V, false><<<(unsigned)blocks, kThreads, 0, s>>>(tx, tr, to, a);
+        auto launch = [&](auto kernel) { kernel<<<(unsigned)blocks, kThreads, 0, s>>>(tx, tr, to, a); };
+        if (vec && tr) launch(dropout_kernel<T, V, true, true>);
+        else if (vec) launch(dropout_kernel<T, V, true, false>);
+        else if (tr) launch(dropout_kernel<T, V, false, true>);
+        else launch(dropout_kernel<T, V, false, false>);
     });
     DSB_LAUNCH_CHECK();
     return DSB_OK;
