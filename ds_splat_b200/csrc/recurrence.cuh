@@ -220,6 +220,9 @@ struct Borders {
     int sequence;          // chain per sequence: its id.  Packed: where to look on, as a sequence of the scan
     int* tables;
     int tile_rows;
+    // Packed: where the sequences around the cursor begin, one per thread, loaded well before they are looked at.  FORWARD:
+    // thread i has that of sequence + i; else of sequence + 1 - i.
+    int window, all_begin, all_end;
 
     __device__ void begin(const RecurrenceArgs& a, int chain, int p0, int* s_tables, int rows) {
         tables = s_tables;
@@ -240,13 +243,18 @@ struct Borders {
             }
             __syncthreads();
             sequence = s_at;
-            look(a);
+            if (sequence >= 0 && sequence < a.sequences) {
+                lo = packed_start(a, sequence);
+                hi = packed_start(a, sequence + 1);
+            }
+            all_begin = packed_start(a, 0);
+            all_end = packed_start(a, a.sequences);
+            load_window(a);
         }
     }
-    __device__ void look(const RecurrenceArgs& a) {   // packed: the bounds of the sequence the cursor stands at
-        const bool any = sequence >= 0 && sequence < a.sequences;
-        lo = any ? packed_start(a, sequence) : 1;
-        hi = any ? packed_start(a, sequence + 1) : 0;
+    __device__ void load_window(const RecurrenceArgs& a) {
+        const int k = FORWARD ? sequence + (int)threadIdx.x : sequence + 1 - (int)threadIdx.x;
+        window = packed_start(a, min(max(k, 0), a.sequences));
     }
     __device__ int* first(int t) const { return tables + t % kTables * 2 * tile_rows; }
     __device__ int* end(int t) const { return first(t) + tile_rows; }
@@ -286,19 +294,20 @@ struct Borders {
             return kBorders;
         }
         const int last = min(p1, a.rows);
-        const int all0 = packed_start(a, 0), all1 = packed_start(a, a.sequences);
         for (int r = tid; r < tile_rows; r += kWalkThreads) {
             const int p = p0 + r;
-            f[r] = p < last && p >= all0 && p < all1 ? kNone : kOutside;
+            f[r] = p < last && p >= all_begin && p < all_end ? kNone : kOutside;
             e[r] = kNone;
         }
-        __syncthreads();
+        __shared__ int s_window[kWalkThreads];
         int done;
         do {   // offsets out of order may lead this astray, but every access stays where it belongs
+            s_window[tid] = window;
+            __syncthreads();
             const int k = FORWARD ? sequence + tid : sequence - tid;
             bool through = false;
-            if (k >= 0 && k < a.sequences) {
-                const int o0 = packed_start(a, k), o1 = packed_start(a, k + 1);
+            if (tid < kWalkThreads - 1 && k >= 0 && k < a.sequences) {
+                const int o0 = FORWARD ? window : s_window[tid + 1], o1 = FORWARD ? s_window[tid + 1] : window;
                 if (o0 < o1) {
                     const int id = sequence_id(a, k);
                     if (o0 >= p0 && o0 < last) f[o0 - p0] = id;
@@ -308,30 +317,44 @@ struct Borders {
             }
             done = __syncthreads_count(through);
             sequence += FORWARD ? done : -done;
-        } while (done == kWalkThreads);
-        look(a);
+            const bool any = done < kWalkThreads - 1 && sequence >= 0 && sequence < a.sequences;
+            const int w0 = any ? s_window[done] : 0, w1 = any ? s_window[done + 1] : 0;
+            lo = any ? (FORWARD ? w0 : w1) : 1;
+            hi = any ? (FORWARD ? w1 : w0) : 0;
+            load_window(a);
+            if (done == kWalkThreads - 1) __syncthreads();   // the window is about to be overwritten
+        } while (done == kWalkThreads - 1);
         return kBorders;
     }
 };
 
-// Sequences without rows hand their state on; offsets and lengths out of order or range are reported.
+// Sequences without rows hand their state on (a warp copies what its lanes have found); offsets and lengths out of order or
+// range are reported.
 __device__ __forceinline__ void pass_empty_sequences(const RecurrenceArgs& a, const float* in, float* out) {
     if (!a.offsets && !a.lengths) return;
+    const int lane = threadIdx.x & 31;
     const long long step = (long long)gridDim.x * kWalkThreads;
-    for (long long s = (long long)blockIdx.x * kWalkThreads + threadIdx.x; s < a.sequences; s += step) {
-        bool empty, bad;
-        if (a.offsets) {
-            const long long o0 = a.offsets[s], o1 = a.offsets[s + 1];
-            empty = o1 <= o0;
-            bad = o1 < o0 || o0 < 0 || o1 > a.rows;
-        } else {
-            const int len = a.lengths[s];
-            empty = len <= 0;
-            bad = len < 0 || len > a.sequence_rows;
+    for (long long s0 = (long long)blockIdx.x * kWalkThreads + (threadIdx.x & ~31); s0 < a.sequences; s0 += step) {
+        const long long s = s0 + lane;
+        bool empty = false, bad = false;
+        if (s < a.sequences) {
+            if (a.offsets) {
+                const long long o0 = a.offsets[s], o1 = a.offsets[s + 1];
+                empty = o1 <= o0;
+                bad = o1 < o0 || o0 < 0 || o1 > a.rows;
+            } else {
+                const int len = a.lengths[s];
+                empty = len <= 0;
+                bad = len < 0 || len > a.sequence_rows;
+            }
         }
         if (bad) atomicMin(a.device_status, DSB_ERR_INVALID_ARGUMENT);
-        if ((empty || bad) && out)
-            for (int c = 0; c < a.channels; ++c) out[s * a.channels + c] = in ? in[s * a.channels + c] : 0.f;
+        unsigned left = __ballot_sync(0xffffffffu, (empty || bad) && out);
+        while (left) {
+            const long long at = (s0 + __ffs(left) - 1) * a.channels;
+            left &= left - 1;
+            for (int c = lane; c < a.channels; c += 32) out[at + c] = in ? in[at + c] : 0.f;
+        }
     }
 }
 
@@ -500,6 +523,34 @@ __device__ __forceinline__ void pass_entries(const RecurrenceArgs& a, const Plac
     }
     if (PLAIN) all.closed = closed;
 }
+
+// States at the borders among a thread's rows, all of them asked for at once: one wait instead of one per border.
+template <bool PLAIN, int V, int L>
+struct BorderStates {
+    float at[L][V];
+    __device__ __forceinline__ BorderStates(const float* states, const int* who, int channels, int channel) {
+#pragma unroll
+        for (int l = 0; l < L; ++l) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) at[l][v] = 0.f;
+            const int s = who[l];
+            if (s >= 0 && states) {
+                const Pack<float, V> q = load_pack<float, V>(states + (long long)s * channels + channel);
+#pragma unroll
+                for (int v = 0; v < V; ++v) at[l][v] = q.e[v];
+            }
+        }
+    }
+    __device__ __forceinline__ void take(int l, float (&h)[V]) const {
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = at[l][v];
+    }
+};
+template <int V, int L>
+struct BorderStates<true, V, L> {     // a plain tile has none
+    __device__ __forceinline__ BorderStates(const float*, const int*, int, int) {}
+    __device__ __forceinline__ void take(int, float (&)[V]) const {}
+};
 
 template <int V>
 __device__ __forceinline__ void load_state(const float* states, long long index, int channels, int channel, float (&o)[V]) {
@@ -702,6 +753,7 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
             float f[L][A], b[L][V];
             Map<V, A> own;
             identity(own);
+            const BorderStates<PLAIN, V, L> begins(p.active ? a.state_in : nullptr, first, a.channels, p.channel);
 #pragma unroll
             for (int l = 0; l < L; ++l) {
                 const int s = PLAIN ? kNone : first[l];
@@ -711,7 +763,7 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
                 if (SHARED) pg.e[0] = gate_now[l];
                 else pg = load_pack<T, A>(&ring[stage].v[SHARED ? 0 : 1][l][threadIdx.x][0]);
                 if (s >= 0) {          // the state before this row is the sequence's own, whatever came before
-                    load_state<V>(p.active ? a.state_in : nullptr, s, a.channels, p.channel, own.b);
+                    begins.take(l, own.b);
                     own.closed = 1;
                 }
                 float e[A], k[A], xv[V];
@@ -747,10 +799,11 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
             if (a.shuffle) apply_map<PLAIN>(h, before);
             store_floats_if<float, V>(to_start, h, keep);
             char* to = to_h;
+            const BorderStates<PLAIN, V, L> again(p.active ? a.state_in : nullptr, first, a.channels, p.channel);
 #pragma unroll
             for (int l = 0; l < L; ++l) {
                 const int s = PLAIN ? kNone : first[l], e = PLAIN ? kNone : end[l];
-                if (s >= 0) load_state<V>(p.active ? a.state_in : nullptr, s, a.channels, p.channel, h);
+                if (s >= 0) again.take(l, h);
                 float o[V];
                 mul_add(h, f[l], h, b[l]);
 #pragma unroll
@@ -877,6 +930,8 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
             float m[L][A], u[L][V];
             Map<V, A> own;
             identity(own);
+            {
+            const BorderStates<PLAIN, V, L> ends(p.active ? a.v_state_out : nullptr, end, a.channels, p.channel);
 #pragma unroll
             for (int l = L - 1; l >= 0; --l) {
                 const bool outside = !PLAIN && first[l] == kOutside;
@@ -886,7 +941,7 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                 else g = load_pack<T, A>(&ring[stage].v[kGateAt][l][threadIdx.x][0]);
                 const Pack<T, V> d = load_pack<T, V>(ring[stage].v[0][l][threadIdx.x]);
                 if (e >= 0) {
-                    load_state<V>(p.active ? a.v_state_out : nullptr, e, a.channels, p.channel, own.b);
+                    ends.take(l, own.b);
                     own.closed = 1;
                 }
                 float f[A], dv[V];
@@ -902,15 +957,17 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                 add(own.b, dv, own.b);
                 mul(own.b, f, own.b);
             }
+            }
             const Map<V, A> after = publish_map<false, PLAIN>(a, p, own, sh[t & 1]);
             if (APPLY) {                       // u_t: h_{t-1}, coupled: h_{t-1} - x_t
                 float h[V];
 #pragma unroll
                 for (int v = 0; v < V; ++v) h[v] = start[v];
+                const BorderStates<PLAIN, V, L> begins(p.active ? a.state_in : nullptr, first, a.channels, p.channel);
 #pragma unroll
                 for (int l = 0; l < L; ++l) {
                     const int s = PLAIN ? kNone : first[l];
-                    if (s >= 0) load_state<V>(p.active ? a.state_in : nullptr, s, a.channels, p.channel, h);
+                    if (s >= 0) begins.take(l, h);
                     const Pack<T, V> xl = load_pack<T, V>(ring[stage].v[kXAt][l][threadIdx.x]);
                     float f[A], k[A], xv[V], n[V];
                     gate_f<LOGIT>(m[l], f);
@@ -940,11 +997,12 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
             entry_state(a, p, sh[t & 1], q);
             if (a.shuffle) apply_map<PLAIN>(q, after);
             char *row_x = to_x + (L - 1) * a.h_stride, *row_gate = to_gate + (L - 1) * a.gate_out_stride;
+            const BorderStates<PLAIN, V, L> again(p.active ? a.v_state_out : nullptr, end, a.channels, p.channel);
 #pragma unroll
             for (int l = L - 1; l >= 0; --l) {
                 const int s = PLAIN ? kNone : first[l], e = PLAIN ? kNone : end[l];
                 const bool outside = s == kOutside;
-                if (e >= 0) load_state<V>(p.active ? a.v_state_out : nullptr, e, a.channels, p.channel, q);
+                if (e >= 0) again.take(l, q);
                 const Pack<T, V> d = load_pack<T, V>(ring[stage].v[0][l][threadIdx.x]);
                 float f[A], k[A], slope[A], dx[V], dg[V], g[V], n[V], sum = 0.f;
                 gate_f<LOGIT>(m[l], f);
