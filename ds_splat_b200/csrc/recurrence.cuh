@@ -182,7 +182,6 @@ __device__ __forceinline__ void gate_k(const float (&e)[A], const float (&f)[A],
 // ---- rows that begin and end sequences ------------------------------------------------------------------------------
 // In the order of the scan: position p is row p, or rows - 1 - p when the scan runs backwards; sequence k of the scan is
 // the tensor's sequence k, or sequences - 1 - k.
-constexpr int kNone = -1, kOutside = -2;
 constexpr int kStages = 2;              // tiles in shared memory: one is worked on, the others are on their way
 constexpr int kTables = kStages + 1;    // border tables: besides, the slowest warp may still read the tile before
 
@@ -211,22 +210,37 @@ __device__ __forceinline__ int starts_up_to(const RecurrenceArgs& a, int shift, 
 
 enum TileKind { kPlain, kBorders, kEmpty };   // no border and every row in a sequence; anything; no row in a sequence
 
-// Follows a walk from tile to tile (FORWARD: upwards): what kind of tile comes, and for tiles with borders the tables
-// first[r] / end[r]: the sequence that begins / ends at the tile's row r, kNone, or (first only) kOutside.  Every member is
-// the same in all threads of the block.
-template <bool FORWARD>
+// The borders of one tile: per group of L rows three bit masks (rows that belong to a sequence, that begin one, that end one),
+// and per row with a border the sequence's id.
+struct BorderTable {
+    unsigned *inside, *first, *end;
+    int *first_id, *end_id;
+    __device__ __forceinline__ BorderTable(int* at, int groups, int tile_rows) {
+        inside = reinterpret_cast<unsigned*>(at);
+        first = inside + groups;
+        end = first + groups;
+        first_id = reinterpret_cast<int*>(end + groups);
+        end_id = first_id + tile_rows;
+    }
+};
+__host__ __device__ constexpr int table_ints(int groups, int rows_per_group) { return groups * (3 + 2 * rows_per_group); }
+
+// Follows a walk from tile to tile (FORWARD: upwards): what kind of tile comes, and the tables of tiles with borders.  Every
+// member but `window` is the same in all threads of the block.
+template <bool FORWARD, int L>
 struct Borders {
     int lo, hi;            // the sequence last met holds positions [lo, hi)
     int sequence;          // chain per sequence: its id.  Packed: where to look on, as a sequence of the scan
     int* tables;
-    int tile_rows;
+    int groups, tile_rows;
     // Packed: where the sequences around the cursor begin, one per thread, loaded well before they are looked at.  FORWARD:
     // thread i has that of sequence + i; else of sequence + 1 - i.
     int window, all_begin, all_end;
 
-    __device__ void begin(const RecurrenceArgs& a, int chain, int p0, int* s_tables, int rows) {
+    __device__ void begin(const RecurrenceArgs& a, int chain, int p0, int* s_tables) {
         tables = s_tables;
-        tile_rows = rows;
+        groups = a.groups;
+        tile_rows = groups * L;
         lo = 1; hi = 0;
         if (!a.table) {
             sequence = sequence_id(a, chain);
@@ -238,7 +252,7 @@ struct Borders {
             // FORWARD: the first sequence to end after p0; else the last to begin before the tile's end
             __shared__ int s_at;
             if (threadIdx.x < 32) {
-                const int n = FORWARD ? starts_up_to(a, 1, p0) : starts_up_to(a, 0, p0 + rows - 1) - 1;
+                const int n = FORWARD ? starts_up_to(a, 1, p0) : starts_up_to(a, 0, p0 + tile_rows - 1) - 1;
                 if (threadIdx.x == 0) s_at = n;
             }
             __syncthreads();
@@ -256,48 +270,57 @@ struct Borders {
         const int k = FORWARD ? sequence + (int)threadIdx.x : sequence + 1 - (int)threadIdx.x;
         window = packed_start(a, min(max(k, 0), a.sequences));
     }
-    __device__ int* first(int t) const { return tables + t % kTables * 2 * tile_rows; }
-    __device__ int* end(int t) const { return first(t) + tile_rows; }
+    __device__ __forceinline__ BorderTable table(int t) const {
+        return BorderTable(tables + t % kTables * table_ints(groups, L), groups, tile_rows);
+    }
+    // The rows of the group at p that lie in [from, to).
+    __device__ __forceinline__ static unsigned mask_of(int p, int from, int to) {
+        const int b = min(max(from - p, 0), L), e = min(max(to - p, 0), L);
+        return b < e ? ((1u << e) - 1u) & ~((1u << b) - 1u) : 0u;
+    }
 
     // Tile t at p0; called by the whole block, tile after tile.  Tables are there after the next barrier.
     __device__ int prepare(const RecurrenceArgs& a, int t, int p0) {
         const int p1 = p0 + tile_rows;
         if (p0 > lo && p1 < hi) return kPlain;
         if (!a.table && (p1 <= lo || p0 >= hi)) return kEmpty;
-        int *f = first(t), *e = end(t);
-        const int tid = threadIdx.x;
+        const BorderTable b = table(t);
+        const int tid = threadIdx.x, p = p0 + tid * L;      // one thread per group
         if (!a.table) {
-            for (int r = tid; r < tile_rows; r += kWalkThreads) {
-                const int p = p0 + r;
-                f[r] = p < lo || p >= hi ? kOutside : p == lo ? sequence : kNone;
-                e[r] = p == hi - 1 && lo < hi ? sequence : kNone;   // a sequence of no rows ends nowhere
+            if (tid < groups) {
+                const int last = lo < hi ? hi - 1 : -1;     // a sequence of no rows ends nowhere
+                b.inside[tid] = mask_of(p, lo, hi);
+                b.first[tid] = lo < hi ? mask_of(p, lo, lo + 1) : 0u;
+                b.end[tid] = mask_of(p, last, last + 1);
+                if (lo >= p && lo < p + L) b.first_id[lo - p0] = sequence;
+                if (last >= p && last < p + L) b.end_id[last - p0] = sequence;
             }
             return kBorders;
         }
         if (a.sequence_rows > 0) {
-            for (int r = tid; r < tile_rows; r += kWalkThreads) {
-                const int p = p0 + r;
-                int b = kOutside, c = kNone;
-                if (p < a.rows) {
-                    const int turn = p / a.sequence_rows, pos = p - turn * a.sequence_rows;
+            if (tid < groups) {
+                unsigned inside = 0, first = 0, end = 0;
+                for (int l = 0; l < L && p + l < a.rows; ++l) {
+                    const int turn = (p + l) / a.sequence_rows, pos = p + l - turn * a.sequence_rows;
                     const int seq = sequence_id(a, turn);
                     const int len = a.lengths ? min(max(a.lengths[seq], 0), a.sequence_rows) : a.sequence_rows;
                     const int at = a.reverse ? a.sequence_rows - len : 0;
-                    if (pos >= at && pos < at + len) {
-                        b = pos == at ? seq : kNone;
-                        c = pos == at + len - 1 ? seq : kNone;
-                    }
+                    if (pos < at || pos >= at + len) continue;
+                    inside |= 1u << l;
+                    if (pos == at) { first |= 1u << l; b.first_id[tid * L + l] = seq; }
+                    if (pos == at + len - 1) { end |= 1u << l; b.end_id[tid * L + l] = seq; }
                 }
-                f[r] = b;
-                e[r] = c;
+                b.inside[tid] = inside;
+                b.first[tid] = first;
+                b.end[tid] = end;
             }
             return kBorders;
         }
         const int last = min(p1, a.rows);
-        for (int r = tid; r < tile_rows; r += kWalkThreads) {
-            const int p = p0 + r;
-            f[r] = p < last && p >= all_begin && p < all_end ? kNone : kOutside;
-            e[r] = kNone;
+        if (tid < groups) {
+            b.inside[tid] = mask_of(p, all_begin, min(all_end, last));
+            b.first[tid] = 0;
+            b.end[tid] = 0;
         }
         __shared__ int s_window[kWalkThreads];
         int done;
@@ -310,8 +333,14 @@ struct Borders {
                 const int o0 = FORWARD ? window : s_window[tid + 1], o1 = FORWARD ? s_window[tid + 1] : window;
                 if (o0 < o1) {
                     const int id = sequence_id(a, k);
-                    if (o0 >= p0 && o0 < last) f[o0 - p0] = id;
-                    if (o1 > p0 && o1 <= last) e[o1 - 1 - p0] = id;
+                    if (o0 >= p0 && o0 < last) {
+                        b.first_id[o0 - p0] = id;
+                        atomicOr(&b.first[(o0 - p0) / L], 1u << ((o0 - p0) % L));
+                    }
+                    if (o1 > p0 && o1 <= last) {
+                        b.end_id[o1 - 1 - p0] = id;
+                        atomicOr(&b.end[(o1 - 1 - p0) / L], 1u << ((o1 - 1 - p0) % L));
+                    }
                 }
                 through = FORWARD ? o1 <= p1 : o0 >= p0;
             }
@@ -524,45 +553,62 @@ __device__ __forceinline__ void pass_entries(const RecurrenceArgs& a, const Plac
     if (PLAIN) all.closed = closed;
 }
 
-// States at the borders among a thread's rows, all of them asked for at once: one wait instead of one per border.
-template <bool PLAIN, int V, int L>
+// The states at the borders among a thread's rows, taken one after the other (FORWARD: upwards).  The next one is asked for
+// when the one before is taken, the first before the thread begins with its rows.
+template <bool FORWARD, int V>
 struct BorderStates {
-    float at[L][V];
-    __device__ __forceinline__ BorderStates(const float* states, const int* who, int channels, int channel) {
+    float next[V];
+    unsigned left;
+    const float* states;
+    const int* ids;
+    int channels, channel;
+    __device__ __forceinline__ BorderStates(const float* s, unsigned mask, const int* who, int count, int at)
+        : left(mask), states(s), ids(who), channels(count), channel(at) {
+        ask();
+    }
+    __device__ __forceinline__ void ask() {
 #pragma unroll
-        for (int l = 0; l < L; ++l) {
+        for (int v = 0; v < V; ++v) next[v] = 0.f;
+        if (left == 0) return;
+        const int l = FORWARD ? __ffs(left) - 1 : 31 - __clz(left);
+        left &= ~(1u << l);
+        if (states) {
+            const Pack<float, V> q = load_pack<float, V>(states + (long long)ids[l] * channels + channel);
 #pragma unroll
-            for (int v = 0; v < V; ++v) at[l][v] = 0.f;
-            const int s = who[l];
-            if (s >= 0 && states) {
-                const Pack<float, V> q = load_pack<float, V>(states + (long long)s * channels + channel);
-#pragma unroll
-                for (int v = 0; v < V; ++v) at[l][v] = q.e[v];
-            }
+            for (int v = 0; v < V; ++v) next[v] = q.e[v];
         }
     }
-    __device__ __forceinline__ void take(int l, float (&h)[V]) const {
+    __device__ __forceinline__ void take(float (&h)[V]) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = at[l][v];
+        for (int v = 0; v < V; ++v) h[v] = next[v];
+        ask();
     }
 };
-template <int V, int L>
-struct BorderStates<true, V, L> {     // a plain tile has none
-    __device__ __forceinline__ BorderStates(const float*, const int*, int, int) {}
-    __device__ __forceinline__ void take(int, float (&)[V]) const {}
-};
-
-template <int V>
-__device__ __forceinline__ void load_state(const float* states, long long index, int channels, int channel, float (&o)[V]) {
-    if (!states) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) o[v] = 0.f;
-        return;
+// What a thread knows of its rows of one tile.
+template <bool PLAIN>
+struct RowBorders {
+    unsigned inside, first, end;
+    const int *first_id, *end_id;
+    __device__ __forceinline__ RowBorders(const BorderTable& t, const Place& p) {
+        inside = t.inside[p.group];
+        first = t.first[p.group];
+        end = t.end[p.group];
+        first_id = t.first_id + p.row0;
+        end_id = t.end_id + p.row0;
     }
-    const Pack<float, V> q = load_pack<float, V>(states + index * channels + channel);
-#pragma unroll
-    for (int v = 0; v < V; ++v) o[v] = q.e[v];
-}
+    __device__ __forceinline__ bool is_outside(int l) const { return !(inside >> l & 1u); }
+    __device__ __forceinline__ bool begins(int l) const { return first >> l & 1u; }
+    __device__ __forceinline__ bool ends(int l) const { return end >> l & 1u; }
+};
+template <>
+struct RowBorders<true> {      // a plain tile: all inside, no borders
+    static constexpr unsigned first = 0, end = 0;
+    const int *first_id = nullptr, *end_id = nullptr;
+    __device__ __forceinline__ RowBorders(const BorderTable&, const Place&) {}
+    __device__ __forceinline__ bool is_outside(int) const { return false; }
+    __device__ __forceinline__ bool begins(int) const { return false; }
+    __device__ __forceinline__ bool ends(int) const { return false; }
+};
 
 // ---- rows on their way through shared memory ---------------------------------------------------------------------------
 template <typename T, int V>
@@ -697,8 +743,8 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
     Map<V, A> all;
     identity(all);
     if (APPLY) carry_of_segment<true>(a, p, sh[0], carry);
-    Borders<true> borders;
-    borders.begin(a, p.chain, t0 * tile_rows, reinterpret_cast<int*>(s_raw + kStages * sizeof(Ring)), tile_rows);
+    Borders<true, L> borders;
+    borders.begin(a, p.chain, t0 * tile_rows, reinterpret_cast<int*>(s_raw + kStages * sizeof(Ring)));
     T gate_now[L], gate_next[L];
     // Fetches tile t, the next of the walk, into the stage `fetched` and moves on; tiles without rows of a sequence are only
     // passed.  Their kinds wait in `kinds`, two bits each, the tile that is worked on lowest.
@@ -749,21 +795,20 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
         }
         auto tile = [&](auto plain) {
             constexpr bool PLAIN = decltype(plain)::value;
-            const int *first = borders.first(t) + p.row0, *end = borders.end(t) + p.row0;
+            const RowBorders<PLAIN> rows(borders.table(t), p);
             float f[L][A], b[L][V];
             Map<V, A> own;
             identity(own);
-            const BorderStates<PLAIN, V, L> begins(p.active ? a.state_in : nullptr, first, a.channels, p.channel);
+            BorderStates<true, V> begins(p.active ? a.state_in : nullptr, rows.first, rows.first_id, a.channels, p.channel);
 #pragma unroll
             for (int l = 0; l < L; ++l) {
-                const int s = PLAIN ? kNone : first[l];
-                const bool outside = s == kOutside;
+                const bool outside = rows.is_outside(l);
                 const Pack<T, V> px = load_pack<T, V>(ring[stage].v[0][l][threadIdx.x]);
                 Pack<T, A> pg;
                 if (SHARED) pg.e[0] = gate_now[l];
                 else pg = load_pack<T, A>(&ring[stage].v[SHARED ? 0 : 1][l][threadIdx.x][0]);
-                if (s >= 0) {          // the state before this row is the sequence's own, whatever came before
-                    begins.take(l, own.b);
+                if (rows.begins(l)) {  // the state before this row is the sequence's own, whatever came before
+                    begins.take(own.b);
                     own.closed = 1;
                 }
                 float e[A], k[A], xv[V];
@@ -799,18 +844,17 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
             if (a.shuffle) apply_map<PLAIN>(h, before);
             store_floats_if<float, V>(to_start, h, keep);
             char* to = to_h;
-            const BorderStates<PLAIN, V, L> again(p.active ? a.state_in : nullptr, first, a.channels, p.channel);
+            BorderStates<true, V> again(p.active ? a.state_in : nullptr, rows.first, rows.first_id, a.channels, p.channel);
 #pragma unroll
             for (int l = 0; l < L; ++l) {
-                const int s = PLAIN ? kNone : first[l], e = PLAIN ? kNone : end[l];
-                if (s >= 0) again.take(l, h);
+                if (rows.begins(l)) again.take(h);
                 float o[V];
                 mul_add(h, f[l], h, b[l]);
 #pragma unroll
-                for (int v = 0; v < V; ++v) o[v] = s == kOutside ? 0.f : h[v];
+                for (int v = 0; v < V; ++v) o[v] = rows.is_outside(l) ? 0.f : h[v];
                 store_floats_if<T, V>(reinterpret_cast<T*>(to), o, wanted && (PLAIN || l < left));
                 to += a.h_stride;
-                if (e >= 0 && p.active) store_floats<float, V>(a.state_out + (long long)e * a.channels + p.channel, h);
+                if (rows.ends(l) && p.active) store_floats<float, V>(a.state_out + (long long)rows.end_id[l] * a.channels + p.channel, h);
             }
         };
         if (kind == kPlain) tile(std::true_type{});
@@ -851,8 +895,8 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
     Map<V, A> all;
     identity(all);
     if (APPLY) carry_of_segment<false>(a, p, sh[0], q_carry);
-    Borders<false> borders;
-    borders.begin(a, p.chain, (t1 - 1) * tile_rows, reinterpret_cast<int*>(s_raw + kStages * sizeof(Ring)), tile_rows);
+    Borders<false, L> borders;
+    borders.begin(a, p.chain, (t1 - 1) * tile_rows, reinterpret_cast<int*>(s_raw + kStages * sizeof(Ring)));
     T gate_now[L], gate_next[L];
     unsigned kinds = 0;    // as in the forward
     int fetched = 0;
@@ -926,22 +970,20 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
         }
         auto tile = [&](auto plain) {
             constexpr bool PLAIN = decltype(plain)::value;
-            const int *first = borders.first(t) + p.row0, *end = borders.end(t) + p.row0;
+            const RowBorders<PLAIN> rows(borders.table(t), p);
             float m[L][A], u[L][V];
             Map<V, A> own;
             identity(own);
-            {
-            const BorderStates<PLAIN, V, L> ends(p.active ? a.v_state_out : nullptr, end, a.channels, p.channel);
+            BorderStates<false, V> ends(p.active ? a.v_state_out : nullptr, rows.end, rows.end_id, a.channels, p.channel);
 #pragma unroll
             for (int l = L - 1; l >= 0; --l) {
-                const bool outside = !PLAIN && first[l] == kOutside;
-                const int e = PLAIN ? kNone : end[l];
+                const bool outside = rows.is_outside(l);
                 Pack<T, A> g;
                 if (SHARED) g.e[0] = gate_now[l];
                 else g = load_pack<T, A>(&ring[stage].v[kGateAt][l][threadIdx.x][0]);
                 const Pack<T, V> d = load_pack<T, V>(ring[stage].v[0][l][threadIdx.x]);
-                if (e >= 0) {
-                    ends.take(l, own.b);
+                if (rows.ends(l)) {
+                    ends.take(own.b);
                     own.closed = 1;
                 }
                 float f[A], dv[V];
@@ -957,17 +999,15 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                 add(own.b, dv, own.b);
                 mul(own.b, f, own.b);
             }
-            }
             const Map<V, A> after = publish_map<false, PLAIN>(a, p, own, sh[t & 1]);
             if (APPLY) {                       // u_t: h_{t-1}, coupled: h_{t-1} - x_t
                 float h[V];
 #pragma unroll
                 for (int v = 0; v < V; ++v) h[v] = start[v];
-                const BorderStates<PLAIN, V, L> begins(p.active ? a.state_in : nullptr, first, a.channels, p.channel);
+                BorderStates<true, V> begins(p.active ? a.state_in : nullptr, rows.first, rows.first_id, a.channels, p.channel);
 #pragma unroll
                 for (int l = 0; l < L; ++l) {
-                    const int s = PLAIN ? kNone : first[l];
-                    if (s >= 0) begins.take(l, h);
+                    if (rows.begins(l)) begins.take(h);
                     const Pack<T, V> xl = load_pack<T, V>(ring[stage].v[kXAt][l][threadIdx.x]);
                     float f[A], k[A], xv[V], n[V];
                     gate_f<LOGIT>(m[l], f);
@@ -984,7 +1024,7 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                     }
                     mul_add(n, f, h, xv);
 #pragma unroll
-                    for (int v = 0; v < V; ++v) h[v] = s == kOutside ? h[v] : n[v];
+                    for (int v = 0; v < V; ++v) h[v] = rows.is_outside(l) ? h[v] : n[v];
                 }
             }
             __syncthreads();
@@ -997,12 +1037,11 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
             entry_state(a, p, sh[t & 1], q);
             if (a.shuffle) apply_map<PLAIN>(q, after);
             char *row_x = to_x + (L - 1) * a.h_stride, *row_gate = to_gate + (L - 1) * a.gate_out_stride;
-            const BorderStates<PLAIN, V, L> again(p.active ? a.v_state_out : nullptr, end, a.channels, p.channel);
+            BorderStates<false, V> again(p.active ? a.v_state_out : nullptr, rows.end, rows.end_id, a.channels, p.channel);
 #pragma unroll
             for (int l = L - 1; l >= 0; --l) {
-                const int s = PLAIN ? kNone : first[l], e = PLAIN ? kNone : end[l];
-                const bool outside = s == kOutside;
-                if (e >= 0) again.take(l, q);
+                const bool outside = rows.is_outside(l);
+                if (rows.ends(l)) again.take(q);
                 const Pack<T, V> d = load_pack<T, V>(ring[stage].v[0][l][threadIdx.x]);
                 float f[A], k[A], slope[A], dx[V], dg[V], g[V], n[V], sum = 0.f;
                 gate_f<LOGIT>(m[l], f);
@@ -1030,7 +1069,8 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                 }
                 store_floats_if<T, V>(reinterpret_cast<T*>(row_x), dx, want_x && (PLAIN || l < left));
                 row_x -= a.h_stride;
-                if (s >= 0 && p.active && a.v_state_in) store_floats<float, V>(a.v_state_in + (long long)s * a.channels + p.channel, q);
+                if (rows.begins(l) && p.active && a.v_state_in)
+                    store_floats<float, V>(a.v_state_in + (long long)rows.first_id[l] * a.channels + p.channel, q);
                 if (!SHARED) {
                     store_floats_if<T, V>(reinterpret_cast<T*>(row_gate), dg, want_gate && (PLAIN || l < left));
                     row_gate -= a.gate_out_stride;
@@ -1057,7 +1097,7 @@ int launch_walk(const RecurrenceLaunch& c, cudaStream_t s) {
         if constexpr (FORWARD) return recurrence_forward_kernel<T, V, LOGIT, COUPLED, SHARED, APPLY>;
         else return recurrence_backward_kernel<T, V, LOGIT, COUPLED, SHARED, APPLY>;
     }();
-    const size_t smem = kStages * sizeof(TileStage<T, V, L, kTensors>) + kTables * 2 * sizeof(int) * c.tile_rows;
+    const size_t smem = kStages * sizeof(TileStage<T, V, L, kTensors>) + kTables * sizeof(int) * table_ints(c.args.groups, L);
     if (smem > 31 * 1024) {   // 48 KB with the static part: asked for once per device
         static std::atomic<u64> asked{0};
         int device = 0;
