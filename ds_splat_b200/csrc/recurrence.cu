@@ -112,6 +112,8 @@ int check_shape(const DsbRecurrence& s, bool step) {
 // The cut depends on the shape alone, never on addresses: the checkpoints of a forward fit every backward of the shape.
 int shape_vec(const DsbRecurrence& s) {
     const bool shared = s.gate_heads != s.channels;
+    // colours: contiguous rows of three 32-bit channels are taken flat
+    if (s.channels == 3 && s.dtype == DSB_DTYPE_F32 && s.x_stride == 3 && (shared || s.gate_stride == 3)) return 3;
     return (shared ? s.channels / s.gate_heads : s.channels) % 4 == 0 ? 4 : 1;
 }
 Layout layout_of(const DsbRecurrence& s) {
@@ -140,7 +142,7 @@ Layout layout_of(const DsbRecurrence& s) {
         return c;
     };
     Layout best = {};
-    if (wide <= 8) {
+    if (wide <= 8) {   // vec 3 among them: one thread per row
         int tx = 1;
         while (tx < wide) tx *= 2;
         best = fill_in(tx);
@@ -333,6 +335,7 @@ int launch_recurrence_backward(const DsbRecurrence& shape, const void* x, const 
     const int elem = dtype_bytes(shape.dtype);
     DSB_TRY(check_inputs(shape, x, gate));
     DSB_TRY(check_alignment(shape, v_h, v_h_stride, elem, wide, "v_h"));
+    DSB_REQUIRE(!v_h || shape_vec(shape) != 3 || v_h_stride == 3, "recurrence: where x's rows of three channels are contiguous, v_h's must be");
     DSB_TRY(check_alignment(shape, v_x, shape.channels, elem, wide, "v_x"));
     DSB_TRY(check_alignment(shape, v_gate, shape.gate_heads, elem, wide && shape.gate_heads == shape.channels, "v_gate"));
     DSB_TRY(check_alignment(shape, state_in, shape.channels, 4, wide, "state_in"));

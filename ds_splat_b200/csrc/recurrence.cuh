@@ -65,7 +65,7 @@ constexpr int kMaxEntries = 32;
 
 // Consecutive rows of a thread: as many as keep the backward's values of a tile in registers and two tiles of every tensor
 // in shared memory with several blocks on an SM.
-template <typename T> __host__ __device__ constexpr int walk_rows(int vec) { return vec == 4 ? (sizeof(T) == 4 ? 3 : 5) : 16; }
+template <typename T> __host__ __device__ constexpr int walk_rows(int vec) { return vec == 4 ? (sizeof(T) == 4 ? 3 : 5) : vec == 3 ? 5 : 16; }
 
 // ---- V channels at a time -------------------------------------------------------------------------------------------
 // Two channels an instruction where the hardware has one; `a` may be a single value for all channels.
@@ -182,8 +182,10 @@ __device__ __forceinline__ void gate_k(const float (&e)[A], const float (&f)[A],
 // ---- rows that begin and end sequences ------------------------------------------------------------------------------
 // In the order of the scan: position p is row p, or rows - 1 - p when the scan runs backwards; sequence k of the scan is
 // the tensor's sequence k, or sequences - 1 - k.
-constexpr int kStages = 2;              // tiles in shared memory: one is worked on, the others are on their way
-constexpr int kTables = kStages + 1;    // border tables: besides, the slowest warp may still read the tile before
+constexpr int kTables = 3;              // border tables: one is read, one is made, and the slowest warp may still read the one before
+// Tiles in shared memory: one is worked on, one is on its way.  Flat tiles, whose rows other threads have copied and other
+// threads write back, need the one before as well.
+__host__ __device__ constexpr int walk_stages(int vec) { return vec == 3 ? 3 : 2; }
 
 __device__ __forceinline__ int sequence_id(const RecurrenceArgs& a, int k) { return a.reverse ? a.sequences - 1 - k : k; }
 // Where the scan's packed sequence k begins (k = sequences: where the last one ends).
@@ -206,6 +208,35 @@ __device__ __forceinline__ int starts_up_to(const RecurrenceArgs& a, int shift, 
         lo += skip;
     }
     return lo;
+}
+
+// The tiles of a segment that its map depends on: those since (FORWARD; else: until) the last sequence to begin there (the first
+// to end).  Called by the whole block; narrows [t0, t1).
+template <bool FORWARD>
+__device__ __forceinline__ void narrow_to_map(const RecurrenceArgs& a, int tile_rows, int& t0, int& t1) {
+    if (!a.table) return;
+    const int last = min(t1 * tile_rows, a.rows) - 1, first = t0 * tile_rows;
+    int at;
+    if (a.sequence_rows > 0) {
+        at = FORWARD ? last / a.sequence_rows * a.sequence_rows : first / a.sequence_rows * a.sequence_rows + (a.sequence_rows - 1);
+    } else {
+        __shared__ int s_found;
+        if (threadIdx.x < 32) {
+            int p;
+            if (FORWARD) {
+                const int n = starts_up_to(a, 0, last);
+                p = n > 0 ? packed_start(a, n - 1) : 0;
+            } else {
+                const int n = starts_up_to(a, 1, first);
+                p = n < a.sequences ? packed_start(a, n + 1) - 1 : a.rows;
+            }
+            if (threadIdx.x == 0) s_found = p;
+        }
+        __syncthreads();
+        at = s_found;
+    }
+    if (FORWARD) t0 = min(max(t0, at / tile_rows), t1 - 1);
+    else t1 = max(min(t1, at / tile_rows + 1), t0 + 1);
 }
 
 enum TileKind { kPlain, kBorders, kEmpty };   // no border and every row in a sequence; anything; no row in a sequence
@@ -709,6 +740,36 @@ __device__ __forceinline__ void store_segment_map(const RecurrenceArgs& a, const
     if (p.tx == 0) a.map_closed[at] = all.closed;
 }
 
+// Flat tiles: three channels, contiguous rows, one thread per row.  Rows of 12 bytes are too narrow to be copied thread by
+// thread (every access would touch 32 sectors), so the block copies a tile as the one piece of memory that it is.
+struct FlatPiece {
+    long long offset;      // of the piece's lowest address, in bytes from the scan's base
+    int rows;
+    __device__ __forceinline__ FlatPiece(const RecurrenceArgs& a, const Place& p, int p0, int tile_rows, long long stride) {
+        rows = min(tile_rows, a.chain_rows - p0);
+        const long long at = (long long)p.chain * a.chain_rows + p0;
+        offset = (a.reverse ? at + rows - 1 : at) * stride;
+    }
+    // Where the scan's row r of the tile lies in the piece.
+    __device__ __forceinline__ int row(const RecurrenceArgs& a, int r) const { return a.reverse ? rows - 1 - r : r; }
+};
+template <int L>
+__device__ __forceinline__ void fetch_flat(unsigned to, const char* base, const FlatPiece& piece) {
+    const float* from = reinterpret_cast<const float*>(base + piece.offset) + threadIdx.x;
+    const int count = piece.rows * 3 - (int)threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < 3 * L; ++i)
+        if (i * kWalkThreads < count) copy_async<float, 1>(to + i * kWalkThreads * 4, from + i * kWalkThreads, true);
+}
+template <int L>
+__device__ __forceinline__ void write_flat(char* base, const FlatPiece& piece, const float* from) {
+    float* to = reinterpret_cast<float*>(base + piece.offset) + threadIdx.x;
+    const int count = piece.rows * 3 - (int)threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < 3 * L; ++i)
+        if (i * kWalkThreads < count) to[i * kWalkThreads] = from ? from[i * kWalkThreads + threadIdx.x] : 0.f;
+}
+
 // A tile of rows that belong to no sequence.
 template <typename T, int V, int L>
 __device__ __forceinline__ void store_zero_rows(char* to, long long stride, int left) {
@@ -721,17 +782,19 @@ __device__ __forceinline__ void store_zero_rows(char* to, long long stride, int 
 template <typename T, int V, bool LOGIT, bool COUPLED, bool SHARED, bool APPLY>
 __global__ void __launch_bounds__(kWalkThreads, 2)
 recurrence_forward_kernel(const RecurrenceArgs a) {
-    constexpr int L = walk_rows<T>(V), A = SHARED ? 1 : V;
+    constexpr int L = walk_rows<T>(V), A = SHARED ? 1 : V, STAGES = walk_stages(V);
+    constexpr bool FLAT = V == 3;
     typedef TileStage<T, V, L, SHARED ? 1 : 2> Ring;
     extern __shared__ __align__(16) unsigned char s_raw[];
     Ring* ring = reinterpret_cast<Ring*>(s_raw);
     __shared__ TileMaps<V, A> sh[2];
     const int tile_rows = a.groups * L;
     const Place p = place_of<V, L>(a);
-    const int t0 = p.segment * a.segment_tiles, t1 = min(t0 + a.segment_tiles, a.tiles);
+    int t0 = p.segment * a.segment_tiles, t1 = min(t0 + a.segment_tiles, a.tiles);
+    if (!APPLY) narrow_to_map<true>(a, tile_rows, t0, t1);
     const char* x = row_pointer<T>(static_cast<const char*>(a.x), p.read_channel, a.x_stride, a, p, t0, tile_rows);
     const char* gate = row_pointer<T>(static_cast<const char*>(a.gate), SHARED ? p.head : p.read_channel, a.gate_stride, a, p, t0, tile_rows);
-    const unsigned s_ring = (unsigned)__cvta_generic_to_shared(s_raw) + threadIdx.x * V * sizeof(T);
+    const unsigned s_ring = (unsigned)__cvta_generic_to_shared(s_raw) + threadIdx.x * (FLAT ? 1 : V) * sizeof(T);
     constexpr unsigned kTensor = L * kWalkThreads * V * sizeof(T);
     const int groups = a.groups;
     const bool wanted = APPLY && a.h && p.active;
@@ -744,55 +807,79 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
     identity(all);
     if (APPLY) carry_of_segment<true>(a, p, sh[0], carry);
     Borders<true, L> borders;
-    borders.begin(a, p.chain, t0 * tile_rows, reinterpret_cast<int*>(s_raw + kStages * sizeof(Ring)));
+    borders.begin(a, p.chain, t0 * tile_rows, reinterpret_cast<int*>(s_raw + STAGES * sizeof(Ring)));
     T gate_now[L], gate_next[L];
     // Fetches tile t, the next of the walk, into the stage `fetched` and moves on; tiles without rows of a sequence are only
-    // passed.  Their kinds wait in `kinds`, two bits each, the tile that is worked on lowest.
-    unsigned kinds = 0;
+    // passed.
     int fetched = 0;
-    auto fetch = [&](int t, int ahead) {
+    auto fetch = [&](int t) {
+        int kind = kEmpty;
         if (t < t1) {
-            const int kind = borders.prepare(a, t, t * tile_rows);
-            kinds |= (unsigned)kind << (2 * ahead);
+            kind = borders.prepare(a, t, t * tile_rows);
             if (kind != kEmpty) {
-                const int rest = a.chain_rows - t * tile_rows;
-                const int left = min(rest - p.row0, L);
-                const unsigned to = s_ring + fetched * sizeof(Ring);
-                fetch_rows<T, V, L>(to, x, a.x_stride, rest >= tile_rows, left, static_cast<const char*>(a.x));
-                if (!SHARED) fetch_rows<T, V, L>(to + kTensor, gate, a.gate_stride, rest >= tile_rows, left, static_cast<const char*>(a.gate));
+                if constexpr (FLAT) {
+                    const FlatPiece piece(a, p, t * tile_rows, tile_rows, a.h_stride);
+                    fetch_flat<L>(s_ring + fetched * sizeof(Ring), static_cast<const char*>(a.x), piece);
+                    if (!SHARED) fetch_flat<L>(s_ring + fetched * sizeof(Ring) + kTensor, static_cast<const char*>(a.gate), piece);
+                } else {
+                    const int rest = a.chain_rows - t * tile_rows;
+                    const int left = min(rest - p.row0, L);
+                    const unsigned to = s_ring + fetched * sizeof(Ring);
+                    fetch_rows<T, V, L>(to, x, a.x_stride, rest >= tile_rows, left, static_cast<const char*>(a.x));
+                    if (!SHARED) fetch_rows<T, V, L>(to + kTensor, gate, a.gate_stride, rest >= tile_rows, left, static_cast<const char*>(a.gate));
+                }
             }
             x += a.x_step;
             if (!SHARED) gate += a.gate_step;
         }
-        fetched = fetched + 1 == kStages ? 0 : fetched + 1;
+        fetched = fetched + 1 == STAGES ? 0 : fetched + 1;
         copies_issued();
+        return kind;
     };
     auto fetch_gates = [&](int t) {
         fetch_shared_gates<T, L>(gate_next, gate, a.gate_stride, t < t1 ? min(a.chain_rows - t * tile_rows - p.row0, L) : 0);
         gate += a.gate_step;
     };
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) fetch(t0 + i, i);
+    int kind = fetch(t0), kind_next = kEmpty, written = -1;   // written: a flat tile whose h waits in shared memory
     if (SHARED) fetch_gates(t0);
+    if (FLAT) copies_landed<0>();
     __syncthreads();
-    int stage = 0;
-    for (int t = t0; t < t1; ++t, kinds >>= 2, stage = stage + 1 == kStages ? 0 : stage + 1, to_h += a.h_step,
+    int stage = 0, stage_written = 0;
+    auto write_back = [&] {
+        if (written >= 0) write_flat<L>(static_cast<char*>(a.h), FlatPiece(a, p, written * tile_rows, tile_rows, a.h_stride), reinterpret_cast<const float*>(&ring[stage_written]));
+        written = -1;
+    };
+    for (int t = t0; t < t1; ++t, kind = kind_next, stage = stage + 1 == STAGES ? 0 : stage + 1, to_h += a.h_step,
              to_start += (long long)groups * a.channels) {
-        const int kind = kinds & 3u;
         const int p0 = t * tile_rows;
         if (SHARED) {
 #pragma unroll
             for (int l = 0; l < L; ++l) gate_now[l] = gate_next[l];
             fetch_gates(t + 1);
         }
-        fetch(t + kStages - 1, kStages - 1);
-        copies_landed<kStages - 1>();
+        kind_next = fetch(t + 1);
+        if (!FLAT) copies_landed<1>();
         const int left = min(a.chain_rows - p0 - p.row0, L);
         if (kind == kEmpty) {
-            if (wanted) store_zero_rows<T, V, L>(to_h, a.h_stride, left);
+            if constexpr (FLAT) {
+                if (APPLY && a.h) write_flat<L>(static_cast<char*>(a.h), FlatPiece(a, p, p0, tile_rows, a.h_stride), nullptr);
+                copies_landed<0>();
+            } else if (wanted) {
+                store_zero_rows<T, V, L>(to_h, a.h_stride, left);
+            }
             __syncthreads();
+            if (FLAT) {
+                write_back();
+                __syncthreads();    // before its stage is filled again
+            }
             continue;
         }
+        const FlatPiece piece(a, p, p0, tile_rows, a.h_stride);
+        // This thread's row l of tensor k; rows of a flat tile past the chain's end give any row's values, masked like others.
+        auto row_at = [&](int k, int l) {
+            if constexpr (FLAT) return &ring[stage].v[0][0][0][0] + k * (L * kWalkThreads * V) + max(piece.row(a, p.row0 + l), 0) * V;
+            else return &ring[stage].v[k][l][threadIdx.x][0];
+        };
         auto tile = [&](auto plain) {
             constexpr bool PLAIN = decltype(plain)::value;
             const RowBorders<PLAIN> rows(borders.table(t), p);
@@ -803,10 +890,10 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
 #pragma unroll
             for (int l = 0; l < L; ++l) {
                 const bool outside = rows.is_outside(l);
-                const Pack<T, V> px = load_pack<T, V>(ring[stage].v[0][l][threadIdx.x]);
+                const Pack<T, V> px = load_pack<T, V>(row_at(0, l));
                 Pack<T, A> pg;
                 if (SHARED) pg.e[0] = gate_now[l];
-                else pg = load_pack<T, A>(&ring[stage].v[SHARED ? 0 : 1][l][threadIdx.x][0]);
+                else pg = load_pack<T, A>(row_at(SHARED ? 0 : 1, l));
                 if (rows.begins(l)) {  // the state before this row is the sequence's own, whatever came before
                     begins.take(own.b);
                     own.closed = 1;
@@ -833,7 +920,9 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
                 mul_add(own.b, f[l], own.b, b[l]);
             }
             const Map<V, A> before = publish_map<true, PLAIN>(a, p, own, sh[t & 1]);
+            if (FLAT) copies_landed<0>();
             __syncthreads();
+            if (FLAT) write_back();
             if (!APPLY) {
                 pass_entries<true, PLAIN>(a, p, sh[t & 1], all);
                 return;
@@ -843,7 +932,7 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
             entry_state(a, p, sh[t & 1], h);
             if (a.shuffle) apply_map<PLAIN>(h, before);
             store_floats_if<float, V>(to_start, h, keep);
-            char* to = to_h;
+            [[maybe_unused]] char* to = to_h;
             BorderStates<true, V> again(p.active ? a.state_in : nullptr, rows.first, rows.first_id, a.channels, p.channel);
 #pragma unroll
             for (int l = 0; l < L; ++l) {
@@ -852,13 +941,25 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
                 mul_add(h, f[l], h, b[l]);
 #pragma unroll
                 for (int v = 0; v < V; ++v) o[v] = rows.is_outside(l) ? 0.f : h[v];
-                store_floats_if<T, V>(reinterpret_cast<T*>(to), o, wanted && (PLAIN || l < left));
-                to += a.h_stride;
+                if constexpr (FLAT) {
+                    store_floats_if<T, V>(row_at(0, l), o, wanted && (PLAIN || l < left));
+                } else {
+                    store_floats_if<T, V>(reinterpret_cast<T*>(to), o, wanted && (PLAIN || l < left));
+                    to += a.h_stride;
+                }
                 if (rows.ends(l) && p.active) store_floats<float, V>(a.state_out + (long long)rows.end_id[l] * a.channels + p.channel, h);
             }
         };
         if (kind == kPlain) tile(std::true_type{});
         else tile(std::false_type{});
+        if (FLAT && APPLY && a.h) {
+            written = t;
+            stage_written = stage;
+        }
+    }
+    if (FLAT) {
+        __syncthreads();
+        write_back();
     }
     if (APPLY) pass_empty_sequences(a, a.state_in, a.state_out);
     else store_segment_map(a, p, all);
@@ -867,7 +968,8 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
 template <typename T, int V, bool LOGIT, bool COUPLED, bool SHARED, bool APPLY>
 __global__ void __launch_bounds__(kWalkThreads, 2)
 recurrence_backward_kernel(const RecurrenceArgs a) {
-    constexpr int L = walk_rows<T>(V), A = SHARED ? 1 : V;
+    constexpr int L = walk_rows<T>(V), A = SHARED ? 1 : V, STAGES = walk_stages(V);
+    constexpr bool FLAT = V == 3;
     constexpr int kX = 1, kGate = 2;                    // places in a stage; v_h has the first
     typedef TileStage<T, V, L, 1 + (APPLY ? 1 : 0) + (SHARED ? 0 : 1)> Ring;
     constexpr int kGateAt = SHARED ? 0 : APPLY ? kGate : 1, kXAt = APPLY ? kX : 0;
@@ -876,11 +978,12 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
     __shared__ TileMaps<V, A> sh[2];
     const int tile_rows = a.groups * L;
     const Place p = place_of<V, L>(a);
-    const int t0 = p.segment * a.segment_tiles, t1 = min(t0 + a.segment_tiles, a.tiles);
+    int t0 = p.segment * a.segment_tiles, t1 = min(t0 + a.segment_tiles, a.tiles);
+    if (!APPLY) narrow_to_map<false>(a, tile_rows, t0, t1);
     const char* vh = row_pointer<T>(static_cast<const char*>(a.v_h), p.read_channel, a.v_h_stride, a, p, t1 - 1, tile_rows);
     const char* x = row_pointer<T>(static_cast<const char*>(a.x), p.read_channel, a.x_stride, a, p, t1 - 1, tile_rows);
     const char* gate = row_pointer<T>(static_cast<const char*>(a.gate), SHARED ? p.head : p.read_channel, a.gate_stride, a, p, t1 - 1, tile_rows);
-    const unsigned s_ring = (unsigned)__cvta_generic_to_shared(s_raw) + threadIdx.x * V * sizeof(T);
+    const unsigned s_ring = (unsigned)__cvta_generic_to_shared(s_raw) + threadIdx.x * (FLAT ? 1 : V) * sizeof(T);
     constexpr unsigned kTensor = L * kWalkThreads * V * sizeof(T);
     const int groups = a.groups;
     const long long row_first = (long long)p.chain * a.chain_rows + (long long)(t1 - 1) * tile_rows + p.row0;
@@ -896,28 +999,35 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
     identity(all);
     if (APPLY) carry_of_segment<false>(a, p, sh[0], q_carry);
     Borders<false, L> borders;
-    borders.begin(a, p.chain, (t1 - 1) * tile_rows, reinterpret_cast<int*>(s_raw + kStages * sizeof(Ring)));
+    borders.begin(a, p.chain, (t1 - 1) * tile_rows, reinterpret_cast<int*>(s_raw + STAGES * sizeof(Ring)));
     T gate_now[L], gate_next[L];
-    unsigned kinds = 0;    // as in the forward
-    int fetched = 0;
-    auto fetch = [&](int t, int ahead) {
+    int fetched = 0;       // as in the forward
+    auto fetch = [&](int t) {
+        int kind = kEmpty;
         if (t >= t0) {
-            const int kind = borders.prepare(a, t, t * tile_rows);
-            kinds |= (unsigned)kind << (2 * ahead);
+            kind = borders.prepare(a, t, t * tile_rows);
             if (kind != kEmpty) {
-                const int rest = a.chain_rows - t * tile_rows;
-                const int left = min(rest - p.row0, L);
-                const unsigned to = s_ring + fetched * sizeof(Ring);
-                if (a.v_h) fetch_rows<T, V, L>(to, vh, a.v_h_stride, rest >= tile_rows, left, static_cast<const char*>(a.v_h));   // else zeros, put there before
-                if (!SHARED) fetch_rows<T, V, L>(to + kGateAt * kTensor, gate, a.gate_stride, rest >= tile_rows, left, static_cast<const char*>(a.gate));
-                if (APPLY) fetch_rows<T, V, L>(to + kXAt * kTensor, x, a.x_stride, rest >= tile_rows, left, static_cast<const char*>(a.x));
+                const unsigned to = s_ring + fetched * sizeof(Ring);   // without v_h: zeros, put there before
+                if constexpr (FLAT) {
+                    const FlatPiece piece(a, p, t * tile_rows, tile_rows, a.h_stride);
+                    if (a.v_h) fetch_flat<L>(to, static_cast<const char*>(a.v_h), piece);
+                    if (!SHARED) fetch_flat<L>(to + kGateAt * kTensor, static_cast<const char*>(a.gate), piece);
+                    if (APPLY) fetch_flat<L>(to + kXAt * kTensor, static_cast<const char*>(a.x), piece);
+                } else {
+                    const int rest = a.chain_rows - t * tile_rows;
+                    const int left = min(rest - p.row0, L);
+                    if (a.v_h) fetch_rows<T, V, L>(to, vh, a.v_h_stride, rest >= tile_rows, left, static_cast<const char*>(a.v_h));
+                    if (!SHARED) fetch_rows<T, V, L>(to + kGateAt * kTensor, gate, a.gate_stride, rest >= tile_rows, left, static_cast<const char*>(a.gate));
+                    if (APPLY) fetch_rows<T, V, L>(to + kXAt * kTensor, x, a.x_stride, rest >= tile_rows, left, static_cast<const char*>(a.x));
+                }
             }
             vh -= a.v_h_step;
             x -= a.x_step;
             if (!SHARED) gate -= a.gate_step;
         }
-        fetched = fetched + 1 == kStages ? 0 : fetched + 1;
+        fetched = fetched + 1 == STAGES ? 0 : fetched + 1;
         copies_issued();
+        return kind;
     };
     // what goes through registers: one tile ahead
     auto fetch_next = [&](int t) {
@@ -934,16 +1044,24 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
     };
     if (!a.v_h) {
 #pragma unroll 1
-        for (int i = 0; i < kStages * L; ++i) memset(ring[i / L].v[0][i % L][threadIdx.x], 0, V * sizeof(T));
+        for (int i = 0; i < STAGES * L; ++i) memset(ring[i / L].v[0][i % L][threadIdx.x], 0, V * sizeof(T));
     }
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) fetch(t1 - 1 - i, i);
+    int kind = fetch(t1 - 1), kind_next = kEmpty, written = -1;   // written: a flat tile whose results wait in shared memory
     fetch_next(t1 - 1);
+    if (FLAT) copies_landed<0>();
     __syncthreads();
-    int stage = 0;
-    for (int t = t1 - 1; t >= t0; --t, kinds >>= 2, stage = stage + 1 == kStages ? 0 : stage + 1, to_x -= a.h_step,
+    int stage = 0, stage_written = 0;
+    auto write_back = [&] {
+        if (written >= 0) {
+            const FlatPiece piece(a, p, written * tile_rows, tile_rows, a.h_stride);
+            const float* from = reinterpret_cast<const float*>(&ring[stage_written]);
+            if (a.v_x) write_flat<L>(static_cast<char*>(a.v_x), piece, from + kXAt * (L * kWalkThreads * V));
+            if (a.v_gate && !SHARED) write_flat<L>(static_cast<char*>(a.v_gate), piece, from + kGateAt * (L * kWalkThreads * V));
+        }
+        written = -1;
+    };
+    for (int t = t1 - 1; t >= t0; --t, kind = kind_next, stage = stage + 1 == STAGES ? 0 : stage + 1, to_x -= a.h_step,
              to_gate -= a.gate_out_step, to_part -= (long long)tile_rows * part_stride) {
-        const int kind = kinds & 3u;
         const int p0 = t * tile_rows;
         if (SHARED) {
 #pragma unroll
@@ -952,8 +1070,8 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
 #pragma unroll
         for (int v = 0; v < V; ++v) start[v] = start_next[v];
         fetch_next(t - 1);
-        fetch(t - kStages + 1, kStages - 1);
-        copies_landed<kStages - 1>();
+        kind_next = fetch(t - 1);
+        if (!FLAT) copies_landed<1>();
         const int left = min(a.chain_rows - p0 - p.row0, L);
         // a shared gate's sum over this block's channels
         auto store_gate_sum = [&](int l, float sum) {
@@ -961,13 +1079,29 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
             else to_part[(long long)l * part_stride] = sum;
         };
         if (kind == kEmpty) {
-            if (want_x) store_zero_rows<T, V, L>(to_x, a.h_stride, left);
-            if (want_gate) store_zero_rows<T, V, L>(to_gate, a.gate_out_stride, left);
+            if constexpr (FLAT) {
+                const FlatPiece piece(a, p, p0, tile_rows, a.h_stride);
+                if (APPLY && a.v_x) write_flat<L>(static_cast<char*>(a.v_x), piece, nullptr);
+                if (APPLY && a.v_gate && !SHARED) write_flat<L>(static_cast<char*>(a.v_gate), piece, nullptr);
+                copies_landed<0>();
+            } else {
+                if (want_x) store_zero_rows<T, V, L>(to_x, a.h_stride, left);
+                if (want_gate) store_zero_rows<T, V, L>(to_gate, a.gate_out_stride, left);
+            }
             if (APPLY && SHARED && a.v_gate && p.there && p.tx == 0)
                 for (int l = 0; l < left; ++l) store_gate_sum(l, 0.f);
             __syncthreads();
+            if (FLAT) {
+                write_back();
+                __syncthreads();    // before its stage is filled again
+            }
             continue;
         }
+        const FlatPiece piece(a, p, p0, tile_rows, a.h_stride);
+        auto row_at = [&](int k, int l) {      // as in the forward
+            if constexpr (FLAT) return &ring[stage].v[0][0][0][0] + k * (L * kWalkThreads * V) + max(piece.row(a, p.row0 + l), 0) * V;
+            else return &ring[stage].v[k][l][threadIdx.x][0];
+        };
         auto tile = [&](auto plain) {
             constexpr bool PLAIN = decltype(plain)::value;
             const RowBorders<PLAIN> rows(borders.table(t), p);
@@ -980,8 +1114,8 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                 const bool outside = rows.is_outside(l);
                 Pack<T, A> g;
                 if (SHARED) g.e[0] = gate_now[l];
-                else g = load_pack<T, A>(&ring[stage].v[kGateAt][l][threadIdx.x][0]);
-                const Pack<T, V> d = load_pack<T, V>(ring[stage].v[0][l][threadIdx.x]);
+                else g = load_pack<T, A>(row_at(kGateAt, l));
+                const Pack<T, V> d = load_pack<T, V>(row_at(0, l));
                 if (rows.ends(l)) {
                     ends.take(own.b);
                     own.closed = 1;
@@ -1008,7 +1142,7 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
 #pragma unroll
                 for (int l = 0; l < L; ++l) {
                     if (rows.begins(l)) begins.take(h);
-                    const Pack<T, V> xl = load_pack<T, V>(ring[stage].v[kXAt][l][threadIdx.x]);
+                    const Pack<T, V> xl = load_pack<T, V>(row_at(kXAt, l));
                     float f[A], k[A], xv[V], n[V];
                     gate_f<LOGIT>(m[l], f);
 #pragma unroll
@@ -1027,7 +1161,9 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                     for (int v = 0; v < V; ++v) h[v] = rows.is_outside(l) ? h[v] : n[v];
                 }
             }
+            if (FLAT) copies_landed<0>();
             __syncthreads();
+            if (FLAT) write_back();
             if (!APPLY) {
                 pass_entries<false, PLAIN>(a, p, sh[t & 1], all);
                 return;
@@ -1036,13 +1172,13 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
             pass_entries<false, PLAIN>(a, p, sh[t & 1], q_carry);
             entry_state(a, p, sh[t & 1], q);
             if (a.shuffle) apply_map<PLAIN>(q, after);
-            char *row_x = to_x + (L - 1) * a.h_stride, *row_gate = to_gate + (L - 1) * a.gate_out_stride;
+            [[maybe_unused]] char *row_x = to_x + (L - 1) * a.h_stride, *row_gate = to_gate + (L - 1) * a.gate_out_stride;
             BorderStates<false, V> again(p.active ? a.v_state_out : nullptr, rows.end, rows.end_id, a.channels, p.channel);
 #pragma unroll
             for (int l = L - 1; l >= 0; --l) {
                 const bool outside = rows.is_outside(l);
                 if (rows.ends(l)) again.take(q);
-                const Pack<T, V> d = load_pack<T, V>(ring[stage].v[0][l][threadIdx.x]);
+                const Pack<T, V> d = load_pack<T, V>(row_at(0, l));
                 float f[A], k[A], slope[A], dx[V], dg[V], g[V], n[V], sum = 0.f;
                 gate_f<LOGIT>(m[l], f);
                 gate_k<LOGIT>(m[l], f, k);
@@ -1067,13 +1203,21 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                     if (SHARED) sum += dg[v];
                     q[v] = outside ? q[v] : n[v];
                 }
-                store_floats_if<T, V>(reinterpret_cast<T*>(row_x), dx, want_x && (PLAIN || l < left));
-                row_x -= a.h_stride;
+                if constexpr (FLAT) {
+                    store_floats_if<T, V>(row_at(kXAt, l), dx, want_x && (PLAIN || l < left));
+                } else {
+                    store_floats_if<T, V>(reinterpret_cast<T*>(row_x), dx, want_x && (PLAIN || l < left));
+                    row_x -= a.h_stride;
+                }
                 if (rows.begins(l) && p.active && a.v_state_in)
                     store_floats<float, V>(a.v_state_in + (long long)rows.first_id[l] * a.channels + p.channel, q);
                 if (!SHARED) {
-                    store_floats_if<T, V>(reinterpret_cast<T*>(row_gate), dg, want_gate && (PLAIN || l < left));
-                    row_gate -= a.gate_out_stride;
+                    if constexpr (FLAT) {
+                        store_floats_if<T, V>(row_at(kGateAt, l), dg, want_gate && (PLAIN || l < left));
+                    } else {
+                        store_floats_if<T, V>(reinterpret_cast<T*>(row_gate), dg, want_gate && (PLAIN || l < left));
+                        row_gate -= a.gate_out_stride;
+                    }
                 } else if (a.v_gate) {
                     sum = p.active ? sum * slope[0] : 0.f;
                     for (int off = a.tx >> 1; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
@@ -1083,6 +1227,14 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
         };
         if (kind == kPlain) tile(std::true_type{});
         else tile(std::false_type{});
+        if (FLAT && APPLY) {
+            written = t;
+            stage_written = stage;
+        }
+    }
+    if (FLAT) {
+        __syncthreads();
+        write_back();
     }
     if (APPLY) pass_empty_sequences(a, a.v_state_out, a.v_state_in);
     else store_segment_map(a, p, all);
@@ -1097,7 +1249,7 @@ int launch_walk(const RecurrenceLaunch& c, cudaStream_t s) {
         if constexpr (FORWARD) return recurrence_forward_kernel<T, V, LOGIT, COUPLED, SHARED, APPLY>;
         else return recurrence_backward_kernel<T, V, LOGIT, COUPLED, SHARED, APPLY>;
     }();
-    const size_t smem = kStages * sizeof(TileStage<T, V, L, kTensors>) + kTables * sizeof(int) * table_ints(c.args.groups, L);
+    const size_t smem = walk_stages(V) * sizeof(TileStage<T, V, L, kTensors>) + kTables * sizeof(int) * table_ints(c.args.groups, L);
     if (smem > 31 * 1024) {   // 48 KB with the static part: asked for once per device
         static std::atomic<u64> asked{0};
         int device = 0;
@@ -1132,6 +1284,8 @@ int run_walk(const RecurrenceLaunch& c, cudaStream_t s) {
 }
 template <typename T, bool FORWARD>
 int run_walk(const RecurrenceLaunch& c, cudaStream_t s) {
+    if constexpr (sizeof(T) == 4)
+        if (c.vec == 3) return run_walk<T, 3, FORWARD>(c, s);
     return c.vec == 4 ? run_walk<T, 4, FORWARD>(c, s) : run_walk<T, 1, FORWARD>(c, s);
 }
 

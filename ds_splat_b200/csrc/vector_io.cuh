@@ -22,20 +22,27 @@ __device__ __forceinline__ void from_float(float v, float& o) { o = v; }
 __device__ __forceinline__ void from_float(float v, __half& o) { o = __float2half_rn(v); }
 __device__ __forceinline__ void from_float(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
 
-template <typename T, int V> struct alignas(V * sizeof(T)) Pack { T e[V]; };
+template <typename T, int V> struct alignas(V == 3 ? sizeof(T) : V * sizeof(T)) Pack { T e[V]; };   // three go one by one
 
 template <typename T, int V>
 __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
+    if constexpr (V == 3) return {{p[0], p[1], p[2]}};
+    else {
     typedef typename RawVec<V * sizeof(T)>::type Raw;
     const Raw raw = *reinterpret_cast<const Raw*>(p);
     Pack<T, V> out;
     static_assert(sizeof(out) == sizeof(raw), "one transaction");
     memcpy(&out, &raw, sizeof(raw));
     return out;
+    }
 }
 
 template <typename T, int V>
 __device__ __forceinline__ void store_floats(T* p, const float (&v)[V]) {
+    if constexpr (V == 3) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) from_float(v[i], p[i]);
+    } else {
     typedef typename RawVec<V * sizeof(T)>::type Raw;
     Pack<T, V> out;
 #pragma unroll
@@ -43,11 +50,16 @@ __device__ __forceinline__ void store_floats(T* p, const float (&v)[V]) {
     Raw raw;
     memcpy(&raw, &out, sizeof(raw));
     *reinterpret_cast<Raw*>(p) = raw;
+    }
 }
 
 // The same under a condition, with only the store itself left out.
 template <typename T, int V>
 __device__ __forceinline__ void store_floats_if(T* p, const float (&v)[V], bool there) {
+    if constexpr (V == 3) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) if (there) from_float(v[i], p[i]);
+    } else {
     typedef typename RawVec<V * sizeof(T)>::type Raw;
     Pack<T, V> out;
 #pragma unroll
@@ -55,6 +67,7 @@ __device__ __forceinline__ void store_floats_if(T* p, const float (&v)[V], bool 
     Raw raw;
     memcpy(&raw, &out, sizeof(raw));
     if (there) *reinterpret_cast<Raw*>(p) = raw;
+    }
 }
 
 // Calls f with a value of the storage type that `dtype` (DSB_DTYPE_*) names; false for an unknown one.

@@ -137,7 +137,12 @@ class _Call:
 
     def run_backward(self, x, gate, state, checkpoints, v_h, v_last, need):
         lib, dev, d = _capi.lib(), x.device, x.shape[-1]
-        v_h, v_h_stride = _rows(v_h, self.lanes) if v_h is not None else (None, d)
+        if v_h is None:
+            v_h_stride = d
+        elif d == 3:
+            v_h, v_h_stride = v_h.contiguous(), d      # rows of three channels are copied as one piece of memory
+        else:
+            v_h, v_h_stride = _rows(v_h, self.lanes)
         v_last = _state(v_last, (self.sequences, d), dev, "the last state's gradient")
         v_x = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
         v_gate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if need[1] else None
