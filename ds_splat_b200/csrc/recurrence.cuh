@@ -65,7 +65,7 @@ constexpr int kMaxEntries = 32;
 
 // Consecutive rows of a thread: as many as keep the backward's values of a tile in registers and two tiles of every tensor
 // in shared memory with several blocks on an SM.
-template <typename T> __host__ __device__ constexpr int walk_rows(int vec) { return vec == 4 ? (sizeof(T) == 4 ? 3 : 5) : vec == 3 ? 5 : 16; }
+template <typename T> __host__ __device__ constexpr int walk_rows(int vec) { return vec == 4 ? (sizeof(T) == 4 ? 3 : 5) : vec == 3 ? 5 : 12; }
 
 // ---- V channels at a time -------------------------------------------------------------------------------------------
 // Two channels an instruction where the hardware has one; `a` may be a single value for all channels.
@@ -267,8 +267,17 @@ struct Borders {
     // Packed: where the sequences around the cursor begin, one per thread, loaded well before they are looked at.  FORWARD:
     // thread i has that of sequence + i; else of sequence + 1 - i.
     int window, all_begin, all_end;
+    int channel, channels; // the block's channels
 
-    __device__ void begin(const RecurrenceArgs& a, int chain, int p0, int* s_tables) {
+    // A border's states are on their way to L2 a tile before they are asked for.
+    __device__ __forceinline__ void warm(const float* states, int id, int all_channels) const {
+        if (!states) return;
+        const char* at = reinterpret_cast<const char*>(states + (long long)id * all_channels + channel);
+        for (int c = 0; c < channels * 4; c += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + c));
+    }
+    __device__ void begin(const RecurrenceArgs& a, int chain, int p0, int* s_tables, int lanes, int head, int part) {
+        channel = head * a.per_head + part * a.tx * lanes;
+        channels = min(a.tx * lanes, a.per_head - part * a.tx * lanes);
         tables = s_tables;
         groups = a.groups;
         tile_rows = groups * L;
@@ -366,10 +375,12 @@ struct Borders {
                     const int id = sequence_id(a, k);
                     if (o0 >= p0 && o0 < last) {
                         b.first_id[o0 - p0] = id;
+                        warm(a.state_in, id, a.channels);
                         atomicOr(&b.first[(o0 - p0) / L], 1u << ((o0 - p0) % L));
                     }
                     if (o1 > p0 && o1 <= last) {
                         b.end_id[o1 - 1 - p0] = id;
+                        if (!FORWARD) warm(a.v_state_out, id, a.channels);
                         atomicOr(&b.end[(o1 - 1 - p0) / L], 1u << ((o1 - 1 - p0) % L));
                     }
                 }
@@ -661,6 +672,9 @@ template <int LEFT>
 __device__ __forceinline__ void copies_landed() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
 // Lanes lie side by side, so that neither the copies nor the reads meet a bank twice.
+template <typename T> __host__ __device__ constexpr unsigned walk_tensor_bytes(int vec) {
+    return walk_rows<T>(vec) * kWalkThreads * vec * sizeof(T);
+}
 template <typename T, int V, int L, int TENSORS>
 struct alignas(16) TileStage {
     T v[TENSORS][L][kWalkThreads][V];
@@ -702,14 +716,29 @@ __device__ void carry_of_segment(const RecurrenceArgs& a, const Place& p, TileMa
 #pragma unroll
     for (int v = 0; v < V; ++v) carry[v] = 0.f;
     if (before == 0) return;
-    const int share = (before + a.entries - 1) / a.entries;
-    const int i0 = min(share * p.entry, before), i1 = min(i0 + share, before);
+    const long long first_map = (long long)p.chain * a.segments;
+    auto map_at = [&](int i) { return first_map + (FORWARD ? i : a.segments - 1 - i); };
+    int from = 0;
+    if (a.table) {         // only what follows the last segment with a border counts
+        __shared__ int s_from;
+        if (threadIdx.x == 0) s_from = 0;
+        __syncthreads();
+        for (int i = before - 1 - (int)threadIdx.x; i >= 0; i -= kWalkThreads)
+            if (a.map_closed[map_at(i)]) {
+                atomicMax(&s_from, i);
+                break;
+            }
+        __syncthreads();
+        from = s_from;
+    }
+    const int share = (before - from + a.entries - 1) / a.entries;
+    const int i0 = min(from + share * p.entry, before), i1 = min(i0 + share, before);
     if (p.there && (!a.shuffle || (threadIdx.x & 31) < a.tx)) {
         Map<V, A> all;
         identity(all);
 #pragma unroll 4
         for (int i = i0; i < i1; ++i) {
-            const long long at = (long long)p.chain * a.segments + (FORWARD ? i : a.segments - 1 - i);
+            const long long at = map_at(i);
             Map<V, A> m;
             const Pack<float, V> pa = load_pack<float, V>(a.map_a + at * a.channels + p.read_channel);
             const Pack<float, V> pb = load_pack<float, V>(a.map_b + at * a.channels + p.read_channel);
@@ -807,7 +836,7 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
     identity(all);
     if (APPLY) carry_of_segment<true>(a, p, sh[0], carry);
     Borders<true, L> borders;
-    borders.begin(a, p.chain, t0 * tile_rows, reinterpret_cast<int*>(s_raw + STAGES * sizeof(Ring)));
+    borders.begin(a, p.chain, t0 * tile_rows, reinterpret_cast<int*>(s_raw + STAGES * sizeof(Ring)), V, p.head, p.part);
     T gate_now[L], gate_next[L];
     // Fetches tile t, the next of the walk, into the stage `fetched` and moves on; tiles without rows of a sequence are only
     // passed.
@@ -887,6 +916,7 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
             Map<V, A> own;
             identity(own);
             BorderStates<true, V> begins(p.active ? a.state_in : nullptr, rows.first, rows.first_id, a.channels, p.channel);
+            BorderStates<true, V> again = begins;       // for the second time through the rows, the first state already there
 #pragma unroll
             for (int l = 0; l < L; ++l) {
                 const bool outside = rows.is_outside(l);
@@ -933,7 +963,6 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
             if (a.shuffle) apply_map<PLAIN>(h, before);
             store_floats_if<float, V>(to_start, h, keep);
             [[maybe_unused]] char* to = to_h;
-            BorderStates<true, V> again(p.active ? a.state_in : nullptr, rows.first, rows.first_id, a.channels, p.channel);
 #pragma unroll
             for (int l = 0; l < L; ++l) {
                 if (rows.begins(l)) again.take(h);
@@ -970,11 +999,12 @@ __global__ void __launch_bounds__(kWalkThreads, 2)
 recurrence_backward_kernel(const RecurrenceArgs a) {
     constexpr int L = walk_rows<T>(V), A = SHARED ? 1 : V, STAGES = walk_stages(V);
     constexpr bool FLAT = V == 3;
-    constexpr int kX = 1, kGate = 2;                    // places in a stage; v_h has the first
-    typedef TileStage<T, V, L, 1 + (APPLY ? 1 : 0) + (SHARED ? 0 : 1)> Ring;
-    constexpr int kGateAt = SHARED ? 0 : APPLY ? kGate : 1, kXAt = APPLY ? kX : 0;
+    // What lies in a stage, in this order; v_h last, as it may be missing: then one tensor of zeros stands for every stage's.
+    constexpr int kXAt = 0, kGateAt = APPLY ? 1 : 0, kVhAt = kGateAt + (SHARED ? 0 : 1);
+    constexpr unsigned kTensor = walk_tensor_bytes<T>(V);
+    const unsigned stage_bytes = (kVhAt + (a.v_h ? 1 : 0)) * kTensor;
     extern __shared__ __align__(16) unsigned char s_raw[];
-    Ring* ring = reinterpret_cast<Ring*>(s_raw);
+    unsigned char* s_zeros = s_raw + STAGES * stage_bytes;
     __shared__ TileMaps<V, A> sh[2];
     const int tile_rows = a.groups * L;
     const Place p = place_of<V, L>(a);
@@ -984,7 +1014,6 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
     const char* x = row_pointer<T>(static_cast<const char*>(a.x), p.read_channel, a.x_stride, a, p, t1 - 1, tile_rows);
     const char* gate = row_pointer<T>(static_cast<const char*>(a.gate), SHARED ? p.head : p.read_channel, a.gate_stride, a, p, t1 - 1, tile_rows);
     const unsigned s_ring = (unsigned)__cvta_generic_to_shared(s_raw) + threadIdx.x * (FLAT ? 1 : V) * sizeof(T);
-    constexpr unsigned kTensor = L * kWalkThreads * V * sizeof(T);
     const int groups = a.groups;
     const long long row_first = (long long)p.chain * a.chain_rows + (long long)(t1 - 1) * tile_rows + p.row0;
     const bool want_x = APPLY && a.v_x && p.active, want_gate = APPLY && a.v_gate && !SHARED && p.active;
@@ -999,7 +1028,7 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
     identity(all);
     if (APPLY) carry_of_segment<false>(a, p, sh[0], q_carry);
     Borders<false, L> borders;
-    borders.begin(a, p.chain, (t1 - 1) * tile_rows, reinterpret_cast<int*>(s_raw + STAGES * sizeof(Ring)));
+    borders.begin(a, p.chain, (t1 - 1) * tile_rows, reinterpret_cast<int*>(s_zeros + (a.v_h ? 0 : kTensor)), V, p.head, p.part);
     T gate_now[L], gate_next[L];
     int fetched = 0;       // as in the forward
     auto fetch = [&](int t) {
@@ -1007,16 +1036,16 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
         if (t >= t0) {
             kind = borders.prepare(a, t, t * tile_rows);
             if (kind != kEmpty) {
-                const unsigned to = s_ring + fetched * sizeof(Ring);   // without v_h: zeros, put there before
+                const unsigned to = s_ring + fetched * stage_bytes;
                 if constexpr (FLAT) {
                     const FlatPiece piece(a, p, t * tile_rows, tile_rows, a.h_stride);
-                    if (a.v_h) fetch_flat<L>(to, static_cast<const char*>(a.v_h), piece);
+                    if (a.v_h) fetch_flat<L>(to + kVhAt * kTensor, static_cast<const char*>(a.v_h), piece);
                     if (!SHARED) fetch_flat<L>(to + kGateAt * kTensor, static_cast<const char*>(a.gate), piece);
                     if (APPLY) fetch_flat<L>(to + kXAt * kTensor, static_cast<const char*>(a.x), piece);
                 } else {
                     const int rest = a.chain_rows - t * tile_rows;
                     const int left = min(rest - p.row0, L);
-                    if (a.v_h) fetch_rows<T, V, L>(to, vh, a.v_h_stride, rest >= tile_rows, left, static_cast<const char*>(a.v_h));
+                    if (a.v_h) fetch_rows<T, V, L>(to + kVhAt * kTensor, vh, a.v_h_stride, rest >= tile_rows, left, static_cast<const char*>(a.v_h));
                     if (!SHARED) fetch_rows<T, V, L>(to + kGateAt * kTensor, gate, a.gate_stride, rest >= tile_rows, left, static_cast<const char*>(a.gate));
                     if (APPLY) fetch_rows<T, V, L>(to + kXAt * kTensor, x, a.x_stride, rest >= tile_rows, left, static_cast<const char*>(a.x));
                 }
@@ -1043,8 +1072,7 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
         }
     };
     if (!a.v_h) {
-#pragma unroll 1
-        for (int i = 0; i < STAGES * L; ++i) memset(ring[i / L].v[0][i % L][threadIdx.x], 0, V * sizeof(T));
+        for (unsigned i = threadIdx.x * 4; i < kTensor; i += kWalkThreads * 4) *reinterpret_cast<unsigned*>(s_zeros + i) = 0;
     }
     int kind = fetch(t1 - 1), kind_next = kEmpty, written = -1;   // written: a flat tile whose results wait in shared memory
     fetch_next(t1 - 1);
@@ -1054,7 +1082,7 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
     auto write_back = [&] {
         if (written >= 0) {
             const FlatPiece piece(a, p, written * tile_rows, tile_rows, a.h_stride);
-            const float* from = reinterpret_cast<const float*>(&ring[stage_written]);
+            const float* from = reinterpret_cast<const float*>(s_raw + stage_written * stage_bytes);
             if (a.v_x) write_flat<L>(static_cast<char*>(a.v_x), piece, from + kXAt * (L * kWalkThreads * V));
             if (a.v_gate && !SHARED) write_flat<L>(static_cast<char*>(a.v_gate), piece, from + kGateAt * (L * kWalkThreads * V));
         }
@@ -1099,8 +1127,8 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
         }
         const FlatPiece piece(a, p, p0, tile_rows, a.h_stride);
         auto row_at = [&](int k, int l) {      // as in the forward
-            if constexpr (FLAT) return &ring[stage].v[0][0][0][0] + k * (L * kWalkThreads * V) + max(piece.row(a, p.row0 + l), 0) * V;
-            else return &ring[stage].v[k][l][threadIdx.x][0];
+            unsigned char* base = k == kVhAt && !a.v_h ? s_zeros : s_raw + stage * stage_bytes + k * kTensor;
+            return reinterpret_cast<T*>(base) + (FLAT ? max(piece.row(a, p.row0 + l), 0) : l * kWalkThreads + (int)threadIdx.x) * V;
         };
         auto tile = [&](auto plain) {
             constexpr bool PLAIN = decltype(plain)::value;
@@ -1115,7 +1143,7 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                 Pack<T, A> g;
                 if (SHARED) g.e[0] = gate_now[l];
                 else g = load_pack<T, A>(row_at(kGateAt, l));
-                const Pack<T, V> d = load_pack<T, V>(row_at(0, l));
+                const Pack<T, V> d = load_pack<T, V>(row_at(kVhAt, l));
                 if (rows.ends(l)) {
                     ends.take(own.b);
                     own.closed = 1;
@@ -1178,7 +1206,7 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
             for (int l = L - 1; l >= 0; --l) {
                 const bool outside = rows.is_outside(l);
                 if (rows.ends(l)) again.take(q);
-                const Pack<T, V> d = load_pack<T, V>(row_at(0, l));
+                const Pack<T, V> d = load_pack<T, V>(row_at(kVhAt, l));
                 float f[A], k[A], slope[A], dx[V], dg[V], g[V], n[V], sum = 0.f;
                 gate_f<LOGIT>(m[l], f);
                 gate_k<LOGIT>(m[l], f, k);
@@ -1244,12 +1272,12 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
 template <typename T, int V, bool FORWARD, bool LOGIT, bool COUPLED, bool SHARED, bool APPLY>
 int launch_walk(const RecurrenceLaunch& c, cudaStream_t s) {
     constexpr int L = walk_rows<T>(V);
-    constexpr int kTensors = FORWARD ? (SHARED ? 1 : 2) : 1 + (APPLY ? 1 : 0) + (SHARED ? 0 : 1);
     auto kernel = [] {
         if constexpr (FORWARD) return recurrence_forward_kernel<T, V, LOGIT, COUPLED, SHARED, APPLY>;
         else return recurrence_backward_kernel<T, V, LOGIT, COUPLED, SHARED, APPLY>;
     }();
-    const size_t smem = walk_stages(V) * sizeof(TileStage<T, V, L, kTensors>) + kTables * sizeof(int) * table_ints(c.args.groups, L);
+    const int tensors = FORWARD ? (SHARED ? 1 : 2) : (APPLY ? 1 : 0) + (SHARED ? 0 : 1) + (c.args.v_h ? 1 : 0);
+    const size_t smem = (walk_stages(V) * tensors + (!FORWARD && !c.args.v_h ? 1 : 0)) * walk_tensor_bytes<T>(V) + kTables * sizeof(int) * table_ints(c.args.groups, L);
     if (smem > 31 * 1024) {   // 48 KB with the static part: asked for once per device
         static std::atomic<u64> asked{0};
         int device = 0;

@@ -97,10 +97,13 @@ def _check_gate(x, gate, form):
         raise ValueError("x must have a channel at least")
 
 
+_sizes = {}     # (workspace, checkpoint) bytes by what they follow from
+
+
 class _Call:
     """What a call's forward and backward pass have in common: the DsbRecurrence (for ``x`` and ``gate`` as they are kept
     here, copied where their rows do not lie as the kernels need them) and the sizes that follow from it."""
-    __slots__ = ("shape", "ref", "lanes", "x", "gate", "sequences", "final_only", "workspace_bytes")
+    __slots__ = ("shape", "ref", "lanes", "x", "gate", "sequences", "final_only", "sizes")
 
     def __init__(self, x, gate, sequences, sequence_rows, form, coupled, reverse, offsets, lengths, final_only=False):
         d, heads = x.shape[-1], gate.shape[-1]
@@ -113,9 +116,16 @@ class _Call:
             1 if reverse else 0, x_stride, gate_stride, _capi.ptr(offsets), _capi.ptr(lengths))
         self.ref = C.byref(self.shape)
 
-    def workspace(self, lib, device):
-        n = self.workspace_bytes
-        return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    def find_sizes(self, lib):
+        s = self.shape
+        key = (s.rows, s.sequences, s.sequence_rows, s.channels, s.gate_heads, s.dtype, s.x_stride, s.gate_stride)
+        got = _sizes.get(key)
+        if got is None:
+            if len(_sizes) > 256:
+                _sizes.clear()
+            got = _sizes[key] = (lib.dsb_recurrence_workspace_bytes(self.ref), lib.dsb_recurrence_checkpoint_bytes(self.ref))
+        self.sizes = got
+        return got
 
     def run(self, state, keep):
         """(h or None, last, checkpoints or None)"""
@@ -123,14 +133,12 @@ class _Call:
         dev, d = x.device, x.shape[-1]
         h = None if self.final_only else torch.empty(x.shape, dtype=x.dtype, device=dev)
         last = torch.empty((self.sequences, d), dtype=torch.float32, device=dev)
-        checkpoints = None
-        if keep:
-            checkpoints = torch.empty(lib.dsb_recurrence_checkpoint_bytes(self.ref), dtype=torch.uint8, device=dev)
-        self.workspace_bytes = lib.dsb_recurrence_workspace_bytes(self.ref)
-        workspace = self.workspace(lib, dev)
+        workspace_bytes, checkpoint_bytes = self.find_sizes(lib)
+        checkpoints = torch.empty(checkpoint_bytes, dtype=torch.uint8, device=dev) if keep else None
+        workspace = torch.empty(workspace_bytes, dtype=torch.uint8, device=dev) if workspace_bytes else None
         rc = lib.dsb_recurrence_forward(
             self.ref, x.data_ptr(), self.gate.data_ptr(), _capi.ptr(state), _capi.ptr(h), last.data_ptr(), _capi.ptr(checkpoints),
-            _capi.ptr(workspace), self.workspace_bytes, _raw_stream(dev.index))
+            _capi.ptr(workspace), workspace_bytes, _raw_stream(dev.index))
         if rc:
             _capi.check(rc)
         return h, last, checkpoints
@@ -147,10 +155,11 @@ class _Call:
         v_x = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
         v_gate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if need[1] else None
         v_state = torch.empty((self.sequences, d), dtype=torch.float32, device=dev) if need[2] else None
-        workspace = self.workspace(lib, dev)
+        workspace_bytes = self.sizes[0]
+        workspace = torch.empty(workspace_bytes, dtype=torch.uint8, device=dev) if workspace_bytes else None
         rc = lib.dsb_recurrence_backward(
             self.ref, x.data_ptr(), gate.data_ptr(), _capi.ptr(state), _capi.ptr(checkpoints), _capi.ptr(v_h), v_h_stride,
-            _capi.ptr(v_last), _capi.ptr(v_x), _capi.ptr(v_gate), _capi.ptr(v_state), _capi.ptr(workspace), self.workspace_bytes,
+            _capi.ptr(v_last), _capi.ptr(v_x), _capi.ptr(v_gate), _capi.ptr(v_state), _capi.ptr(workspace), workspace_bytes,
             _raw_stream(dev.index))
         if rc:
             _capi.check(rc)
