@@ -1247,7 +1247,7 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                         row_gate -= a.gate_out_stride;
                     }
                 } else if (a.v_gate) {
-                    sum = p.active ? sum * slope[0] : 0.f;
+                    sum = p.active && !outside ? sum * slope[0] : 0.f;   // whatever lies in the gates of rows outside
                     for (int off = a.tx >> 1; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
                     if (p.there && p.tx == 0 && (PLAIN || l < left)) store_gate_sum(l, sum);
                 }

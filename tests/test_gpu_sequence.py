@@ -36,7 +36,7 @@ def make(n, d, heads, s, dtype, form, seed):
 
 
 def check(layout, count, rows, d, heads, dtype="fp32", form="logit", coupled=False, reverse=False, final_only=False, state=True,
-          begin=None, seed=1):
+          begin=None, seed=1, outside_gate="inf"):
     """count: rows of every sequence; rows: rows of a dense or padded sequence, or of the packed tensor."""
     s = len(count)
     n = rows if layout == "packed" else rows * s
@@ -55,7 +55,7 @@ def check(layout, count, rows, d, heads, dtype="fp32", form="logit", coupled=Fal
     want = O.recurrence(*(t.double().cpu().numpy() for t in (x, gate)), st.cpu().numpy() if state else np.zeros((s, d)), begin, count,
                         form, coupled, reverse, None if final_only else v_h.double().cpu().numpy(), v_last.cpu().numpy())
     # what lies in rows of no sequence must not matter
-    x[out], gate[out], v_h[out] = float("nan"), float("inf"), float("nan")
+    x[out], gate[out], v_h[out] = float("nan"), float(outside_gate), float("nan")
     lead = (n,) if layout == "packed" else (s, rows)
     x, gate, v_h = (t.view(*lead, -1) for t in (x, gate, v_h))
     leaves = [x.requires_grad_(), gate.requires_grad_()] + ([st.requires_grad_()] if state else [])
@@ -121,6 +121,59 @@ def test_packed_borders(reverse):
     check("packed", [50, 60], 200, 16, 4, begin=[33, 83], reverse=reverse)           # rows before the first sequence
     check("packed", [3], 3000, 64, 64, reverse=reverse)                              # tiles without a sequence
     check("packed", [], 70, 8, 8, reverse=reverse)                                   # rows without a sequence
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("form", ["logit", "decay"])
+def test_nan_gates_in_rows_of_no_sequence(form, reverse):
+    for d, heads in ((12, 12), (12, 3), (7, 1), (3, 1), (3, 3)):
+        check("padded", [0, 5, 90], 90, d, heads, form=form, reverse=reverse, coupled=True, outside_gate="nan")
+        check("packed", [20, 30], 400, d, heads, form=form, reverse=reverse, begin=[40, 60], outside_gate="-inf")
+        check("packed", [20, 30], 400, d, heads, form=form, reverse=reverse, begin=[40, 60], outside_gate="nan")
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+def test_rows_of_three_channels(reverse):
+    """32-bit rows of three channels are copied as one piece of memory: whole and partial tiles of 1280 rows, with and without
+    borders, padding that covers tiles, several tiles per block, and rows that do not lie together."""
+    kw = dict(reverse=reverse, coupled=True, form="decay")
+    for heads in (1, 3):
+        for rows in (1, 5, 1279, 1280, 1281, 4000):
+            check("dense", [rows], rows, 3, heads, **kw)
+        check("padded", [0, 1, 3000, 5000], 5000, 3, heads, **kw)
+        check("packed", [1] * 3000, 3001, 3, heads, **kw)
+        check("packed", [700, 0, 4000, 0, 0, 3, 1280, 1], 6500, 3, heads, final_only=True, **kw)
+        check("packed", [300] * 9, 2800, 3, heads, state=False, **kw)
+    wide = torch.randn(2, 2000, 8, device="cuda")
+    gate = torch.rand(2, 2000, 1, device="cuda")
+    a = ds.gated_recurrence(wide[..., 1:4], gate, reverse=reverse, form="decay")
+    b = ds.gated_recurrence(wide[..., 1:4].contiguous(), gate, reverse=reverse, form="decay")
+    for p, q in zip(a, b):      # two ways through the rows: sums of a few units, rounded in another order
+        torch.testing.assert_close(p, q, rtol=1e-5, atol=1e-4)
+    x = wide[..., 1:4].contiguous().requires_grad_()
+    h, _ = ds.gated_recurrence(x, gate, reverse=reverse, form="decay")
+    v = torch.randn(2, 2000, 8, device="cuda")[..., 2:5]          # a gradient whose rows do not lie together
+    got, = torch.autograd.grad(h, x, v, retain_graph=True)
+    assert torch.equal(got, torch.autograd.grad(h, x, v.contiguous())[0])
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("d, heads, dtype", [(64, 64, "fp32"), (64, 1, "bf16"), (6, 6, "fp16"), (4, 1, "fp32"), (3, 1, "fp32"), (1, 1, "bf16")])
+def test_many_tiles_and_segments(d, heads, dtype, reverse):
+    """Long enough to be cut into segments whose maps are carried on: one sequence, a few whose borders lie anywhere, and a padded
+    batch; the composition passes segments with and without borders."""
+    check("dense", [12000], 12000, d, heads, dtype=dtype, reverse=reverse, coupled=True)
+    check("packed", [1, 5000, 0, 40, 40, 1, 6800, 13], 12000, d, heads, dtype=dtype, reverse=reverse)
+    check("padded", [0, 4000, 37], 4000, d, heads, dtype=dtype, reverse=reverse)
+
+
+def test_more_borders_in_a_tile_than_threads_look_at_once():
+    for reverse in (False, True):
+        check("packed", [1] * 2500, 2600, 1, 1, reverse=reverse)
+        check("packed", [0, 1, 0] * 700, 700, 3, 1, reverse=reverse, coupled=True)
+        check("packed", [0] * 255 + [1] + [0] * 600 + [2], 9, 8, 8, reverse=reverse)
+        check("dense", [1] * 2500, 1, 4, 4, reverse=reverse)
+        check("padded", [1, 0] * 900, 2, 1, 1, reverse=reverse)
 
 
 def test_no_rows_and_no_sequences():

@@ -147,6 +147,9 @@ def test_c_entry_points_refuse_null_pointers_small_workspaces_and_misaligned_ten
     backward = lambda **k: lib.dsb_recurrence_backward(  # noqa: E731
         C.byref(shape), 256, 256, None, k.get("marks", 256), 256, k.get("stride", 8), k.get("v_last", None), k.get("v_x", 256),
         k.get("v_gate", 256), k.get("v_state", None), 256, k.get("bytes", need), None)
+    colours = shape_of(rows=4, sequences=1, sequence_rows=4, channels=3, heads=1, x_stride=3, gate_stride=1)
+    assert lib.dsb_recurrence_backward(C.byref(colours), 256, 256, None, 256, 256, 5, None, 256, 256, None, 256, 1 << 20, None) == -1
+    assert "contiguous" in lib.dsb_last_error().decode()
     for k in (dict(marks=None), dict(marks=264), dict(stride=9), dict(v_last=512, v_state=512), dict(v_x=260), dict(v_gate=260)):
         assert backward(**k) == -1, k
     assert backward(bytes=0) == -3
