@@ -5,7 +5,6 @@
 // Not part of the reference as an operator of its own; its blend (cpp/rasterizer_kernels.cu:341-431) is the coupled form
 // over a tile's list, back to front, with f = 1 - alpha.
 //
-//
 // recurrence.cuh holds the kernels that walk along sequences, recurrence_<direction>_<type>.cu instantiate them; here are the
 // single-row kernel, the argument checks and the rules by which a call is cut into blocks.
 #include <cmath>
@@ -73,7 +72,7 @@ recurrence_step_kernel(const T* x, const T* gate, float* state, T* h, const long
 // ---- host ----------------------------------------------------------------------------------------------------------------
 
 struct Layout {            // how a call is cut; the same for the forward and the backward of one shape
-    int vec;               // channels per thread: 4 or 1
+    int vec;               // channels per thread: 4, 3 or 1
     int tx, groups;        // threads side by side on one row; groups of rows in a tile
     bool shuffle;
     int per_head;          // channels that share a gate; all of them when every channel has its own
@@ -85,6 +84,8 @@ struct Layout {            // how a call is cut; the same for the forward and th
     int64_t segments, segment_tiles;       // of a chain
 };
 constexpr int kSms = 148, kBlocksPerSm = 2;
+// A chain of fewer tiles is not cut: a tile after another takes a block about 2 us, a second launch and its first tile 6 us.
+constexpr int kLeastTilesToCut = 8;
 
 int check_shape(const DsbRecurrence& s, bool step) {
     DSB_REQUIRE(s.dtype == DSB_DTYPE_F32 || s.dtype == DSB_DTYPE_F16 || s.dtype == DSB_DTYPE_BF16, "recurrence: unknown dtype %d", s.dtype);
@@ -147,7 +148,7 @@ Layout layout_of(const DsbRecurrence& s) {
         while (tx < wide) tx *= 2;
         best = fill_in(tx);
         const int64_t blocks = best.chains * best.heads;
-        if (2 * blocks < kSms * kBlocksPerSm) best.segments = kSms * kBlocksPerSm / blocks;
+        if (2 * blocks < kSms * kBlocksPerSm && best.tiles >= kLeastTilesToCut) best.segments = kSms * kBlocksPerSm / blocks;
     } else {
         // The number of threads that share a row, and whether sequences are cut (which reads the inputs twice), by what share
         // of the threads' time goes into elements: threads without channels, SMs without their two blocks, pieces of a row that
@@ -166,7 +167,7 @@ Layout layout_of(const DsbRecurrence& s) {
             const double whole = share * (per_sm <= 1 ? 0.65 * per_sm : per_sm / (kBlocksPerSm * std::ceil(per_sm / kBlocksPerSm)));
             int64_t segments = (int64_t)(kBlocksPerSm / per_sm);
             if (segments > c.tiles) segments = c.tiles;
-            const double cut = segments > 1 ? share * per_sm * segments / kBlocksPerSm / 1.6 : 0;
+            const double cut = segments > 1 && c.tiles >= kLeastTilesToCut ? share * per_sm * segments / kBlocksPerSm / 1.6 : 0;
             if (whole > most) { most = whole; best = c; }
             if (cut > most) { most = cut; best = c; best.segments = segments; }
         }
