@@ -561,7 +561,7 @@ __device__ __forceinline__ Map<V, A> publish_map(const RecurrenceArgs& a, const 
 }
 // Once a tile's maps are published: the first `tx` threads carry the state through them in their order and leave every entry's
 // starting state in the place of its b.  Nobody else needs the state between tiles.  Two barriers a tile, but the
-// composition costs the block one thread's work per channel instead of every thread's.
+// composition costs the block one thread's work per channel instead of every thread's.  The second barrier is the caller's.
 template <bool FORWARD, bool PLAIN, int V, int A>
 __device__ __forceinline__ void pass_entries(const RecurrenceArgs& a, const Place& p, TileMaps<V, A>& sh, float (&carry)[V]) {
     if (threadIdx.x < a.tx) {
@@ -573,7 +573,6 @@ __device__ __forceinline__ void pass_entries(const RecurrenceArgs& a, const Plac
             apply_map<PLAIN>(carry, m);
         }
     }
-    __syncthreads();
 }
 template <int V, int A>
 __device__ __forceinline__ void entry_state(const RecurrenceArgs& a, const Place& p, const TileMaps<V, A>& sh, float (&h)[V]) {
@@ -754,6 +753,7 @@ __device__ void carry_of_segment(const RecurrenceArgs& a, const Place& p, TileMa
     }
     __syncthreads();
     pass_entries<true, false>(a, p, sh, carry);   // only the first threads' carry counts
+    __syncthreads();
 }
 
 // Leaves the composition of a whole segment's tiles.
@@ -959,6 +959,7 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
             }
             float h[V];
             pass_entries<true, PLAIN>(a, p, sh[t & 1], carry);
+            __syncthreads();
             entry_state(a, p, sh[t & 1], h);
             if (a.shuffle) apply_map<PLAIN>(h, before);
             store_floats_if<float, V>(to_start, h, keep);
@@ -1162,7 +1163,15 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                 mul(own.b, f, own.b);
             }
             const Map<V, A> after = publish_map<false, PLAIN>(a, p, own, sh[t & 1]);
-            if (APPLY) {                       // u_t: h_{t-1}, coupled: h_{t-1} - x_t
+            if (FLAT) copies_landed<0>();
+            __syncthreads();
+            if (FLAT) write_back();
+            if (!APPLY) {
+                pass_entries<false, PLAIN>(a, p, sh[t & 1], all);
+                return;
+            }
+            pass_entries<false, PLAIN>(a, p, sh[t & 1], q_carry);
+            {   // u_t: h_{t-1}, coupled: h_{t-1} - x_t.  Worked out while the first threads carry q through the tile's maps.
                 float h[V];
 #pragma unroll
                 for (int v = 0; v < V; ++v) h[v] = start[v];
@@ -1189,15 +1198,8 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                     for (int v = 0; v < V; ++v) h[v] = rows.is_outside(l) ? h[v] : n[v];
                 }
             }
-            if (FLAT) copies_landed<0>();
             __syncthreads();
-            if (FLAT) write_back();
-            if (!APPLY) {
-                pass_entries<false, PLAIN>(a, p, sh[t & 1], all);
-                return;
-            }
             float q[V];
-            pass_entries<false, PLAIN>(a, p, sh[t & 1], q_carry);
             entry_state(a, p, sh[t & 1], q);
             if (a.shuffle) apply_map<PLAIN>(q, after);
             [[maybe_unused]] char *row_x = to_x + (L - 1) * a.h_stride, *row_gate = to_gate + (L - 1) * a.gate_out_stride;
