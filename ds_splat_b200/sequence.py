@@ -229,7 +229,7 @@ def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, state: Optional[torch.
             _require(lengths, "lengths", x.device, torch.int32)
             if tuple(lengths.shape) != (x.shape[0],):
                 raise ValueError(f"lengths must have one entry per sequence: {list(lengths.shape)} against {x.shape[0]}")
-            lengths = lengths.contiguous()
+            lengths = lengths.contiguous() if x.shape[1] else None     # no rows: nothing to cut short
     sequences = x.shape[0] if offsets is None else offsets.numel() - 1
     state = _state(state, (sequences, x.shape[-1]), x.device, "state")
     call = _Call(x, gate, sequences, x.shape[1] if offsets is None else 0, form, coupled, reverse, offsets, lengths, final_only)

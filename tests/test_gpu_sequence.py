@@ -183,6 +183,8 @@ def test_no_rows_and_no_sequences():
     assert h.shape == (3, 0, 8) and torch.equal(last, st)
     dx, dst = torch.autograd.grad(last, (x, st), torch.ones_like(last))
     assert dx.shape == x.shape and torch.equal(dst, torch.ones_like(st))
+    h, last = ds.gated_recurrence(x, x.detach(), st, lengths=torch.zeros(3, dtype=torch.int32, device="cuda"))
+    assert h.shape == (3, 0, 8) and torch.equal(last, st)
     h, last = ds.gated_recurrence(torch.zeros(0, 5, 8, device="cuda"), torch.zeros(0, 5, 8, device="cuda"))
     assert h.shape == (0, 5, 8) and last.shape == (0, 8)
     h, last = ds.gated_recurrence(torch.zeros(0, 8, device="cuda"), torch.zeros(0, 1, device="cuda"),
@@ -606,9 +608,65 @@ def test_training_step_with_dropped_splats(accumulate):
     gone = (dropped == 0).view(-1)
     left = base["opacities"].view(-1)[gone] if accumulate else torch.zeros(int(gone.sum()), device="cuda")
     assert torch.equal(got.views["opacities"].view(-1)[gone], left)
+    # every splat dropped: nothing is drawn, and the gradients are zero
+    none = GradientBuffer(sc.n, "cuda")
+    images = []
+    renderer.render_views(cams[:2], lambda i, image: (images.append(float(image.abs().max())), vimgs[i])[1], none, dropout=SplatDropout(1.0, 1))
+    assert images == [0.0, 0.0] and not none.views["opacities"].any() and not none.views["shs"].any()
     # the data-parallel step hands the argument on, and without it nothing changes
     again = GradientBuffer(sc.n, "cuda")
     data_parallel_step(renderer, cams, vimgs, again, dropout=drop)
     assert bool((again.views["opacities"].view(-1)[gone] == 0).all())
     data_parallel_step(renderer, cams, vimgs, again)
     assert bool((again.views["opacities"].view(-1)[gone] != 0).any())
+
+
+def test_calls_on_two_streams_at_once():
+    """Calls that overlap share nothing: workspaces, border tables and checkpoints are each call's own."""
+    inputs = [make(20000, 64, 16, 3, "bf16", "logit", 20 + i) for i in range(2)]
+    offsets = torch.tensor([0, 7000, 7001, 20000], dtype=torch.int32, device="cuda")
+
+    def run(x, g, st, v_h, v_last):
+        leaves = [t.detach().requires_grad_() for t in (x, g, st)]
+        h, last = ds.gated_recurrence(*leaves, offsets=offsets, coupled=True)
+        return [h.detach(), last.detach(), *torch.autograd.grad((h, last), leaves, (v_h, v_last))]
+
+    want = [run(*i) for i in inputs]
+    streams = [torch.cuda.Stream() for _ in inputs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(4):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(run(*inputs[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for r in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[k]))
+
+
+def test_changed_inputs_are_noticed_before_the_backward_pass():
+    x = torch.randn(2, 30, 8, device="cuda", requires_grad=True)
+    g = torch.randn(2, 30, 8, device="cuda")
+    lengths = torch.tensor([30, 4], dtype=torch.int32, device="cuda")
+    h, _ = ds.gated_recurrence(x, g, lengths=lengths)
+    lengths[1] = 9
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        h.sum().backward()
+    h, _ = ds.gated_recurrence(x, g)
+    g.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        h.sum().backward()
+
+
+def test_gradients_of_gradients_are_refused():
+    x = torch.randn(1, 9, 4, device="cuda", requires_grad=True)
+    h, _ = ds.gated_recurrence(x, x)
+    first, = torch.autograd.grad(h.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(first.sum(), x)
+    y = ds.dropout(x, 0.5, (1, 1))
+    first, = torch.autograd.grad((y * y).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(first.sum(), x)
