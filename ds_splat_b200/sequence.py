@@ -210,6 +210,8 @@ def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, state: Optional[torch.
     final_only  return ``(None, last)`` and do not write ``h``.
 
     Rows that belong to no sequence come back as zeros, their gradients too; a sequence of no rows hands its state on.
+    Kept for the backward pass: the inputs, and a float32 state per channel and 3 to 12 rows.  No call waits for the device;
+    a training step can be captured into a graph (as always with torch, while no eager graph of the same leaves lives).
     Offsets and lengths live on the device and are not read back: values out of order or range make the results invalid and
     are reported by ``dsb_take_device_status`` and by the rasterizer's calls that synchronise."""
     _check_gate(x, gate, form)

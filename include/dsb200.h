@@ -476,7 +476,9 @@ int dsb_adam_step(float* params, const float* grads, float* exp_avg, float* exp_
  * channels; this entry takes any number of channels and any lists, a tile's `ranges` among them.
  *
  * Rows: x and h are [rows][channels], gate is [rows][gate_heads]; each head's gate is shared by channels / gate_heads
- * consecutive channels.  Rows are x_stride / gate_stride elements apart; h and the gradients are contiguous.
+ * consecutive channels.  Rows are x_stride / gate_stride elements apart; h and the gradients are contiguous.  Where the
+ * channels that share a gate (all of them when each has its own) are a multiple of four, every row of x, h, the gradients
+ * and per-channel gates starts on a boundary of four elements.  At most 2^31 - 2^16 rows.
  *   sequence_rows > 0: sequence s is rows s * sequence_rows ..., rows == sequences * sequence_rows; with `lengths`
  *                      (int32 per sequence on the device) only its first lengths[s] rows belong to it.
  *   sequence_rows == 0: packed; sequence s is rows [offsets[s], offsets[s+1]) (int32 on the device, nondecreasing,
@@ -487,10 +489,11 @@ int dsb_adam_step(float* params, const float* grads, float* exp_avg, float* exp_
  * States and their gradients are float [sequences][channels].  Decays are meant to lie in [-1, 1]: the scan forms
  * products of a sequence's decays, which overflow where the sequence itself would not if many of them are larger.
  *
- * checkpoints (dsb_recurrence_checkpoint_bytes; NULL when no backward follows) receives the states between the pieces
- * a sequence is cut into, which the backward starts from; nothing else is kept.  workspace:
- * dsb_recurrence_workspace_bytes, for either direction, free again when the call's work is done.
- * Results do not depend on timing: the same call gives the same bits. */
+ * checkpoints (dsb_recurrence_checkpoint_bytes: a float per channel and group of 3 to 12 rows; NULL when no backward
+ * follows) receives the states that the backward starts from; the backward of a call gets the same shape, strides
+ * included, and nothing else is kept.  workspace: dsb_recurrence_workspace_bytes, for either direction, free again when
+ * the call's work is done; calls that overlap need one each.  Both are 16-byte aligned.  No call synchronises, and no
+ * kernel waits for another block.  Results do not depend on timing: the same call gives the same bits. */
 #define DSB_GATE_DECAY 0
 #define DSB_GATE_LOGIT 1
 typedef struct DsbRecurrence {
@@ -507,7 +510,8 @@ int64_t dsb_recurrence_checkpoint_bytes(const DsbRecurrence* shape);
 int dsb_recurrence_forward(const DsbRecurrence* shape, const void* x, const void* gate, const float* state_in /* may be NULL */,
                            void* h /* NULL: only the state is wanted */, float* state_out,
                            float* checkpoints /* may be NULL */, void* workspace, int64_t workspace_bytes, void* stream);
-/* v_h (rows v_h_stride elements apart) or v_state_out may be NULL (zero); of the results v_x, v_gate and v_state_in
+/* v_h (rows v_h_stride elements apart; contiguous where x has contiguous rows of three 32-bit channels) or v_state_out may
+ * be NULL (zero); of the results v_x, v_gate and v_state_in
  * those that are NULL are not wanted.  v_gate sums over the channels that share a gate, in a fixed order. */
 int dsb_recurrence_backward(const DsbRecurrence* shape, const void* x, const void* gate, const float* state_in /* as forward */,
                             const float* checkpoints, const void* v_h, int64_t v_h_stride, const float* v_state_out,
