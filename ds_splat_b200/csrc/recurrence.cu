@@ -72,7 +72,7 @@ recurrence_step_kernel(const T* x, const T* gate, float* state, T* h, const long
 // ---- host ----------------------------------------------------------------------------------------------------------------
 
 struct Layout {            // how a call is cut; the same for the forward and the backward of one shape
-    int vec;               // channels per thread: 4, 3 or 1
+    int vec;               // channels per thread: 4, 3, 2 or 1
     int tx, groups;        // threads side by side on one row; groups of rows in a tile
     bool shuffle;
     int per_head;          // channels that share a gate; all of them when every channel has its own
@@ -115,7 +115,8 @@ int shape_vec(const DsbRecurrence& s) {
     const bool shared = s.gate_heads != s.channels;
     // colours: contiguous rows of three 32-bit channels are taken flat
     if (s.channels == 3 && s.dtype == DSB_DTYPE_F32 && s.x_stride == 3 && (shared || s.gate_stride == 3)) return 3;
-    return (shared ? s.channels / s.gate_heads : s.channels) % 4 == 0 ? 4 : 1;
+    const int together = shared ? s.channels / s.gate_heads : s.channels;
+    return together % 4 == 0 ? 4 : together % 2 == 0 ? 2 : 1;
 }
 Layout layout_of(const DsbRecurrence& s) {
     Layout l = {};
@@ -269,21 +270,24 @@ int run_direction(const DsbRecurrence& shape, const Cut& c, cudaStream_t s) {
     return rc;
 }
 
-// Vector tiles (four channels a thread) need every row of every tensor on a boundary of four elements.
-int check_alignment(const DsbRecurrence& s, const void* p, int64_t stride, int elem, bool wide, const char* name) {
-    if (!p || !wide) return DSB_OK;
-    DSB_REQUIRE(aligned(p, 4 * elem) && stride % 4 == 0,
-                "recurrence: with channels in fours, %s must start on a boundary of four elements and its rows lie a multiple of "
-                "four elements apart", name);
+// Channels that a thread takes `lanes` at a time need every row of every tensor on such a boundary.
+int vector_lanes(const DsbRecurrence& s) {
+    const int vec = shape_vec(s);
+    return vec == 3 ? 1 : vec;
+}
+int check_alignment(const void* p, int64_t stride, int elem, int lanes, const char* name) {
+    if (!p || lanes == 1) return DSB_OK;
+    DSB_REQUIRE(aligned(p, lanes * elem) && stride % lanes == 0,
+                "recurrence: with these channels %s must start on a boundary of %d elements and its rows lie a multiple of that apart",
+                name, lanes);
     return DSB_OK;
 }
 #define DSB_TRY(expr) do { const int rc__ = (expr); if (rc__ != DSB_OK) return rc__; } while (0)
 
 int check_inputs(const DsbRecurrence& s, const void* x, const void* gate) {
-    const bool wide = shape_vec(s) == 4;
-    const int elem = dtype_bytes(s.dtype);
-    DSB_TRY(check_alignment(s, x, s.x_stride, elem, wide, "x"));
-    return check_alignment(s, gate, s.gate_stride, elem, wide && s.gate_heads == s.channels, "the gate");
+    const int lanes = vector_lanes(s), elem = dtype_bytes(s.dtype);
+    DSB_TRY(check_alignment(x, s.x_stride, elem, lanes, "x"));
+    return check_alignment(gate, s.gate_stride, elem, s.gate_heads == s.channels ? lanes : 1, "the gate");
 }
 
 }  // namespace
@@ -308,12 +312,11 @@ int launch_recurrence_forward(const DsbRecurrence& shape, const void* x, const v
     if (shape.rows == 0) return pass_states(state_in, state_out, (int64_t)shape.sequences * shape.channels, s);
     DSB_REQUIRE(x && gate, "recurrence: null pointer");
     DSB_REQUIRE(!state_in || state_in != state_out, "recurrence: state_out must not be state_in");
-    const bool wide = shape_vec(shape) == 4;
-    const int elem = dtype_bytes(shape.dtype);
+    const int lanes = vector_lanes(shape), elem = dtype_bytes(shape.dtype);
     DSB_TRY(check_inputs(shape, x, gate));
-    DSB_TRY(check_alignment(shape, h, shape.channels, elem, wide, "h"));
-    DSB_TRY(check_alignment(shape, state_in, shape.channels, 4, wide, "state_in"));
-    DSB_TRY(check_alignment(shape, state_out, shape.channels, 4, wide, "state_out"));
+    DSB_TRY(check_alignment(h, shape.channels, elem, lanes, "h"));
+    DSB_TRY(check_alignment(state_in, shape.channels, 4, lanes, "state_in"));
+    DSB_TRY(check_alignment(state_out, shape.channels, 4, lanes, "state_out"));
     Cut c;
     DSB_TRY(make_cut(shape, true, workspace, workspace_bytes, checkpoints, &c));
     const bool r = shape.reverse != 0;
@@ -332,16 +335,15 @@ int launch_recurrence_backward(const DsbRecurrence& shape, const void* x, const 
     if (shape.rows == 0) return pass_states(v_state_out, v_state_in, (int64_t)shape.sequences * shape.channels, s);
     DSB_REQUIRE(x && gate && checkpoints, "recurrence: null pointer");
     DSB_REQUIRE(!v_state_in || v_state_in != v_state_out, "recurrence: v_state_in must not be v_state_out");
-    const bool wide = shape_vec(shape) == 4;
-    const int elem = dtype_bytes(shape.dtype);
+    const int lanes = vector_lanes(shape), elem = dtype_bytes(shape.dtype);
     DSB_TRY(check_inputs(shape, x, gate));
-    DSB_TRY(check_alignment(shape, v_h, v_h_stride, elem, wide, "v_h"));
+    DSB_TRY(check_alignment(v_h, v_h_stride, elem, lanes, "v_h"));
     DSB_REQUIRE(!v_h || shape_vec(shape) != 3 || v_h_stride == 3, "recurrence: where x's rows of three channels are contiguous, v_h's must be");
-    DSB_TRY(check_alignment(shape, v_x, shape.channels, elem, wide, "v_x"));
-    DSB_TRY(check_alignment(shape, v_gate, shape.gate_heads, elem, wide && shape.gate_heads == shape.channels, "v_gate"));
-    DSB_TRY(check_alignment(shape, state_in, shape.channels, 4, wide, "state_in"));
-    DSB_TRY(check_alignment(shape, v_state_out, shape.channels, 4, wide, "v_state_out"));
-    DSB_TRY(check_alignment(shape, v_state_in, shape.channels, 4, wide, "v_state_in"));
+    DSB_TRY(check_alignment(v_x, shape.channels, elem, lanes, "v_x"));
+    DSB_TRY(check_alignment(v_gate, shape.gate_heads, elem, shape.gate_heads == shape.channels ? lanes : 1, "v_gate"));
+    DSB_TRY(check_alignment(state_in, shape.channels, 4, lanes, "state_in"));
+    DSB_TRY(check_alignment(v_state_out, shape.channels, 4, lanes, "v_state_out"));
+    DSB_TRY(check_alignment(v_state_in, shape.channels, 4, lanes, "v_state_in"));
     Cut c;
     DSB_TRY(make_cut(shape, false, workspace, workspace_bytes, const_cast<float*>(checkpoints), &c));
     const bool r = shape.reverse != 0;
@@ -360,13 +362,12 @@ int launch_recurrence_step(const DsbRecurrence& shape, const void* x, const void
     DSB_TRY(check_shape(shape, true));
     if (shape.rows == 0) return DSB_OK;
     DSB_REQUIRE(x && gate && state && h, "recurrence: null pointer");
-    const bool wide = shape_vec(shape) == 4;
-    const int elem = dtype_bytes(shape.dtype);
+    const int lanes = vector_lanes(shape), elem = dtype_bytes(shape.dtype);
     DSB_TRY(check_inputs(shape, x, gate));
-    DSB_TRY(check_alignment(shape, h, shape.channels, elem, wide, "h"));
-    DSB_TRY(check_alignment(shape, state, shape.channels, 4, wide, "the state"));
+    DSB_TRY(check_alignment(h, shape.channels, elem, lanes, "h"));
+    DSB_TRY(check_alignment(state, shape.channels, 4, lanes, "the state"));
     const long long count = shape.rows * shape.channels;
-    const long long blocks = (count / (wide ? 4 : 1) + kWalkThreads - 1) / kWalkThreads;
+    const long long blocks = (count / lanes + kWalkThreads - 1) / kWalkThreads;
     DSB_REQUIRE(blocks <= kMaxBlocks, "recurrence: too many elements for one launch");
     const int per_head = shape.channels / shape.gate_heads;
     with_dtype(shape.dtype, [&](auto tag) {
@@ -377,8 +378,10 @@ int launch_recurrence_step(const DsbRecurrence& shape, const void* x, const void
                                                              shape.coupled != 0);
         };
         const bool logit = shape.gate_form == DSB_GATE_LOGIT;
-        if (wide && logit) launch(recurrence_step_kernel<T, 4, true>);
-        else if (wide) launch(recurrence_step_kernel<T, 4, false>);
+        if (lanes == 4 && logit) launch(recurrence_step_kernel<T, 4, true>);
+        else if (lanes == 4) launch(recurrence_step_kernel<T, 4, false>);
+        else if (lanes == 2 && logit) launch(recurrence_step_kernel<T, 2, true>);
+        else if (lanes == 2) launch(recurrence_step_kernel<T, 2, false>);
         else if (logit) launch(recurrence_step_kernel<T, 1, true>);
         else launch(recurrence_step_kernel<T, 1, false>);
     });

@@ -65,7 +65,7 @@ constexpr int kMaxEntries = 32;
 
 // Consecutive rows of a thread: as many as keep the backward's values of a tile in registers and two tiles of every tensor
 // in shared memory with several blocks on an SM.
-template <typename T> __host__ __device__ constexpr int walk_rows(int vec) { return vec == 4 ? (sizeof(T) == 4 ? 3 : 5) : vec == 3 ? 5 : 12; }
+template <typename T> __host__ __device__ constexpr int walk_rows(int vec) { return vec == 4 ? (sizeof(T) == 4 ? 3 : 5) : vec == 3 ? 5 : vec == 2 ? (sizeof(T) == 4 ? 6 : 8) : 12; }
 
 // ---- V channels at a time -------------------------------------------------------------------------------------------
 // Two channels an instruction where the hardware has one; `a` may be a single value for all channels.
@@ -655,16 +655,10 @@ struct RowBorders<true> {      // a plain tile: all inside, no borders
 template <typename T, int V>
 __device__ __forceinline__ void copy_async(unsigned to, const T* from, bool there) {
     constexpr int kBytes = V * sizeof(T);
-    if (kBytes == 2) {                            // below what an asynchronous copy takes
-        unsigned short v = 0;
-        if (there) v = *reinterpret_cast<const unsigned short*>(from);
-        asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(v) : "memory");
-    } else {
-        const int bytes = there ? kBytes : 0;     // what is not copied is filled with zeros
-        if (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-        else if (kBytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-        else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-    }
+    const int bytes = there ? kBytes : 0;         // what is not copied is filled with zeros
+    if (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+    else if (kBytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT>
@@ -698,6 +692,22 @@ __device__ __forceinline__ void fetch_rows(unsigned to, const char* from, const 
         for (int l = 0; l < L; ++l) copy_async<T, V>(to + l * kRow, reinterpret_cast<const T*>(l < left ? from + l * stride : base), l < left);
     }
 }
+// Single 16-bit elements are below what an asynchronous copy takes: loaded, all tensors' rows together, and stored.
+template <typename T, int L>
+struct NarrowRows {
+    T v[L];
+    __device__ __forceinline__ void load(const char* from, const long long& stride, int left) {
+#pragma unroll
+        for (int l = 0; l < L; ++l) {
+            memset(&v[l], 0, sizeof(T));
+            if (l < left) v[l] = *reinterpret_cast<const T*>(from + l * stride);
+        }
+    }
+    __device__ __forceinline__ void store(unsigned char* stage) const {
+#pragma unroll
+        for (int l = 0; l < L; ++l) reinterpret_cast<T*>(stage)[l * kWalkThreads + threadIdx.x] = v[l];
+    }
+};
 // A gate that channels share is read directly, as every thread of a row wants the same value.
 template <typename T, int L>
 __device__ __forceinline__ void fetch_shared_gates(T (&own)[L], const char* from, const long long& stride, int left) {
@@ -853,9 +863,18 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
                 } else {
                     const int rest = a.chain_rows - t * tile_rows;
                     const int left = min(rest - p.row0, L);
-                    const unsigned to = s_ring + fetched * sizeof(Ring);
-                    fetch_rows<T, V, L>(to, x, a.x_stride, rest >= tile_rows, left, static_cast<const char*>(a.x));
-                    if (!SHARED) fetch_rows<T, V, L>(to + kTensor, gate, a.gate_stride, rest >= tile_rows, left, static_cast<const char*>(a.gate));
+                    if constexpr (V * sizeof(T) == 2) {
+                        NarrowRows<T, L> rx, rg;
+                        rx.load(x, a.x_stride, left);
+                        if (!SHARED) rg.load(gate, a.gate_stride, left);
+                        unsigned char* to = s_raw + fetched * sizeof(Ring);
+                        rx.store(to);
+                        if (!SHARED) rg.store(to + kTensor);
+                    } else {
+                        const unsigned to = s_ring + fetched * sizeof(Ring);
+                        fetch_rows<T, V, L>(to, x, a.x_stride, rest >= tile_rows, left, static_cast<const char*>(a.x));
+                        if (!SHARED) fetch_rows<T, V, L>(to + kTensor, gate, a.gate_stride, rest >= tile_rows, left, static_cast<const char*>(a.gate));
+                    }
                 }
             }
             x += a.x_step;
@@ -1046,9 +1065,20 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                 } else {
                     const int rest = a.chain_rows - t * tile_rows;
                     const int left = min(rest - p.row0, L);
-                    if (a.v_h) fetch_rows<T, V, L>(to + kVhAt * kTensor, vh, a.v_h_stride, rest >= tile_rows, left, static_cast<const char*>(a.v_h));
-                    if (!SHARED) fetch_rows<T, V, L>(to + kGateAt * kTensor, gate, a.gate_stride, rest >= tile_rows, left, static_cast<const char*>(a.gate));
-                    if (APPLY) fetch_rows<T, V, L>(to + kXAt * kTensor, x, a.x_stride, rest >= tile_rows, left, static_cast<const char*>(a.x));
+                    if constexpr (V * sizeof(T) == 2) {
+                        NarrowRows<T, L> rx, rg, rv;
+                        if (a.v_h) rv.load(vh, a.v_h_stride, left);
+                        if (!SHARED) rg.load(gate, a.gate_stride, left);
+                        if (APPLY) rx.load(x, a.x_stride, left);
+                        unsigned char* at = s_raw + fetched * stage_bytes;
+                        if (a.v_h) rv.store(at + kVhAt * kTensor);
+                        if (!SHARED) rg.store(at + kGateAt * kTensor);
+                        if (APPLY) rx.store(at + kXAt * kTensor);
+                    } else {
+                        if (a.v_h) fetch_rows<T, V, L>(to + kVhAt * kTensor, vh, a.v_h_stride, rest >= tile_rows, left, static_cast<const char*>(a.v_h));
+                        if (!SHARED) fetch_rows<T, V, L>(to + kGateAt * kTensor, gate, a.gate_stride, rest >= tile_rows, left, static_cast<const char*>(a.gate));
+                        if (APPLY) fetch_rows<T, V, L>(to + kXAt * kTensor, x, a.x_stride, rest >= tile_rows, left, static_cast<const char*>(a.x));
+                    }
                 }
             }
             vh -= a.v_h_step;
@@ -1316,6 +1346,7 @@ template <typename T, bool FORWARD>
 int run_walk(const RecurrenceLaunch& c, cudaStream_t s) {
     if constexpr (sizeof(T) == 4)
         if (c.vec == 3) return run_walk<T, 3, FORWARD>(c, s);
+    if (c.vec == 2) return run_walk<T, 2, FORWARD>(c, s);
     return c.vec == 4 ? run_walk<T, 4, FORWARD>(c, s) : run_walk<T, 1, FORWARD>(c, s);
 }
 

@@ -80,7 +80,7 @@ def _state(t: Optional[torch.Tensor], shape, device, name):
     _require(t, name, device, torch.float32)
     if t.shape != shape:
         raise ValueError(f"{name} must have the shape {list(shape)}, got {list(t.shape)}")
-    return _rows(t, 4 if shape[-1] % 4 == 0 else 1)[0].contiguous()
+    return _rows(t, 4 if shape[-1] % 4 == 0 else 2 if shape[-1] % 2 == 0 else 1)[0].contiguous()
 
 
 def _check_gate(x, gate, form):
@@ -110,7 +110,8 @@ class _Call:
 
     def __init__(self, x, gate, sequences, sequence_rows, form, coupled, reverse, offsets, lengths, final_only=False):
         d, heads = x.shape[-1], gate.shape[-1]
-        self.lanes = lanes = 4 if (d // heads if heads != d else d) % 4 == 0 else 1
+        together = d // heads if heads != d else d
+        self.lanes = lanes = 4 if together % 4 == 0 else 2 if together % 2 == 0 else 1
         self.x, x_stride = _rows(x, lanes)
         self.gate, gate_stride = _rows(gate, lanes if heads == d else 1)
         self.sequences, self.final_only = sequences, final_only
