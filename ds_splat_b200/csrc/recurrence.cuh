@@ -5,12 +5,13 @@
 // that an infinity of the sequence before cannot meet a zero).
 //
 // A block walks along one stretch of rows and a block of channels, tile by tile, and carries the state in registers: it
-// reads everything once and writes everything once.  Inside a tile a thread runs L consecutive rows of V channels, a warp
-// composes its threads' maps with shuffles, the block its warps' through shared memory (one barrier a tile); the next
-// tile's rows are on their way into shared memory meanwhile (each thread copies what it will read itself, so their arrival
-// needs no barrier).  Where sequences and channels alone make too few blocks for the GPU, a sequence is cut into segments:
-// a first launch leaves every segment's map, and each block of the second starts from the composition of those before it.
-// That reads the inputs twice, the second time mostly from L2 where the call is small enough to need it.
+// reads everything once and writes everything once.  Inside a tile a thread runs L consecutive rows of V channels, and the
+// threads' maps meet in shared memory, where one thread per channel passes the state through them (two barriers a tile).
+// The next tile's rows are on their way into shared memory meanwhile; each thread copies what it will read itself, so their
+// arrival needs no barrier.  Where sequences and channels alone make too few blocks for the GPU, a sequence is cut into
+// segments: a first launch leaves every segment's map, and each block of the second starts from the composition of those
+// before it.  That reads the inputs twice, the second time from L2 where the call is small enough to need it; with packed
+// sequences only what lies behind a segment's last border is read twice.
 //
 // The backward walks from the last row to the first on q.  It needs h_{t-1}, and recomputes it in 32 bits from states that the
 // forward leaves at every thread's first row (a 32-bit value per L rows and channel): the h that was written out is
@@ -18,8 +19,21 @@
 //
 // Every order of composition is fixed by the shape alone, so results do not depend on timing; no block waits for another.
 //
-// What bounds it: instruction issue.  A tile without a sequence border ("plain") therefore has code of its own without any
-// test per row, and the form of the gate, the coupling and shared gates are template parameters.
+// Measured on 8 x 4096 x 2560 bf16, per-channel logits, coupled: forward 132 us for 570 MB, backward 209 us for 906 MB
+// (checkpoints included), 4.3 TB/s or 0.66 of the copy rate each.  What bounds it: instruction issue and the waits between a
+// tile's phases; DRAM is 45% busy, a scheduler issues in 47% of the cycles, 24 (39) instructions an element.  What led there,
+// forward + backward of that case:
+//   three launches (maps, a thread per channel over all chunks, apply), everything read twice           1810 us
+//   walking with the state in registers                                                                 1177
+//   code of its own for tiles without a border ("plain"), gate forms compiled in, states per row group   650
+//   gates kept as exp(-g): f and 1 - f from it in three instructions, without branches                   477
+//   two channels an instruction, no register spills (L chosen for 128 registers; every spill cost more
+//   than the occupancy it bought)                                                                        327
+//   blocks of 256 threads with as many threads a row as make two blocks an SM, maps through shared
+//   memory: the same here, but 0.9 to 0.75 of the time with padded, packed and narrow sequences          340
+// Tried and slower: three or four stages of prefetch (fewer blocks), 128 threads (row pieces below two sectors), every thread
+// passing through all of a tile's maps (one barrier, 10 instructions an element more).  Without the pass through the maps
+// the forward would take 114 us.
 #pragma once
 #include <atomic>
 #include <type_traits>
@@ -63,8 +77,9 @@ constexpr int kWalkThreads = 256;
 constexpr int kWalkWarps = kWalkThreads / 32;
 constexpr int kMaxEntries = 32;
 
-// Consecutive rows of a thread: as many as keep the backward's values of a tile in registers and two tiles of every tensor
-// in shared memory with several blocks on an SM.
+// Consecutive rows of a thread: as many as keep a tile's values in the 128 registers that two blocks on an SM leave a thread
+// (a row more spills: 8 x 4096 x 2560 bf16 backward 209 -> 273 us; a row less costs 4% by more tiles), and two tiles of every
+// tensor in shared memory.
 template <typename T> __host__ __device__ constexpr int walk_rows(int vec) { return vec == 4 ? (sizeof(T) == 4 ? 3 : 5) : vec == 3 ? 5 : vec == 2 ? (sizeof(T) == 4 ? 6 : 8) : 12; }
 
 // ---- V channels at a time -------------------------------------------------------------------------------------------
@@ -399,14 +414,14 @@ struct Borders {
     }
 };
 
-// Sequences without rows hand their state on (a warp copies what its lanes have found); offsets and lengths out of order or
-// range are reported.
+// Sequences without rows hand their state on; offsets and lengths out of order or range are reported.  Neighbours in the list go
+// to different blocks, and a warp copies what its lanes have found.
 __device__ __forceinline__ void pass_empty_sequences(const RecurrenceArgs& a, const float* in, float* out) {
     if (!a.offsets && !a.lengths) return;
     const int lane = threadIdx.x & 31;
     const long long step = (long long)gridDim.x * kWalkThreads;
-    for (long long s0 = (long long)blockIdx.x * kWalkThreads + (threadIdx.x & ~31); s0 < a.sequences; s0 += step) {
-        const long long s = s0 + lane;
+    for (long long s0 = blockIdx.x + (long long)(threadIdx.x & ~31) * gridDim.x; s0 < a.sequences; s0 += step) {
+        const long long s = s0 + (long long)lane * gridDim.x;
         bool empty = false, bad = false;
         if (s < a.sequences) {
             if (a.offsets) {
@@ -422,9 +437,10 @@ __device__ __forceinline__ void pass_empty_sequences(const RecurrenceArgs& a, co
         if (bad) atomicMin(a.device_status, DSB_ERR_INVALID_ARGUMENT);
         unsigned left = __ballot_sync(0xffffffffu, (empty || bad) && out);
         while (left) {
-            const long long at = (s0 + __ffs(left) - 1) * a.channels;
+            const long long at = (s0 + (long long)(__ffs(left) - 1) * gridDim.x) * a.channels;
             left &= left - 1;
-            for (int c = lane; c < a.channels; c += 32) out[at + c] = in ? in[at + c] : 0.f;
+#pragma unroll 8
+            for (int c = lane; c < a.channels; c += 32) out[at + c] = in ? __ldg(in + at + c) : 0.f;
         }
     }
 }
