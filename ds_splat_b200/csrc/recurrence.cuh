@@ -1326,7 +1326,7 @@ int launch_walk(const RecurrenceLaunch& c, cudaStream_t s) {
     }();
     const int tensors = FORWARD ? (SHARED ? 1 : 2) : (APPLY ? 1 : 0) + (SHARED ? 0 : 1) + (c.args.v_h ? 1 : 0);
     const size_t smem = (walk_stages(V) * tensors + (!FORWARD && !c.args.v_h ? 1 : 0)) * walk_tensor_bytes<T>(V) + kTables * sizeof(int) * table_ints(c.args.groups, L);
-    if (smem > 31 * 1024) {   // 48 KB with the static part: asked for once per device
+    {   // more than 48 KB with the static part, for most calls: asked for once per device
         static std::atomic<u64> asked{0};
         int device = 0;
         DSB_CUDA_CHECK(cudaGetDevice(&device));

@@ -158,13 +158,22 @@ def test_rows_of_three_channels(reverse):
 
 
 @pytest.mark.parametrize("reverse", [False, True])
-@pytest.mark.parametrize("d, heads, dtype", [(64, 64, "fp32"), (64, 1, "bf16"), (6, 6, "fp16"), (4, 1, "fp32"), (3, 1, "fp32"), (1, 1, "bf16")])
+@pytest.mark.parametrize("d, heads, dtype", [(64, 64, "fp32"), (48, 3, "fp32"), (64, 1, "bf16"), (6, 6, "fp16"), (4, 1, "fp32"), (3, 1, "fp32"), (1, 1, "bf16")])
 def test_many_tiles_and_segments(d, heads, dtype, reverse):
     """Long enough to be cut into segments whose maps are carried on: one sequence, a few whose borders lie anywhere, and a padded
     batch; the composition passes segments with and without borders."""
     check("dense", [12000], 12000, d, heads, dtype=dtype, reverse=reverse, coupled=True)
     check("packed", [1, 5000, 0, 40, 40, 1, 6800, 13], 12000, d, heads, dtype=dtype, reverse=reverse)
     check("padded", [0, 4000, 37], 4000, d, heads, dtype=dtype, reverse=reverse)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("d", [148, 160, 192, 204, 256])
+def test_only_the_last_state_of_long_wide_rows(d, dtype):
+    """Segments without an output: the backward pass over them holds just under 31 KB beside its static shared memory."""
+    for reverse in (False, True):
+        check("dense", [9000], 9000, d, d, dtype=dtype, final_only=True, reverse=reverse)
+        check("packed", [1, 4000, 0, 40, 4959], 9000, d, d, dtype=dtype, final_only=True, reverse=reverse)
 
 
 def test_more_borders_in_a_tile_than_threads_look_at_once():
