@@ -244,8 +244,9 @@ def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, state: Optional[torch.
 
 def gated_recurrence_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, *, form: str = "logit",
                           coupled: bool = False) -> torch.Tensor:
-    """One row of every sequence: x [S, D], gate [S, H], ``state`` (float32 [S, D], contiguous) updated in place; returns
-    the new states in the type of ``x``.  For generating token by token; it keeps nothing for a backward pass."""
+    """One row of every sequence: x [S, D], gate [S, H], ``state`` (float32 [S, D], contiguous, sharing no memory with
+    them) updated in place; returns the new states in the type of ``x``.  For generating token by token; it keeps nothing
+    for a backward pass."""
     _check_gate(x, gate, form)
     if x.dim() != 2:
         raise ValueError(f"x must be [S, D], got {list(x.shape)}")

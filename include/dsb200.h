@@ -517,7 +517,8 @@ int dsb_recurrence_backward(const DsbRecurrence* shape, const void* x, const voi
                             const float* checkpoints, const void* v_h, int64_t v_h_stride, const float* v_state_out,
                             void* v_x, void* v_gate, float* v_state_in, void* workspace, int64_t workspace_bytes, void* stream);
 /* The same for one new row of every sequence: x [sequences][channels], gate [sequences][gate_heads], state updated in
- * place, h contiguous.  Of `shape`, rows == sequences; offsets, lengths, sequence_rows and reverse are not looked at. */
+ * place, h contiguous, neither of them overlapping x or gate.  Of `shape`, rows == sequences; offsets, lengths,
+ * sequence_rows and reverse are not looked at. */
 int dsb_recurrence_step(const DsbRecurrence* shape, const void* x, const void* gate, float* state, void* h, void* stream);
 
 /* Dropout from a counter-based generator; the mask is not stored, the backward is the same call on the gradient:
