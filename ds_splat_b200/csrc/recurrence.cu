@@ -76,7 +76,8 @@ struct Layout {            // how a call is cut; the same for the forward and th
     int tx, groups;        // threads side by side on one row; groups of rows in a tile
     bool shuffle;
     int per_head;          // channels that share a gate; all of them when every channel has its own
-    int heads;             // 1 when every channel has its own gate
+    int head_blocks;       // blocks side by side, without the parts; 1 when every channel has its own gate
+    int block_heads;       // heads of a block
     int parts;             // channel blocks per head
     bool table;            // one chain over all rows, with sequence borders anywhere; else one chain per sequence
     int tile_rows;
@@ -123,8 +124,9 @@ Layout layout_of(const DsbRecurrence& s) {
     if (s.rows == 0) return l;
     l.vec = shape_vec(s);
     const bool shared = s.gate_heads != s.channels;
-    l.heads = shared ? s.gate_heads : 1;
-    l.per_head = s.channels / l.heads;
+    l.head_blocks = shared ? s.gate_heads : 1;
+    l.block_heads = 1;
+    l.per_head = s.channels / l.head_blocks;
     const int wide = (l.per_head + l.vec - 1) / l.vec;
     const int rows = s.dtype == DSB_DTYPE_F32 ? walk_rows<float>(l.vec) : walk_rows<__half>(l.vec);
     const int piece = l.vec * dtype_bytes(s.dtype);
@@ -145,10 +147,18 @@ Layout layout_of(const DsbRecurrence& s) {
     };
     Layout best = {};
     if (wide <= 8) {   // vec 3 among them: one thread per row
+        // Narrow heads lie side by side in a block until a row's piece fills two sectors; a head alone in a block would read a
+        // sector a row for a few bytes (29 x 3642 rows of 112 fp16 heads of 3 channels, a training pass: 670 us then, 401 so;
+        // 56528 packed rows of 106 bf16 heads of 3, the forward alone: 192 and 130).
         int tx = 1;
         while (tx < wide) tx *= 2;
+        while (shared && tx <= 16 && l.block_heads < s.gate_heads && l.block_heads * l.per_head * dtype_bytes(s.dtype) < 64) {
+            l.block_heads *= 2;
+            tx *= 2;
+        }
+        l.head_blocks = (l.head_blocks + l.block_heads - 1) / l.block_heads;
         best = fill_in(tx);
-        const int64_t blocks = best.chains * best.heads;
+        const int64_t blocks = best.chains * best.head_blocks;
         if (2 * blocks < kSms * kBlocksPerSm && best.tiles >= kLeastTilesToCut) best.segments = kSms * kBlocksPerSm / blocks;
     } else {
         // The number of threads that share a row, and whether sequences are cut (which reads the inputs twice), by what share
@@ -164,7 +174,7 @@ Layout layout_of(const DsbRecurrence& s) {
             const double elements = 20.0 * rows * l.vec;
             double share = (double)wide / (c.parts * tx) * (c.groups * tx) / kWalkThreads * elements / (elements + 60 + 9 * c.groups);
             if (c.parts > 1 && tx * piece % 32 != 0) share *= 0.93;
-            const double per_sm = (double)(c.chains * c.heads * c.parts) / kSms;
+            const double per_sm = (double)(c.chains * c.head_blocks * c.parts) / kSms;
             const double whole = share * (per_sm <= 1 ? 0.65 * per_sm : per_sm / (kBlocksPerSm * std::ceil(per_sm / kBlocksPerSm)));
             int64_t segments = (int64_t)(kBlocksPerSm / per_sm);
             if (segments > c.tiles) segments = c.tiles;
@@ -210,7 +220,8 @@ int make_cut(const DsbRecurrence& s, bool forward, void* workspace, int64_t work
     a.tiles = (int)l.tiles; a.segments = (int)l.segments; a.segment_tiles = (int)l.segment_tiles;
     a.checkpoints = checkpoints;
     a.sequences = s.sequences; a.sequence_rows = s.sequence_rows; a.channels = s.channels; a.gate_heads = s.gate_heads;
-    a.heads = l.heads; a.per_head = l.per_head; a.parts = l.parts;
+    a.per_head = l.per_head; a.head_blocks = l.head_blocks; a.block_heads = l.block_heads; a.head_threads = l.tx / l.block_heads;
+    a.parts = l.parts;
     a.tx = l.tx; a.groups = l.groups; a.shuffle = l.shuffle; a.entries = l.shuffle ? kWalkWarps : l.groups;
     a.logit = s.gate_form == DSB_GATE_LOGIT; a.coupled = s.coupled != 0; a.reverse = s.reverse != 0;
     a.shared = s.gate_heads != s.channels; a.table = l.table;
@@ -228,7 +239,7 @@ int make_cut(const DsbRecurrence& s, bool forward, void* workspace, int64_t work
         a.map_closed = reinterpret_cast<int*>(w); w += up16(maps * 4);
     }
     if (!forward && a.shared && l.parts > 1) a.gate_parts = reinterpret_cast<float*>(w);
-    const int64_t blocks = l.chains * l.segments * l.heads * l.parts;
+    const int64_t blocks = l.chains * l.segments * l.head_blocks * l.parts;
     DSB_REQUIRE(blocks <= kMaxBlocks, "recurrence: too many blocks for one launch");
     c.launch.vec = l.vec; c.launch.tile_rows = l.tile_rows; c.launch.blocks = (unsigned)blocks;
     return device_status_address(&a.device_status);

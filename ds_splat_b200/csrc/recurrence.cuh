@@ -59,7 +59,9 @@ struct RecurrenceArgs {
     long long h_stride, gate_out_stride;           // contiguous results of channels / heads
     long long x_step, gate_step, v_h_step, h_step, gate_out_step;   // from tile to tile
     int tiles, segments, segment_tiles;
-    int sequences, sequence_rows, channels, gate_heads, heads, per_head, parts;
+    int sequences, sequence_rows, channels, gate_heads, per_head;
+    int head_blocks, block_heads, head_threads;    // of a row; heads of a block; threads of a head (all tx, or a power of two)
+    int parts;             // blocks that share a head
     int tx, groups;        // threads side by side on one row, groups of L rows in a tile
     int shuffle, entries;  // whether a warp composes its maps by itself, and how many maps a tile leaves in shared memory
     int reverse, table;    // table: one chain over all rows, with sequence borders anywhere; else one chain per sequence
@@ -290,9 +292,9 @@ struct Borders {
         const char* at = reinterpret_cast<const char*>(states + (long long)id * all_channels + channel);
         for (int c = 0; c < channels * 4; c += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + c));
     }
-    __device__ void begin(const RecurrenceArgs& a, int chain, int p0, int* s_tables, int lanes, int head, int part) {
-        channel = head * a.per_head + part * a.tx * lanes;
-        channels = min(a.tx * lanes, a.per_head - part * a.tx * lanes);
+    __device__ void begin(const RecurrenceArgs& a, int chain, int p0, int* s_tables, int lanes, int block_head, int part) {
+        channel = block_head * a.per_head + part * a.tx * lanes;
+        channels = a.block_heads > 1 ? min(a.block_heads * a.per_head, a.channels - channel) : min(a.tx * lanes, a.per_head - part * a.tx * lanes);
         tables = s_tables;
         groups = a.groups;
         tile_rows = groups * L;
@@ -511,22 +513,25 @@ __device__ __forceinline__ Map<V, A> get_map(const TileMaps<V, A>& sh, int entry
 // Where many threads share a row, every group of rows leaves its map in shared memory (any number of threads a row, so that
 // the blocks can be made as many as the SMs hold).  Where few do (1, 2, 4 or 8), groups are many: a warp composes its own.
 struct Place {
-    int chain, segment, head, part, channel, tx;
+    int chain, segment, part, tx;
+    int block_head, head, channel;   // the block's first head; this thread's, and its first channel
     int row0, group;       // this thread's first row inside a tile, and which of the tile's groups of rows that is
     int entry;             // whose map in shared memory includes this thread's rows
-    bool there, active;    // there: one of the tile's groups; active: and not beyond the head's last channel
+    bool there, active;    // there: one of the tile's groups; active: and not beyond the head's last channel or the last head
+    bool leads;            // the first thread of a head
     int read_channel;      // what to read all the same where a thread has no channel
 };
 template <int V, int L>
 __device__ __forceinline__ Place place_of(const RecurrenceArgs& a) {
     Place p;
-    const int blocks = a.heads * a.parts;
+    const int blocks = a.head_blocks * a.parts;
     const int rest = (int)(blockIdx.x / (unsigned)blocks);
     const int block = (int)(blockIdx.x - (unsigned)rest * blocks);
     p.segment = rest / a.chains;
     p.chain = rest - p.segment * a.chains;
-    p.head = block / a.parts;
-    p.part = block - p.head * a.parts;
+    const int head_block = block / a.parts;
+    p.part = block - head_block * a.parts;
+    p.block_head = head_block * a.block_heads;
     const int tid = threadIdx.x;
     p.group = tid / a.tx;
     p.tx = tid - p.group * a.tx;
@@ -534,10 +539,14 @@ __device__ __forceinline__ Place place_of(const RecurrenceArgs& a) {
     if (!p.there) p.group = 0;
     p.entry = a.shuffle ? tid >> 5 : p.group;
     p.row0 = p.group * L;
-    const int c = (p.part * a.tx + p.tx) * V;
-    p.active = p.there && c < a.per_head;
+    const int within = p.tx / a.head_threads, lane = p.tx - within * a.head_threads;
+    const int c = (p.part * a.head_threads + lane) * V;
+    p.head = p.block_head + within;
     p.channel = p.head * a.per_head + c;
-    p.read_channel = p.active ? p.channel : p.head * a.per_head;
+    p.active = p.there && c < a.per_head && p.channel < a.channels;
+    p.leads = lane == 0 && p.active;
+    p.read_channel = p.active ? p.channel : p.block_head * a.per_head;
+    if (p.channel >= a.channels) p.head = p.block_head;   // its gates are read and not used
     return p;
 }
 
@@ -862,7 +871,7 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
     identity(all);
     if (APPLY) carry_of_segment<true>(a, p, sh[0], carry);
     Borders<true, L> borders;
-    borders.begin(a, p.chain, t0 * tile_rows, reinterpret_cast<int*>(s_raw + STAGES * sizeof(Ring)), V, p.head, p.part);
+    borders.begin(a, p.chain, t0 * tile_rows, reinterpret_cast<int*>(s_raw + STAGES * sizeof(Ring)), V, p.block_head, p.part);
     T gate_now[L], gate_next[L];
     // Fetches tile t, the next of the walk, into the stage `fetched` and moves on; tiles without rows of a sequence are only
     // passed.
@@ -1064,7 +1073,7 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
     identity(all);
     if (APPLY) carry_of_segment<false>(a, p, sh[0], q_carry);
     Borders<false, L> borders;
-    borders.begin(a, p.chain, (t1 - 1) * tile_rows, reinterpret_cast<int*>(s_zeros + (a.v_h ? 0 : kTensor)), V, p.head, p.part);
+    borders.begin(a, p.chain, (t1 - 1) * tile_rows, reinterpret_cast<int*>(s_zeros + (a.v_h ? 0 : kTensor)), V, p.block_head, p.part);
     T gate_now[L], gate_next[L];
     int fetched = 0;       // as in the forward
     auto fetch = [&](int t) {
@@ -1163,7 +1172,7 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                 if (want_x) store_zero_rows<T, V, L>(to_x, a.h_stride, left);
                 if (want_gate) store_zero_rows<T, V, L>(to_gate, a.gate_out_stride, left);
             }
-            if (APPLY && SHARED && a.v_gate && p.there && p.tx == 0)
+            if (APPLY && SHARED && a.v_gate && p.leads)
                 for (int l = 0; l < left; ++l) store_gate_sum(l, 0.f);
             __syncthreads();
             if (FLAT) {
@@ -1296,8 +1305,8 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
                     }
                 } else if (a.v_gate) {
                     sum = p.active && !outside ? sum * slope[0] : 0.f;   // whatever lies in the gates of rows outside
-                    for (int off = a.tx >> 1; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-                    if (p.there && p.tx == 0 && (PLAIN || l < left)) store_gate_sum(l, sum);
+                    for (int off = a.head_threads >> 1; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                    if (p.leads && (PLAIN || l < left)) store_gate_sum(l, sum);
                 }
             }
         };

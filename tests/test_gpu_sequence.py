@@ -176,6 +176,19 @@ def test_only_the_last_state_of_long_wide_rows(d, dtype):
         check("packed", [1, 4000, 0, 40, 4959], 9000, d, d, dtype=dtype, final_only=True, reverse=reverse)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("d, heads", [(10, 5), (18, 9), (21, 7), (78, 26), (99, 33), (35, 7), (36, 3), (80, 5), (68, 17), (14, 2), (108, 9)])
+def test_many_narrow_heads(d, heads, dtype):
+    """Several heads in a block, the last block's not all there; cut into segments and not."""
+    for reverse in (False, True):
+        kw = dict(dtype=dtype, reverse=reverse, coupled=dtype == "bf16", form="decay" if reverse else "logit")
+        check("dense", [90] * 2, 90, d, heads, **kw)
+        check("dense", [7000], 7000, d, heads, **kw)
+        check("packed", [1, 3000, 0, 0, 40, 1, 800, 13], 3900, d, heads, outside_gate="nan", **kw)
+        check("padded", [0, 2500, 37, 1], 2500, d, heads, outside_gate="nan", **kw)
+        check("packed", [1] * 400 + [0] * 300 + [200], 700, d, heads, final_only=True, **kw)
+
+
 def test_more_borders_in_a_tile_than_threads_look_at_once():
     for reverse in (False, True):
         check("packed", [1] * 2500, 2600, 1, 1, reverse=reverse)
