@@ -294,7 +294,7 @@ struct Borders {
     }
     __device__ void begin(const RecurrenceArgs& a, int chain, int p0, int* s_tables, int lanes, int block_head, int part) {
         channel = block_head * a.per_head + part * a.tx * lanes;
-        channels = a.block_heads > 1 ? min(a.block_heads * a.per_head, a.channels - channel) : min(a.tx * lanes, a.per_head - part * a.tx * lanes);
+        channels = min(a.tx * lanes, a.channels - channel);
         tables = s_tables;
         groups = a.groups;
         tile_rows = groups * L;
@@ -521,7 +521,7 @@ struct Place {
     bool leads;            // the first thread of a head
     int read_channel;      // what to read all the same where a thread has no channel
 };
-template <int V, int L>
+template <int V, int L, bool SHARED>
 __device__ __forceinline__ Place place_of(const RecurrenceArgs& a) {
     Place p;
     const int blocks = a.head_blocks * a.parts;
@@ -539,14 +539,25 @@ __device__ __forceinline__ Place place_of(const RecurrenceArgs& a) {
     if (!p.there) p.group = 0;
     p.entry = a.shuffle ? tid >> 5 : p.group;
     p.row0 = p.group * L;
-    const int within = p.tx / a.head_threads, lane = p.tx - within * a.head_threads;
-    const int c = (p.part * a.head_threads + lane) * V;
-    p.head = p.block_head + within;
-    p.channel = p.head * a.per_head + c;
-    p.active = p.there && c < a.per_head && p.channel < a.channels;
-    p.leads = lane == 0 && p.active;
-    p.read_channel = p.active ? p.channel : p.block_head * a.per_head;
-    if (p.channel >= a.channels) p.head = p.block_head;   // its gates are read and not used
+    // Without shared gates the same arithmetic with one head: any shorter form of it made the coupled backward of four 16-bit
+    // channels a thread spill 130 bytes (8 x 4096 x 2560, a training pass: 348 -> 392 us).
+    if (SHARED) {
+        const int within = p.tx / a.head_threads, lane = p.tx - within * a.head_threads;
+        const int c = (p.part * a.head_threads + lane) * V;
+        p.head = p.block_head + within;
+        p.channel = p.head * a.per_head + c;
+        p.active = p.there && c < a.per_head && p.channel < a.channels;
+        p.leads = lane == 0 && p.active;
+        p.read_channel = p.active ? p.channel : p.block_head * a.per_head;
+        if (p.channel >= a.channels) p.head = p.block_head;   // its gates are read and not used
+    } else {
+        const int c = (p.part * a.tx + p.tx) * V;
+        p.head = p.block_head;
+        p.active = p.there && c < a.per_head;
+        p.leads = false;
+        p.channel = p.head * a.per_head + c;
+        p.read_channel = p.active ? p.channel : p.head * a.per_head;
+    }
     return p;
 }
 
@@ -853,7 +864,7 @@ recurrence_forward_kernel(const RecurrenceArgs a) {
     Ring* ring = reinterpret_cast<Ring*>(s_raw);
     __shared__ TileMaps<V, A> sh[2];
     const int tile_rows = a.groups * L;
-    const Place p = place_of<V, L>(a);
+    const Place p = place_of<V, L, SHARED>(a);
     int t0 = p.segment * a.segment_tiles, t1 = min(t0 + a.segment_tiles, a.tiles);
     if (!APPLY) narrow_to_map<true>(a, tile_rows, t0, t1);
     const char* x = row_pointer<T>(static_cast<const char*>(a.x), p.read_channel, a.x_stride, a, p, t0, tile_rows);
@@ -1052,7 +1063,7 @@ recurrence_backward_kernel(const RecurrenceArgs a) {
     unsigned char* s_zeros = s_raw + STAGES * stage_bytes;
     __shared__ TileMaps<V, A> sh[2];
     const int tile_rows = a.groups * L;
-    const Place p = place_of<V, L>(a);
+    const Place p = place_of<V, L, SHARED>(a);
     int t0 = p.segment * a.segment_tiles, t1 = min(t0 + a.segment_tiles, a.tiles);
     if (!APPLY) narrow_to_map<false>(a, tile_rows, t0, t1);
     const char* vh = row_pointer<T>(static_cast<const char*>(a.v_h), p.read_channel, a.v_h_stride, a, p, t1 - 1, tile_rows);
