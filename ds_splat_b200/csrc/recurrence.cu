@@ -147,12 +147,15 @@ Layout layout_of(const DsbRecurrence& s) {
     };
     Layout best = {};
     if (wide <= 8) {   // vec 3 among them: one thread per row
-        // Narrow heads lie side by side in a block until a row's piece fills two sectors; a head alone in a block would read a
-        // sector a row for a few bytes (29 x 3642 rows of 112 fp16 heads of 3 channels, a training pass: 670 us then, 401 so;
-        // 56528 packed rows of 106 bf16 heads of 3, the forward alone: 192 and 130).
+        // Narrow heads lie side by side in a block: a head alone in one would read a sector a row for a few bytes (29 x 3642 rows
+        // of 112 fp16 heads of 3 channels, a training pass: 670 us then, 401 so).  As many as a row's piece needs to fill a line
+        // of 128 bytes while eight threads a row are enough, so that warps compose their maps by themselves; with more threads,
+        // two sectors have to do.  On the device, 8 x 4096 x 1024: 64 bf16 heads of 16 at 32 / 64 / 128 bytes, which takes 4 / 8 /
+        // 16 threads, 170 / 121 / 170 us; 128 fp32 heads of 8 at 32 / 64 / 128 bytes, 2 / 4 / 8 threads, 301 / 205 / 164.
         int tx = 1;
         while (tx < wide) tx *= 2;
-        while (shared && tx <= 16 && l.block_heads < s.gate_heads && l.block_heads * l.per_head * dtype_bytes(s.dtype) < 64) {
+        while (shared && tx <= 16 && l.block_heads < s.gate_heads &&
+               l.block_heads * l.per_head * dtype_bytes(s.dtype) < (tx < 8 ? 128 : 64)) {
             l.block_heads *= 2;
             tx *= 2;
         }
