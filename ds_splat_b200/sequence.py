@@ -71,6 +71,18 @@ def _rows(t: torch.Tensor, lanes: int):
     return t.clone(memory_format=torch.contiguous_format), width
 
 
+def _flat_as(t: torch.Tensor, stride: int, flat: bool):
+    """``_rows``'s pair for rows that lie one behind the other exactly when ``flat``."""
+    width = t.shape[-1]
+    if (stride == width) == flat:
+        return t, stride
+    if flat:
+        return t.clone(memory_format=torch.contiguous_format), width
+    apart = torch.empty((t.numel() // width, width + 1), dtype=t.dtype, device=t.device)
+    apart[:, :width] = t.reshape(-1, width)
+    return apart, width + 1
+
+
 def _state(t: Optional[torch.Tensor], shape, device, name):
     if t is None:
         return None
@@ -147,8 +159,42 @@ class _Call:
             _capi.check(rc)
         return h, last, checkpoints
 
-    def run_backward(self, x, gate, state, checkpoints, v_h, v_last, need):
-        lib, dev, d = _capi.lib(), x.device, x.shape[-1]
+    def as_handed_out(self, x, gate, state, checkpoints, borders, dev):
+        """(x, gate, state, checkpoints, borders, DsbRecurrence) of a backward pass.  Hooks on saved tensors (activation checkpointing,
+        offloading) hand out others than those that were saved: at other addresses, and laid out otherwise."""
+        s = self.shape
+        for t, name, width in ((x, "x", s.channels), (gate, "gate", s.gate_heads)):
+            _require(t, name, dev, x.dtype)
+            if t.shape[-1] != width or t.numel() != s.rows * width or _capi.DTYPES.get(t.dtype) != s.dtype:
+                raise RuntimeError(f"a hook handed out a {name} of another shape or type than was saved")
+        x, x_stride = _rows(x, self.lanes)
+        gate, gate_stride = _rows(gate, self.lanes if s.gate_heads == s.channels else 1)
+        if s.channels == 3:     # whether rows of three are contiguous decides the cut, and with it what the checkpoints are of
+            x, x_stride = _flat_as(x, x_stride, s.x_stride == 3)
+            if s.gate_heads == 3:
+                gate, gate_stride = _flat_as(gate, gate_stride, s.gate_stride == 3)
+        state = _state(state, (self.sequences, s.channels), dev, "state")
+        _require(checkpoints, "the saved states", dev, torch.uint8)
+        if checkpoints.numel() != self.sizes[1]:
+            raise RuntimeError("a hook handed out something else than was saved")
+        if not checkpoints.is_contiguous() or checkpoints.data_ptr() % 16:
+            checkpoints = checkpoints.clone(memory_format=torch.contiguous_format)
+        shape = type(s).from_buffer_copy(s)
+        shape.x_stride, shape.gate_stride = x_stride, gate_stride
+        if borders is not None:
+            packed = s.sequence_rows == 0
+            _require(borders, "offsets" if packed else "lengths", dev, torch.int32)
+            if borders.numel() != self.sequences + packed:
+                raise RuntimeError("a hook handed out something else than was saved")
+            borders = borders.contiguous()
+            shape.offsets, shape.lengths = (borders.data_ptr(), None) if packed else (None, borders.data_ptr())
+        return x, gate, state, checkpoints, borders, shape
+
+    def run_backward(self, x, gate, state, checkpoints, borders, v_h, v_last, need):
+        lib, dev, d = _capi.lib(), (v_h if v_last is None else v_last).device, x.shape[-1]
+        v_x = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
+        v_gate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if need[1] else None
+        x, gate, state, checkpoints, borders, shape = self.as_handed_out(x, gate, state, checkpoints, borders, dev)
         if v_h is None:
             v_h_stride = d
         elif d == 3:
@@ -156,13 +202,11 @@ class _Call:
         else:
             v_h, v_h_stride = _rows(v_h, self.lanes)
         v_last = _state(v_last, (self.sequences, d), dev, "the last state's gradient")
-        v_x = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
-        v_gate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if need[1] else None
         v_state = torch.empty((self.sequences, d), dtype=torch.float32, device=dev) if need[2] else None
         workspace_bytes = self.sizes[0]
         workspace = torch.empty(workspace_bytes, dtype=torch.uint8, device=dev) if workspace_bytes else None
         rc = lib.dsb_recurrence_backward(
-            self.ref, x.data_ptr(), gate.data_ptr(), _capi.ptr(state), _capi.ptr(checkpoints), _capi.ptr(v_h), v_h_stride,
+            C.byref(shape), x.data_ptr(), gate.data_ptr(), _capi.ptr(state), checkpoints.data_ptr(), _capi.ptr(v_h), v_h_stride,
             _capi.ptr(v_last), _capi.ptr(v_x), _capi.ptr(v_gate), _capi.ptr(v_state), _capi.ptr(workspace), workspace_bytes,
             _raw_stream(dev.index))
         if rc:
@@ -171,7 +215,7 @@ class _Call:
 
 
 class _GatedRecurrence(torch.autograd.Function):
-    """Over (x, gate, state) and a ``_Call`` with the offsets or lengths it points at."""
+    """Over (x, gate, state), a ``_Call`` and the offsets or lengths its forward points at."""
 
     @staticmethod
     def forward(ctx, x, gate, state, call, borders):
@@ -185,11 +229,12 @@ class _GatedRecurrence(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
-        x, gate, state, checkpoints, _ = ctx.saved_tensors
+        x, gate, state, checkpoints, borders = ctx.saved_tensors
         v_h, v_last = (None, grads[0]) if len(grads) == 1 else grads
         if v_h is None and v_last is None:
             return (None,) * 5
-        v = _on(x.device, ctx.call.run_backward, x, gate, state, checkpoints, v_h, v_last, ctx.needs_input_grad)
+        v = _on((v_h if v_last is None else v_last).device, ctx.call.run_backward, x, gate, state, checkpoints, borders, v_h, v_last,
+                ctx.needs_input_grad)
         return (*v, None, None)
 
 
@@ -211,7 +256,8 @@ def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, state: Optional[torch.
     final_only  return ``(None, last)`` and do not write ``h``.
 
     Rows that belong to no sequence come back as zeros, their gradients too; a sequence of no rows hands its state on.
-    Kept for the backward pass: the inputs, and a float32 state per channel and 3 to 12 rows.  No call waits for the device;
+    Kept for the backward pass: the inputs, and a float32 state per channel and 3 to 12 rows, all of them as saved tensors,
+    so that activation checkpointing and hooks that offload them work.  No call waits for the device;
     a training step can be captured into a graph (as always with torch, while no eager graph of the same leaves lives).
     Offsets and lengths live on the device and are not read back: values out of order or range make the results invalid and
     are reported by ``dsb_take_device_status`` and by the rasterizer's calls that synchronise."""
