@@ -14,6 +14,21 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (run on the B200 box)")
 
 
+# Comparisons with the reference's own kernels (test_gpu_reference.py) that carry no mark of their own.
+REFERENCE_COMPARISONS = {"test_background_term_of_the_backward_against_reference_cuda", "test_scale_modifier_against_reference_cuda"}
+
+
+def pytest_collection_modifyitems(items):
+    """Skips them where the reference's kernels were not built and could not be.  With the sources there, a missing library is a
+    failed build, and they fail."""
+    from oracle import ref_cuda
+    if ref_cuda.available() or ref_cuda.reference_root():
+        return
+    for item in items:
+        if item.path.name == "test_gpu_reference.py" and getattr(item, "originalname", None) in REFERENCE_COMPARISONS:
+            item.add_marker(pytest.mark.skip(reason="oracle/_ref/libref_splat.so not built"))
+
+
 def oracle_camera(view, sh_degree=3, max_sh_degree=3, bg=(0.0, 0.0, 0.0)):
     from oracle import oracle as O
     return O.Camera(view=view.view, proj=view.proj, campos=view.campos, tanfovx=view.tanfovx, tanfovy=view.tanfovy,
