@@ -139,14 +139,16 @@ __device__ __forceinline__ void add(float (&r)[V], const float (&a)[A], const fl
 // A gate is kept as one register: a decay as itself, a logit g as e = exp(-g), from which f = 1 / (1 + e) and 1 - f = e f
 // follow with full relative precision however close to 0 or 1 they are.  e is kept below 2^126, where 1 / (1 + e) is still a
 // normal number (1.2e-38); a NaN stays one.
-// Errors, with u = 2^-24 and L = log2 e: 2^x by the hardware 4 u, its argument's rounding |g| 1.2 u, the quotient 2 u, 1 + e and
-// the product u each.  32-bit gates get the argument's rounding error back to first order (three instructions more).
+// Errors relative to f and to 1 - f, with u = 2^-24: 2^x by the hardware 4 u, the quotient 2 u, 1 + e and the product u each, and up
+// to 1.22 |g| u by the argument g log2 e (its rounding u, the constant's own 0.22 u).  16-bit gates are left with that: at most
+// 2^-17, where half a step of their type is 2^-11 or 2^-8.  32-bit gates get it back to first order from the product's and the
+// constant's rests, four instructions and one rounding more: 9 u in all for |g| <= 87; beyond, e keeps its value at 87.
 template <typename T, bool LOGIT, int A>
 __device__ __forceinline__ void gate_registers(const Pack<T, A>& gate, float (&e)[A]) {
     float g[A];
 #pragma unroll
     for (int v = 0; v < A; ++v) g[v] = to_float(gate.e[v]);
-    constexpr float kLog2e = 1.44269502f, kLn2 = 0.693147181f;
+    constexpr float kLog2e = 1.44269502f, kLog2eRest = 1.92596299e-8f, kLn2 = 0.693147181f;
     if constexpr (!LOGIT) {
 #pragma unroll
         for (int v = 0; v < A; ++v) e[v] = g[v];
@@ -155,7 +157,7 @@ __device__ __forceinline__ void gate_registers(const Pack<T, A>& gate, float (&e
         for (int v = 0; v < A; ++v) {
             float y;
             asm("{\n\t.reg .f32 t;\n\tmin.NaN.f32 t, %1, 0f42AE0000;\n\tmax.NaN.f32 %0, t, 0fC2AE0000;\n\t}" : "=f"(y) : "f"(-g[v]));   // +-87
-            const float hi = y * kLog2e, lo = fmaf(y, kLog2e, -hi);
+            const float hi = y * kLog2e, lo = fmaf(y, kLog2eRest, fmaf(y, kLog2e, -hi));
             asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[v]) : "f"(hi));
             e[v] = fmaf(e[v], lo * kLn2, e[v]);
         }

@@ -249,8 +249,9 @@ def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, state: Optional[torch.
              sequence b.  [N, D] with ``offsets`` (int32 [S + 1], nondecreasing, within [0, N]): sequence s is rows
              ``offsets[s] .. offsets[s + 1]`` (a tile's ``ranges`` of the rasterizer are such offsets).  At most 2^31 - 2^16 rows.
     gate     x's shape with H for D: each of the H gates of a row is shared by D / H consecutive channels.  As logits
-             (``form="logit"``) decays near 1 keep their precision in 16-bit types; as ``"decay"`` they are taken as they
-             are and are meant to lie in [-1, 1].
+             (``form="logit"``) decays near 1 keep their precision in 16-bit types (f and 1 - f are each good to 9 * 2^-24 of
+             themselves, with 16-bit logits to (9 + 1.22 |gate|) * 2^-24; a logit beyond +-87 counts as +-87); as
+             ``"decay"`` they are taken as they are and are meant to lie in [-1, 1].
     state    float32 [S, D], each sequence's state before its first row; None = zeros.
     reverse  run from each sequence's last row to its first (``last`` is then the state after the first row).
     final_only  return ``(None, last)`` and do not write ``h``.

@@ -471,7 +471,8 @@ int dsb_adam_step(float* params, const float* grads, float* exp_avg, float* exp_
 /* Gated linear recurrence over depth-ordered lists or any other sequences, per channel:
  *     f_t = gate_t (DSB_GATE_DECAY) or 1 / (1 + exp(-gate_t)) (DSB_GATE_LOGIT)
  *     h_t = f_t h_{t-1} + x_t,   or with `coupled`   h_t = f_t h_{t-1} + (1 - f_t) x_t
- * from h_{-1} = state_in (zeros when NULL) to state_out = the last h, over each of `sequences` sequences.  The blend of
+ * (f and 1 - f are each good to 9 * 2^-24 of themselves, to (9 + 1.22 |gate|) * 2^-24 with 16-bit logits; a logit beyond +-87
+ * counts as +-87) from h_{-1} = state_in (zeros when NULL) to state_out = the last h, over each of `sequences` sequences.  The blend of
  * dsb_blend_forward is the coupled form run back to front (`reverse`) with gate 1 - alpha shared by the colour
  * channels; this entry takes any number of channels and any lists, a tile's `ranges` among them.
  *

@@ -9,9 +9,11 @@ because each row's share passes through at most one rounding per row between it 
 import numpy as np
 
 U = 2.0 ** -24
-# Roundings a row adds, in units of u, over its product f h and its input i together.  A logit's gate: the exponential 5
-# (2 ulp = 4 u, its argument 1), the sum 1 + t up to 3.5 of the result, the quotient 1, the product 1: 10.5; 1 - f at most
-# 11 more relative to f >= 1/2.  The input's product 1, the fused multiply-add 1, the two of the grouping's products.
+# Roundings a row adds, in units of u, relative to its product f h and to its input i.  A logit's gate: the exponential 5
+# (2 ulp = 4 u, its argument's correction 1), the sum 1 + e 1, the reciprocal 2 (1 ulp), the product e f of 1 - f 1: 9.  The
+# input's product 1, the fused multiply-add 1, the two of the grouping's products: 13.
+# 16-bit logits are not corrected: 1.22 |g| more.  The 3 that are left cover |g| <= 2.4; callers double the bound, which covers
+# |g| <= 15.  Beyond that the gates by themselves are what to compare.
 ROW = 16.0
 
 
