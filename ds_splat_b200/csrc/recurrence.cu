@@ -23,6 +23,7 @@ template <> int run_recurrence_backward<__nv_bfloat16>(const RecurrenceLaunch&, 
 namespace {
 
 constexpr long long kMaxRows = (1ll << 31) - (1 << 16);   // positions are 32-bit, the last tile's end included
+constexpr int kMaxChannels = (int)kMaxRows;               // and so are channels, with those of threads beyond the last
 constexpr long long kMaxBlocks = (1ll << 31) - 1;
 
 // v_gate = sum of the channel blocks' shares of it, in their order
@@ -93,6 +94,7 @@ int check_shape(const DsbRecurrence& s, bool step) {
     DSB_REQUIRE(s.gate_form == DSB_GATE_DECAY || s.gate_form == DSB_GATE_LOGIT, "recurrence: unknown gate form %d", s.gate_form);
     DSB_REQUIRE(s.channels >= 1 && s.gate_heads >= 1 && s.channels % s.gate_heads == 0,
                 "recurrence: %d channels do not split into %d gate heads", s.channels, s.gate_heads);
+    DSB_REQUIRE(s.channels <= kMaxChannels, "recurrence: at most 2^31 - 2^16 channels, got %d", s.channels);
     DSB_REQUIRE(s.rows >= 0 && s.rows <= kMaxRows, "recurrence: at most 2^31 - 2^16 rows, got %lld", (long long)s.rows);
     DSB_REQUIRE(s.sequences >= 0, "recurrence: negative number of sequences");
     if (step) {

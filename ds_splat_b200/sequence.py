@@ -30,6 +30,8 @@ from torch._C import _cuda_getCurrentRawStream as _raw_stream   # the current st
 
 from . import _capi
 
+MAX_CHANNELS = (1 << 31) - (1 << 16)   # as the library's
+
 
 def _on(device, call, *args):
     """``call(*args)`` with ``device`` current (the library launches on the current device)."""
@@ -108,8 +110,8 @@ def _check_gate(x, gate, form):
         d, heads = x.shape[-1], gate.shape[-1]
         if heads < 1 or d % heads != 0:
             raise ValueError(f"{d} channels do not split into {heads} gate heads")
-    elif x.shape[-1] < 1:
-        raise ValueError("x must have a channel at least")
+    if not 1 <= x.shape[-1] <= MAX_CHANNELS:
+        raise ValueError(f"x must have 1 to 2^31 - 2^16 channels, got {x.shape[-1]}")
 
 
 _sizes = {}     # (workspace, checkpoint) bytes by what they follow from
@@ -121,6 +123,8 @@ class _Call:
     __slots__ = ("shape", "ref", "lanes", "x", "gate", "sequences", "final_only", "sizes")
 
     def __init__(self, x, gate, sequences, sequence_rows, form, coupled, reverse, offsets, lengths, final_only=False):
+        if sequences >= 1 << 31:
+            raise ValueError(f"at most 2^31 - 1 sequences, got {sequences}")
         d, heads = x.shape[-1], gate.shape[-1]
         together = d // heads if heads != d else d
         self.lanes = lanes = 4 if together % 4 == 0 else 2 if together % 2 == 0 else 1
@@ -247,7 +251,8 @@ def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, state: Optional[torch.
 
     x        [B, T, D]: B sequences of T rows; with ``lengths`` (int32 [B]) only the first ``lengths[b]`` of them belong to
              sequence b.  [N, D] with ``offsets`` (int32 [S + 1], nondecreasing, within [0, N]): sequence s is rows
-             ``offsets[s] .. offsets[s + 1]`` (a tile's ``ranges`` of the rasterizer are such offsets).  At most 2^31 - 2^16 rows.
+             ``offsets[s] .. offsets[s + 1]`` (a tile's ``ranges`` of the rasterizer are such offsets).  At most 2^31 - 2^16
+             rows, as many channels, and 2^31 - 1 sequences.
     gate     x's shape with H for D: each of the H gates of a row is shared by D / H consecutive channels.  As logits
              (``form="logit"``) decays near 1 keep their precision in 16-bit types (f and 1 - f are each good to 9 * 2^-24 of
              themselves, with 16-bit logits to (9 + 1.22 |gate|) * 2^-24; a logit beyond +-87 counts as +-87); as

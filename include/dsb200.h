@@ -479,7 +479,8 @@ int dsb_adam_step(float* params, const float* grads, float* exp_avg, float* exp_
  * Rows: x and h are [rows][channels], gate is [rows][gate_heads]; each head's gate is shared by channels / gate_heads
  * consecutive channels.  Rows are x_stride / gate_stride elements apart; h and the gradients are contiguous.  Where the
  * channels that share a gate (all of them when each has its own) are a multiple of four (two), every row of x, h, the
- * states, the gradients and per-channel gates starts on a boundary of four (two) elements.  At most 2^31 - 2^16 rows.
+ * states, the gradients and per-channel gates starts on a boundary of four (two) elements.  At most 2^31 - 2^16 rows and
+ * as many channels.
  *   sequence_rows > 0: sequence s is rows s * sequence_rows ..., rows == sequences * sequence_rows; with `lengths`
  *                      (int32 per sequence on the device) only its first lengths[s] rows belong to it.
  *   sequence_rows == 0: packed; sequence s is rows [offsets[s], offsets[s+1]) (int32 on the device, nondecreasing,
