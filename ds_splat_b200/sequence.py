@@ -26,7 +26,10 @@ import ctypes as C
 from typing import Optional, Tuple, Union
 
 import torch
-from torch._C import _cuda_getCurrentRawStream as _raw_stream   # the current stream's handle without an object around it
+try:
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream   # the current stream's handle without an object around it
+except ImportError:        # a torch without CUDA: the entry points refuse its tensors before they ask for a stream
+    _raw_stream = None
 
 from . import _capi
 
