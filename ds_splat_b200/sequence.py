@@ -265,6 +265,8 @@ def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, state: Optional[torch.
     final_only  return ``(None, last)`` and do not write ``h``.
 
     Rows that belong to no sequence come back as zeros, their gradients too; a sequence of no rows hands its state on.
+    What is not finite stays so to the end of its sequence and reaches no other sequence or channel; an infinity may become a
+    NaN where the decays after it have a product below 2^-126.  Values below 2^-126 may count as zero.
     Kept for the backward pass: the inputs, and a float32 state per channel and 3 to 12 rows, all of them as saved tensors,
     so that activation checkpointing and hooks that offload them work.  No call waits for the device;
     a training step can be captured into a graph (as always with torch, while no eager graph of the same leaves lives).
@@ -370,10 +372,11 @@ def dropout(x: torch.Tensor, p: float, rng: Union[Tuple[int, int], torch.Tensor]
 
     rng  the pair (seed, step), each within [0, 2^64): one seed per place in a model, one step per training step.  Or an
          int64 CUDA tensor of two elements holding them, read when the kernel runs: a captured graph draws a new mask at
-         every replay when the tensor is advanced between (or inside) the replays.
+         every replay when the tensor is advanced between (or inside) the replays.  Where activation checkpointing runs a block
+         a second time, the tensor is read a second time: advance it after the backward pass, or give the pair as numbers.
     residual  a tensor of x's shape and type to add.
 
-    Dropped elements leave no trace of what they held; p = 1 drops everything."""
+    Dropped elements leave no trace of what they held; p = 1 drops everything.  Values below 2^-126 may count as zero."""
     _require(x, "x")
     if x.dtype not in _capi.DTYPES:
         raise RuntimeError(f"x must be float32, float16 or bfloat16, got {x.dtype}")

@@ -489,7 +489,9 @@ int dsb_adam_step(float* params, const float* grads, float* exp_avg, float* exp_
  * A sequence of no rows hands its state on.  Offsets or lengths out of order or range keep every access in bounds and
  * are reported through the device status word (DSB_ERR_INVALID_ARGUMENT); the results are then not valid.
  * States and their gradients are float [sequences][channels].  Decays are meant to lie in [-1, 1]: the scan forms
- * products of a sequence's decays, which overflow where the sequence itself would not if many of them are larger.
+ * products of a sequence's decays, which overflow where the sequence itself would not if many of them are larger.  What is
+ * not finite stays so to the end of its sequence and reaches no other sequence or channel, but an infinity may become a NaN
+ * where the decays after it have a product below 2^-126.  Values below 2^-126 may count as zero.
  *
  * checkpoints (dsb_recurrence_checkpoint_bytes: a float per channel and group of 3 to 12 rows; NULL when no backward
  * follows) receives the states that the backward starts from; the backward of a call gets the same shape, strides
@@ -526,7 +528,7 @@ int dsb_recurrence_step(const DsbRecurrence* shape, const void* x, const void* g
 /* Dropout from a counter-based generator; the mask is not stored, the backward is the same call on the gradient:
  *     out_i = [residual_i +] (word_i >= round(p * 2^32) ? x_i / (1 - p) : 0)
  * with word_i = word (i mod 4) of Philox4x32-10 under the key `seed` and the counter (i div 4, step), i = row * cols +
- * col.  residual may be NULL; out may be x or residual.  rng: NULL, or two int64 on the device (seed, step) that
+ * col.  Values below 2^-126 may count as zero.  residual may be NULL; out may be x or residual.  rng: NULL, or two int64 on the device (seed, step) that
  * replace the arguments, so that a captured graph draws a new mask when they change; rng_used (may be NULL) then
  * receives the pair that was used. */
 int dsb_dropout(const void* x, const void* residual, void* out, int64_t rows, int64_t cols, int64_t x_stride,

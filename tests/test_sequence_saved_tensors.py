@@ -227,3 +227,23 @@ def test_gradients_do_not_depend_on_where_saved_tensors_have_been(how, layout, s
     for name, a, b in zip(("dx", "dgate", "dstate"), got, want):
         assert torch.equal(a, b), name
     assert _capi.take_device_status() == 0 and junk
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pair", ["numbers", "tensor"])
+def test_dropout_in_a_checkpointed_block_draws_the_same_mask_again(pair):
+    """The block runs twice.  A pair that lives on the device is read both times: it is advanced after the backward pass."""
+    x = torch.randn(2, 500, 32, device="cuda", requires_grad=True)
+    gate = torch.randn(2, 500, 32, device="cuda", requires_grad=True)
+    rng = (7, 9) if pair == "numbers" else torch.tensor([7, 9], dtype=torch.int64, device="cuda")
+    v = torch.randn(2, 500, 32, device="cuda")
+
+    def block(x, gate):
+        h = ds.dropout(ds.gated_recurrence(x, gate, coupled=True)[0], 0.3, rng, residual=x)
+        return h * torch.sigmoid(h)                        # its own backward pass takes the recomputed h
+
+    want_out = block(x, gate)
+    want = torch.autograd.grad(want_out, (x, gate), v)
+    out = checkpoint(block, x, gate, use_reentrant=False)
+    got = torch.autograd.grad(out, (x, gate), v)
+    assert torch.equal(out, want_out) and all(torch.equal(a, b) for a, b in zip(got, want))
