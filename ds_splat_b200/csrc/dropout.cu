@@ -56,9 +56,10 @@ __device__ __forceinline__ void philox_words_at(u64 first_block, u32 step_lo, u3
 // Each thread takes V consecutive elements a trip (V a multiple of 4: whole counter blocks).  VEC: they lie in one row, at
 // addresses that allow one transaction; else every element finds its own row.  The loads of a trip are issued before its
 // random words are worked out.  What bounds it, on tensors of 168 MB: with 32-bit ones memory (77 us with a residual, 59 without,
-// 1.0 and 0.87 of the copy rate); with 16-bit ones, twice the elements, the generator (87 and 85 us, with and without):
-// five 32 x 32 -> 64 bit products an element, which the multiplier takes four cycles each for.  Six blocks an SM (40
-// registers) were the fastest of 4, 6 and 8; one trip per thread instead of a few loses a fifth.
+// 1.0 and 0.87 of the copy rate).  With 16-bit ones, twice the elements, 85 us with and without: the generator, in 22 instructions an
+// element, but no unit of the GPU is full.  Issue slots are busy for 64% of the time; the five 32 x 32 -> 64 bit products an
+// element, at four cycles each, keep the multiplier busy for half of it (45 us); DRAM 33% (58% with a residual).  Six blocks an SM
+// (40 registers) were the fastest of 4, 6 and 8; one trip per thread instead of a few loses a fifth.
 template <typename T, int V, bool VEC, bool RESIDUAL>
 __global__ void __launch_bounds__(kThreads, 6)
 dropout_kernel(const T* x, const T* residual, T* out, const DropoutArgs a) {

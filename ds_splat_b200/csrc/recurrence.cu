@@ -85,6 +85,10 @@ struct Layout {            // how a call is cut; the same for the forward and th
     int64_t chains, chain_rows, tiles;     // tiles of a chain
     int64_t segments, segment_tiles;       // of a chain
 };
+// Two blocks are what registers allow an SM, and shared memory too but for some calls with one thread a row, whose 256 groups make
+// large border tables: a single 32-bit channel (81 KB of tables; 36 to 72 KB of stages in the backward, 48 in the forward with a
+// gate of its own) and three with gates of their own (39 KB; 90 and 135 KB of stages).  Those run one block an SM, and where they
+// are cut, twice the segments that run at once.
 constexpr int kSms = 148, kBlocksPerSm = 2;
 // A chain of fewer tiles is not cut: a tile after another takes a block about 2 us, a second launch and its first tile 6 us.
 constexpr int kLeastTilesToCut = 8;

@@ -27,8 +27,8 @@
 //   walking with the state in registers                                                                 1177
 //   code of its own for tiles without a border ("plain"), gate forms compiled in, states per row group   650
 //   gates kept as exp(-g): f and 1 - f from it in three instructions, without branches                   477
-//   two channels an instruction, no register spills (L chosen for 128 registers; every spill cost more
-//   than the occupancy it bought)                                                                        327
+//   two channels an instruction, registers not spilled (L chosen for 128 registers; every large spill cost
+//   more than the occupancy it bought; 8 to 12 bytes a thread remain in six 16-bit backward kernels)     327
 //   blocks of 256 threads with as many threads a row as make two blocks an SM, maps through shared
 //   memory: the same here, but 0.9 to 0.75 of the time with padded, packed and narrow sequences          340
 // Tried and slower: three or four stages of prefetch (fewer blocks), 128 threads (row pieces below two sectors), every thread
