@@ -496,7 +496,8 @@ int dsb_adam_step(float* params, const float* grads, float* exp_avg, float* exp_
  * checkpoints (dsb_recurrence_checkpoint_bytes: a float per channel and group of 3 to 12 rows; NULL when no backward
  * follows) receives the states that the backward starts from; the backward of a call gets the same shape, strides
  * included, and nothing else is kept.  workspace: dsb_recurrence_workspace_bytes, for either direction, free again when
- * the call's work is done; calls that overlap need one each.  Both are 16-byte aligned.  No call synchronises, and no
+ * the call's work is done; calls that overlap need one each.  Both are 16-byte aligned.  Results overlap neither inputs
+ * nor one another.  No call synchronises, and no
  * kernel waits for another block.  Results do not depend on timing: the same call gives the same bits. */
 #define DSB_GATE_DECAY 0
 #define DSB_GATE_LOGIT 1
