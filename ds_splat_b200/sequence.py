@@ -120,10 +120,15 @@ def _check_gate(x, gate, form):
 _sizes = {}     # (workspace, checkpoint) bytes by what they follow from
 
 
+def _lies_as_saved(t, dtype, count, index):
+    """Whether ``t`` is as a contiguous tensor of these was when it was saved (and is where it was not replaced)."""
+    return t.dtype is dtype and t.numel() == count and t.get_device() == index and t.is_contiguous() and t.data_ptr() % 16 == 0
+
+
 class _Call:
     """What a call's forward and backward pass have in common: the DsbRecurrence (for ``x`` and ``gate`` as they are kept
     here, copied where their rows do not lie as the kernels need them) and the sizes that follow from it."""
-    __slots__ = ("shape", "ref", "lanes", "x", "gate", "sequences", "final_only", "sizes")
+    __slots__ = ("shape", "ref", "lanes", "x", "gate", "sequences", "final_only", "key", "sizes", "contiguous")
 
     def __init__(self, x, gate, sequences, sequence_rows, form, coupled, reverse, offsets, lengths, final_only=False):
         if sequences >= 1 << 31:
@@ -133,20 +138,20 @@ class _Call:
         self.lanes = lanes = 4 if together % 4 == 0 else 2 if together % 2 == 0 else 1
         self.x, x_stride = _rows(x, lanes)
         self.gate, gate_stride = _rows(gate, lanes if heads == d else 1)
-        self.sequences, self.final_only = sequences, final_only
+        self.sequences, self.final_only, self.contiguous = sequences, final_only, x_stride == d and gate_stride == heads
+        rows, dtype = x.numel() // d, _capi.DTYPES[x.dtype]
+        self.key = (rows, sequences, sequence_rows, d, heads, dtype, x_stride, gate_stride)
         self.shape = _capi.DsbRecurrence(
-            x.numel() // d, sequences, sequence_rows, d, heads, _capi.DTYPES[x.dtype], _capi.GATE_FORMS[form], 1 if coupled else 0,
-            1 if reverse else 0, x_stride, gate_stride, _capi.ptr(offsets), _capi.ptr(lengths))
+            rows, sequences, sequence_rows, d, heads, dtype, _capi.GATE_FORMS[form], 1 if coupled else 0, 1 if reverse else 0, x_stride,
+            gate_stride, _capi.ptr(offsets), _capi.ptr(lengths))
         self.ref = C.byref(self.shape)
 
     def find_sizes(self, lib):
-        s = self.shape
-        key = (s.rows, s.sequences, s.sequence_rows, s.channels, s.gate_heads, s.dtype, s.x_stride, s.gate_stride)
-        got = _sizes.get(key)
+        got = _sizes.get(self.key)
         if got is None:
             if len(_sizes) > 256:
                 _sizes.clear()
-            got = _sizes[key] = (lib.dsb_recurrence_workspace_bytes(self.ref), lib.dsb_recurrence_checkpoint_bytes(self.ref))
+            got = _sizes[self.key] = (lib.dsb_recurrence_workspace_bytes(self.ref), lib.dsb_recurrence_checkpoint_bytes(self.ref))
         self.sizes = got
         return got
 
@@ -167,9 +172,18 @@ class _Call:
         return h, last, checkpoints
 
     def as_handed_out(self, x, gate, state, checkpoints, borders, dev):
-        """(x, gate, state, checkpoints, borders, DsbRecurrence) of a backward pass.  Hooks on saved tensors (activation checkpointing,
-        offloading) hand out others than those that were saved: at other addresses, and laid out otherwise."""
-        s = self.shape
+        """(x, gate, state, checkpoints, borders, DsbRecurrence) of a backward pass.  Hooks on saved tensors (activation
+        checkpointing, offloading) hand out others than those that were saved: at other addresses, and laid out otherwise."""
+        s, index, dtype = self.shape, -1 if dev.index is None else dev.index, x.dtype
+        rows, sequences, sequence_rows, d, heads, code, _, _ = self.key
+        packed = sequence_rows == 0
+        if (self.contiguous and _capi.DTYPES.get(dtype) == code and _lies_as_saved(x, dtype, rows * d, index) and x.shape[-1] == d
+                and _lies_as_saved(gate, dtype, rows * heads, index)
+                and _lies_as_saved(checkpoints, torch.uint8, self.sizes[1], index)
+                and (state is None or _lies_as_saved(state, torch.float32, sequences * d, index))
+                and (borders is None or (_lies_as_saved(borders, torch.int32, sequences + packed, index)
+                                         and borders.data_ptr() == (s.offsets if packed else s.lengths)))):
+            return x, gate, state, checkpoints, borders, s      # the forward's descriptor says all of this
         for t, name, width in ((x, "x", s.channels), (gate, "gate", s.gate_heads)):
             _require(t, name, dev, x.dtype)
             if t.shape[-1] != width or t.numel() != s.rows * width or _capi.DTYPES.get(t.dtype) != s.dtype:
@@ -189,7 +203,6 @@ class _Call:
         shape = type(s).from_buffer_copy(s)
         shape.x_stride, shape.gate_stride = x_stride, gate_stride
         if borders is not None:
-            packed = s.sequence_rows == 0
             _require(borders, "offsets" if packed else "lengths", dev, torch.int32)
             if borders.numel() != self.sequences + packed:
                 raise RuntimeError("a hook handed out something else than was saved")
@@ -197,8 +210,8 @@ class _Call:
             shape.offsets, shape.lengths = (borders.data_ptr(), None) if packed else (None, borders.data_ptr())
         return x, gate, state, checkpoints, borders, shape
 
-    def run_backward(self, x, gate, state, checkpoints, borders, v_h, v_last, need):
-        lib, dev, d = _capi.lib(), (v_h if v_last is None else v_last).device, x.shape[-1]
+    def run_backward(self, x, gate, state, checkpoints, borders, v_h, v_last, need, dev):
+        lib, d = _capi.lib(), x.shape[-1]
         v_x = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
         v_gate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if need[1] else None
         x, gate, state, checkpoints, borders, shape = self.as_handed_out(x, gate, state, checkpoints, borders, dev)
@@ -240,8 +253,8 @@ class _GatedRecurrence(torch.autograd.Function):
         v_h, v_last = (None, grads[0]) if len(grads) == 1 else grads
         if v_h is None and v_last is None:
             return (None,) * 5
-        v = _on((v_h if v_last is None else v_last).device, ctx.call.run_backward, x, gate, state, checkpoints, borders, v_h, v_last,
-                ctx.needs_input_grad)
+        dev = (v_h if v_last is None else v_last).device
+        v = _on(dev, ctx.call.run_backward, x, gate, state, checkpoints, borders, v_h, v_last, ctx.needs_input_grad, dev)
         return (*v, None, None)
 
 
